@@ -57,6 +57,7 @@ enum lc_status {
 #define LC_DEV_BAD_BLOCK 0x1   /* block-table entry outside [0, num_blocks)            */
 #define LC_DEV_BAD_POS 0x2     /* position outside the block table or RoPE table       */
 #define LC_DEV_TIMEOUT 0x4     /* a pipeline wait exceeded its bound                    */
+#define LC_DEV_OUT_OF_BLOCKS 0x8 /* lc_step_tables: too few free pages for every request */
 
 const char *lc_status_string(int status);
 /* Maps a device status word (read back by the caller) to an lc_status code. */
@@ -296,6 +297,147 @@ int lc_gather_kv(void *k_out, void *v_out, const void *k_pool,
                  const int *block_tables, int table_stride,
                  const int *context_lens, int len_offset, int batch,
                  int max_context_len, int *dev_status, lc_stream_t stream);
+
+/* ------------------------------------------------------------------------- */
+/* A step's page bookkeeping on the GPU.                                      */
+/* ------------------------------------------------------------------------- */
+/* What lc_block_alloc and lc_kv_pool_prepare_step do on the host, from lengths
+ * that live on the device, so that a whole serving step (bookkeeping, layers,
+ * token selection) can be one CUDA graph without a host upload. The state is
+ * the caller's device memory: free_pages, a stack of free page numbers
+ * (int32 [num_blocks], entries [0, *free_count) are free, the last is handed
+ * out first; a stack filled with num_blocks - 1, ..., 1, 0 hands out pages in
+ * the order of a fresh lc_block_alloc), *free_count, and block_tables, int32
+ * [num_slots][table_stride], one row per sequence slot. Workspace: one word of
+ * lc_step_workspace_size() bytes, zeroed once (lc_paged_decode_workspace_init),
+ * left zero; calls that share it are ordered on one stream. */
+size_t lc_step_workspace_size(void);
+
+/* Request b of `batch` (at most 8192) adds new_lens[b] >= 0 tokens to the
+ * context_lens[b] cached ones of slot slots[b] (distinct; NULL: slot b).
+ *   - Pages to cover them come off the stack into the slot's table row. In
+ *     request order, a request gets all the pages it needs or none: the first
+ *     one for which the stack is too small and all later ones that need a page
+ *     go without (LC_DEV_OUT_OF_BLOCKS). free_pages itself is only read.
+ *   - step_tables (NULL: none), int32 [batch][step_stride]: the rows in request
+ *     order, -1 past the last page; what the attention calls take.
+ *   - Token rows in request order, request b's at row_starts[b] (int32
+ *     [batch + 1]): positions[r] and slot_map[r] = page * 16 + position % 16,
+ *     the token's place in a pool, or -1 for a request that went without.
+ *     Rows from row_starts[batch] up to max_tokens are padding (-1, -1);
+ *     tokens past max_tokens are left out (LC_DEV_BAD_POS).
+ *   - context_out[b]: the cached tokens after the step (unchanged for a request
+ *     that went without). *free_count_out: the free pages left.
+ * context_out may be context_lens and free_count_out may be free_count. A
+ * request with a negative length, a slot out of range or more tokens than its
+ * table row holds gets no rows and no pages (LC_DEV_BAD_POS; context_out is
+ * context_lens[b], or 0 where that or the slot was out of range). */
+int lc_step_tables(int *block_tables, int table_stride, int num_slots, const int *slots,
+                   const int *context_lens, const int *new_lens, int batch,
+                   const int *free_pages, const int *free_count, int64_t num_blocks,
+                   int *step_tables, int step_stride, int *positions, int *slot_map,
+                   int max_tokens, int *row_starts, int *context_out, int *free_count_out,
+                   void *workspace, size_t workspace_bytes, int *dev_status,
+                   lc_stream_t stream);
+
+/* Returns the pages of `count` finished requests (context_lens[i] cached tokens
+ * in slot slots[i]; NULL: slot i) to the stack, in request order and each one's
+ * last page first, as lc_block_alloc_release_seq does. The table rows are left
+ * as they are. free_count_out may be free_count. Pages beyond num_blocks on the
+ * stack are dropped (LC_DEV_BAD_BLOCK). */
+int lc_step_release(int *free_pages, const int *free_count, int64_t num_blocks,
+                    const int *block_tables, int table_stride, int num_slots,
+                    const int *slots, const int *context_lens, int count,
+                    int *free_count_out, void *workspace, size_t workspace_bytes,
+                    int *dev_status, lc_stream_t stream);
+
+/* ------------------------------------------------------------------------- */
+/* Per-head norm of q and k, RoPE and append by slot.                         */
+/* ------------------------------------------------------------------------- */
+/* For num_rows token rows of `qkv` ([q | k | v] as for lc_rope_append, only
+ * read), row r at position positions[r]:
+ *   u = x + bias;  y = u / sqrt(mean(u^2) + eps) * w per head of q and k
+ *   (w = q_norm or k_norm, bf16 [head_dim]);  rotate-half RoPE of y
+ * in fp32, rounded to bf16 once. The rotated q goes to q_out (rows q_out_stride
+ * apart; it may be the qkv rows themselves), k and v + bias to the pools at
+ * slot_map[r] = page * 16 + offset. Each bias and each norm weight may be NULL
+ * (none). slot_map[r] = -1: the row's k and v are not stored. positions[r] =
+ * -1: a padding row, nothing is read or written for it. A position outside the
+ * tables (LC_DEV_BAD_POS) leaves the row alone, a slot outside the pool
+ * (LC_DEV_BAD_BLOCK) its k and v. Rows may come from any mix of sequences, in
+ * any order. All pointers 16-byte aligned, strides multiples of 8. */
+int lc_qk_norm_rope_append(void *q_out, int64_t q_out_stride, const void *qkv,
+                           int64_t row_stride, int num_rows, const int *positions,
+                           const int *slot_map, const void *q_bias, const void *k_bias,
+                           const void *v_bias, const void *q_norm, const void *k_norm,
+                           float eps, const float *cos_cache, const float *sin_cache,
+                           int rope_rows, void *k_pool, void *v_pool, int64_t num_blocks,
+                           int num_layers, int layer, int num_q_heads, int num_kv_heads,
+                           int head_dim, int *dev_status, lc_stream_t stream);
+
+/* ------------------------------------------------------------------------- */
+/* The cache in 4 bits.                                                       */
+/* ------------------------------------------------------------------------- */
+/* kv_pool: uint8 [num_blocks][num_layers][num_kv_heads][lc_kv4_page_bytes], 16-byte
+ * aligned: per page and kv head K, then V, each as [16][head_dim / 2] code bytes
+ * (e2m1, even dim in the low nibble) followed by [16][head_dim / 16] scale bytes
+ * (e4m3, one per 16 dims): 4.5 bits per element, 9/32 of the bf16 pools. An
+ * element stands for e2m1 * e4m3 * k_scale (v_scale for V). A group of 16 dims
+ * with largest magnitude a gets the scale e4m3(a / (6 k_scale)) and the codes
+ * e2m1(x / (scale * k_scale)), both to nearest even from the fp32 values; a
+ * group with an infinity or NaN gets a NaN scale. k_scale and v_scale (2^-64 ..
+ * 2^64; the same in every call on a pool) move the scales into e4m3's range:
+ * groups with a largest magnitude between 0.1 and 2600 times the factor keep
+ * full precision; powers of two make the unpacked bf16 values exact. */
+size_t lc_kv4_page_bytes(int head_dim); /* 18 * head_dim; 0 if unsupported */
+
+/* lc_qk_norm_rope_append into a 4-bit pool. */
+int lc_qk_norm_rope_append_kv4(void *q_out, int64_t q_out_stride, const void *qkv,
+                               int64_t row_stride, int num_rows, const int *positions,
+                               const int *slot_map, const void *q_bias, const void *k_bias,
+                               const void *v_bias, const void *q_norm, const void *k_norm,
+                               float eps, const float *cos_cache, const float *sin_cache,
+                               int rope_rows, void *kv_pool, float k_scale, float v_scale,
+                               int64_t num_blocks, int num_layers, int layer,
+                               int num_q_heads, int num_kv_heads, int head_dim,
+                               int *dev_status, lc_stream_t stream);
+
+/* Unpacks each sequence's pages of one layer into bf16 pools of one layer: page
+ * j of sequence b becomes page b * P + j, P = ceil(max_context_len / 16), of
+ * k_out and v_out (bf16 [batch * P][1][num_kv_heads][16][head_dim]). Tokens past
+ * the sequence's n_b = context_lens[b] + len_offset in its last page are zeros;
+ * pages past it are left alone. lc_paged_prefill over these pools (num_layers
+ * 1, layer 0, table row b = b * P, b * P + 1, ...) is the attention of a prompt
+ * that continues a cached context. Table entries outside the pool give zeros
+ * (LC_DEV_BAD_BLOCK). max_context_len must not exceed a table row. */
+int lc_unpack_kv4(void *k_out, void *v_out, const void *kv_pool, int64_t num_blocks,
+                  int num_layers, int layer, int num_kv_heads, int head_dim,
+                  const int *block_tables, int table_stride, const int *context_lens,
+                  int len_offset, int batch, int max_context_len, float k_scale,
+                  float v_scale, int *dev_status, lc_stream_t stream);
+
+/* Workspace of lc_paged_decode_kv4 on the current device, as
+ * lc_paged_decode_workspace_size: zero it once (lc_paged_decode_workspace_init),
+ * and again after a status word with LC_DEV_TIMEOUT. */
+size_t lc_paged_decode_kv4_workspace_size(int batch, int num_q_heads, int num_kv_heads,
+                                          int head_dim, int tokens_per_seq);
+
+/* lc_paged_decode over a 4-bit pool, for the newest tokens_per_seq tokens of
+ * each sequence (1: a decode step; a few: drafted tokens checked at once). q and
+ * out rows: [batch * tokens_per_seq][Hq * head_dim]; row b * tokens_per_seq + i
+ * attends over the first n_b - (tokens_per_seq - 1 - i) tokens of sequence b,
+ * n_b = context_lens[b] + len_offset, all of them in the cache. A row without
+ * tokens gets zeros. K and V enter the products exactly as stored, the
+ * probabilities as fp16, sums are fp32. max_context_len (0: unknown) trims the
+ * grid for little work. Table entries outside the pool (LC_DEV_BAD_BLOCK) read
+ * as zeros. */
+int lc_paged_decode_kv4(void *out, int64_t out_stride, const void *q, int64_t q_stride,
+                        const void *kv_pool, int64_t num_blocks, int num_layers, int layer,
+                        int num_q_heads, int num_kv_heads, int head_dim,
+                        const int *block_tables, int table_stride, const int *context_lens,
+                        int len_offset, int batch, int tokens_per_seq, int max_context_len,
+                        float k_scale, float v_scale, float sm_scale, void *workspace,
+                        size_t workspace_bytes, int *dev_status, lc_stream_t stream);
 
 /* ------------------------------------------------------------------------- */
 /* Host-side mirror of the reference's Rust layer API (owning objects).       */

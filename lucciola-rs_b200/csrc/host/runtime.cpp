@@ -30,6 +30,7 @@ extern "C" const char *lc_status_string(int status) {
 extern "C" int lc_status_from_device_word(int word) {
     if (word & LC_DEV_TIMEOUT) return LC_ERR_DEVICE_TIMEOUT;
     if (word & (LC_DEV_BAD_BLOCK | LC_DEV_BAD_POS)) return LC_ERR_DEVICE_BOUNDS;
+    if (word & LC_DEV_OUT_OF_BLOCKS) return LC_ERR_OUT_OF_BLOCKS;
     return LC_OK;
 }
 

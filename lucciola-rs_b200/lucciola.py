@@ -57,6 +57,24 @@ SIGNATURES = {
                                 _i32, _vp, _i32, _vp, _i32, _i32, _i32, _f32, _vp, _vp]),
     "lc_gather_kv": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i32, _vp,
                             _i32, _i32, _i32, _vp, _vp]),
+    "lc_step_workspace_size": (_sz, []),
+    "lc_step_tables": (_i32, [_vp, _i32, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _i64, _vp, _i32,
+                              _vp, _vp, _i32, _vp, _vp, _vp, _vp, _sz, _vp, _vp]),
+    "lc_step_release": (_i32, [_vp, _vp, _i64, _vp, _i32, _i32, _vp, _vp, _i32, _vp, _vp, _sz,
+                               _vp, _vp]),
+    "lc_qk_norm_rope_append": (_i32, [_vp, _i64, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp,
+                                      _vp, _f32, _vp, _vp, _i32, _vp, _vp, _i64, _i32, _i32,
+                                      _i32, _i32, _i32, _vp, _vp]),
+    "lc_kv4_page_bytes": (_sz, [_i32]),
+    "lc_qk_norm_rope_append_kv4": (_i32, [_vp, _i64, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp,
+                                          _vp, _vp, _f32, _vp, _vp, _i32, _vp, _f32, _f32, _i64,
+                                          _i32, _i32, _i32, _i32, _i32, _vp, _vp]),
+    "lc_unpack_kv4": (_i32, [_vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i32, _vp, _i32,
+                             _i32, _i32, _f32, _f32, _vp, _vp]),
+    "lc_paged_decode_kv4_workspace_size": (_sz, [_i32, _i32, _i32, _i32, _i32]),
+    "lc_paged_decode_kv4": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _i32, _i32,
+                                   _vp, _i32, _vp, _i32, _i32, _i32, _i32, _f32, _f32, _f32, _vp,
+                                   _sz, _vp, _vp]),
     "lc_rope_table_host": (None, [_i32, _i32, _f32, _f32, _vp, _vp]),
     "lc_rope_cache_new": (_i32, [_i32, _i32, _f32, _f32, _vp, C.POINTER(_vp)]),
     "lc_rope_cache_cos": (_vp, [_vp]),
@@ -130,7 +148,7 @@ for _name, (_res, _args) in SIGNATURES.items():
     _fn.argtypes = _args
 
 LC_OK = 0
-LC_DEV_BAD_BLOCK, LC_DEV_BAD_POS, LC_DEV_TIMEOUT = 1, 2, 4
+LC_DEV_BAD_BLOCK, LC_DEV_BAD_POS, LC_DEV_TIMEOUT, LC_DEV_OUT_OF_BLOCKS = 1, 2, 4, 8
 
 
 class LucciolaError(RuntimeError):
@@ -313,6 +331,116 @@ def gather_kv(k_out, v_out, k_pool, v_pool, num_blocks, num_layers, layer, num_k
                            block_tables.stride(0), _p(context_lens), len_offset,
                            context_lens.shape[0], max_context_len, _p(dev_status),
                            _stream(stream)), "lc_gather_kv")
+
+
+# ------------------------------------------------ device-side step, 4-bit cache --
+
+def _nbytes(t):
+    return 0 if t is None else t.numel() * t.element_size()
+
+
+def alloc_step_workspace(device="cuda"):
+    """Zeroed workspace for step_tables / step_release."""
+    import torch
+    return torch.zeros(lib.lc_step_workspace_size(), dtype=torch.uint8, device=device)
+
+
+def step_tables(block_tables, context_lens, new_lens, free_pages, free_count, positions, slot_map,
+                row_starts, context_out, free_count_out, workspace, slots=None, step_tables=None,
+                dev_status=None, stream=None):
+    """A step's pages, table rows, positions and slot map from the requests' lengths.
+    All int32 device tensors; context_out may be context_lens, free_count_out free_count."""
+    check(lib.lc_step_tables(_p(block_tables), block_tables.stride(0), block_tables.shape[0],
+                             _p(slots), _p(context_lens), _p(new_lens), context_lens.shape[0],
+                             _p(free_pages), _p(free_count), free_pages.shape[0], _p(step_tables),
+                             0 if step_tables is None else step_tables.stride(0), _p(positions),
+                             _p(slot_map), positions.shape[0], _p(row_starts), _p(context_out),
+                             _p(free_count_out), _p(workspace), _nbytes(workspace),
+                             _p(dev_status), _stream(stream)), "lc_step_tables")
+
+
+def step_release(free_pages, free_count, block_tables, context_lens, free_count_out, workspace,
+                 slots=None, dev_status=None, stream=None):
+    """Returns the pages of finished requests to the free stack."""
+    check(lib.lc_step_release(_p(free_pages), _p(free_count), free_pages.shape[0],
+                              _p(block_tables), block_tables.stride(0), block_tables.shape[0],
+                              _p(slots), _p(context_lens), context_lens.shape[0],
+                              _p(free_count_out), _p(workspace), _nbytes(workspace),
+                              _p(dev_status), _stream(stream)), "lc_step_release")
+
+
+def qk_norm_rope_append(q_out, qkv, positions, slot_map, cos, sin, k_pool, v_pool, num_blocks,
+                        num_layers, layer, num_q_heads, num_kv_heads, head_dim, q_norm=None,
+                        k_norm=None, eps=1e-6, q_bias=None, k_bias=None, v_bias=None,
+                        dev_status=None, stream=None):
+    """Bias, RMS norm per q / k head, RoPE and append by slot, into bf16 pools."""
+    check(lib.lc_qk_norm_rope_append(
+        _p(q_out), q_out.stride(0), _p(qkv), qkv.stride(0), positions.shape[0], _p(positions),
+        _p(slot_map), _p(q_bias), _p(k_bias), _p(v_bias), _p(q_norm), _p(k_norm), eps, _p(cos),
+        _p(sin), cos.shape[0], _p(k_pool), _p(v_pool), num_blocks, num_layers, layer, num_q_heads,
+        num_kv_heads, head_dim, _p(dev_status), _stream(stream)), "lc_qk_norm_rope_append")
+
+
+def kv4_page_bytes(head_dim) -> int:
+    return lib.lc_kv4_page_bytes(head_dim)
+
+
+def alloc_kv4_pool(num_blocks, num_layers, num_kv_heads, head_dim, device="cuda"):
+    """Zeroed 4-bit pool: uint8 [num_blocks][num_layers][Hkv][page bytes]."""
+    import torch
+    nbytes = kv4_page_bytes(head_dim)
+    if nbytes == 0:
+        raise LucciolaError(2, "lc_kv4_page_bytes")
+    return torch.zeros(num_blocks, num_layers, num_kv_heads, nbytes, dtype=torch.uint8,
+                       device=device)
+
+
+def qk_norm_rope_append_kv4(q_out, qkv, positions, slot_map, cos, sin, kv_pool, num_blocks,
+                            num_layers, layer, num_q_heads, num_kv_heads, head_dim, k_scale=1.0,
+                            v_scale=1.0, q_norm=None, k_norm=None, eps=1e-6, q_bias=None,
+                            k_bias=None, v_bias=None, dev_status=None, stream=None):
+    """qk_norm_rope_append into a 4-bit pool."""
+    check(lib.lc_qk_norm_rope_append_kv4(
+        _p(q_out), q_out.stride(0), _p(qkv), qkv.stride(0), positions.shape[0], _p(positions),
+        _p(slot_map), _p(q_bias), _p(k_bias), _p(v_bias), _p(q_norm), _p(k_norm), eps, _p(cos),
+        _p(sin), cos.shape[0], _p(kv_pool), k_scale, v_scale, num_blocks, num_layers, layer,
+        num_q_heads, num_kv_heads, head_dim, _p(dev_status), _stream(stream)),
+        "lc_qk_norm_rope_append_kv4")
+
+
+def unpack_kv4(k_out, v_out, kv_pool, num_blocks, num_layers, layer, num_kv_heads, head_dim,
+               block_tables, context_lens, max_context_len, k_scale=1.0, v_scale=1.0,
+               len_offset=0, dev_status=None, stream=None):
+    """The sequences' 4-bit pages as bf16 pages [batch * P][1][Hkv][16][hd]."""
+    check(lib.lc_unpack_kv4(_p(k_out), _p(v_out), _p(kv_pool), num_blocks, num_layers, layer,
+                            num_kv_heads, head_dim, _p(block_tables), block_tables.stride(0),
+                            _p(context_lens), len_offset, context_lens.shape[0], max_context_len,
+                            k_scale, v_scale, _p(dev_status), _stream(stream)), "lc_unpack_kv4")
+
+
+def alloc_decode_kv4_workspace(batch, num_q_heads, num_kv_heads, head_dim, tokens_per_seq=1,
+                               device="cuda"):
+    """Zeroed workspace for paged_decode_kv4."""
+    import torch
+    n = lib.lc_paged_decode_kv4_workspace_size(batch, num_q_heads, num_kv_heads, head_dim,
+                                               tokens_per_seq)
+    return torch.zeros(n, dtype=torch.uint8, device=device)
+
+
+def paged_decode_kv4(out, q, kv_pool, num_blocks, num_layers, layer, num_q_heads, num_kv_heads,
+                     head_dim, block_tables, context_lens, max_context_len=0, tokens_per_seq=1,
+                     k_scale=1.0, v_scale=1.0, sm_scale=None, len_offset=0, workspace=None,
+                     dev_status=None, stream=None):
+    """Attention of each sequence's newest tokens_per_seq tokens over a 4-bit pool."""
+    if sm_scale is None:
+        sm_scale = 1.0 / math.sqrt(head_dim)
+    check(lib.lc_paged_decode_kv4(_p(out), out.stride(0), _p(q), q.stride(0), _p(kv_pool),
+                                  num_blocks, num_layers, layer, num_q_heads, num_kv_heads,
+                                  head_dim, _p(block_tables), block_tables.stride(0),
+                                  _p(context_lens), len_offset, context_lens.shape[0],
+                                  tokens_per_seq, max_context_len, k_scale, v_scale, sm_scale,
+                                  _p(workspace), _nbytes(workspace), _p(dev_status),
+                                  _stream(stream)), "lc_paged_decode_kv4")
 
 
 # ------------------------------------------------------------ host mirrors --
