@@ -2,7 +2,41 @@
 // paged cache (kv4.cuh). For query token i of T of sequence b, which holds n
 // tokens with them, and query head h of kv head h / (Hq / Hkv):
 //     out = softmax_t(q . k_t * sm_scale) . v_t    over t < n - (T - 1 - i)
+// in one pass: a running maximum m and sum l per query row, the output rescaled
+// when m rises.
+//
+// Split. The T * Hq/Hkv query rows of a kv head are the columns of its products,
+// kCols = 8 or 16 at a time; (sequence, kv head, slice of columns) is a segment.
+// The pages of all segments form one stream, cut evenly over a persistent grid:
+// every CTA moves the same bytes whatever the lengths are. A segment cut across
+// CTAs leaves (O, m, l) pieces in the workspace; the CTA that finishes it last
+// (arrival counter) joins them in the order of the stream, so the result does
+// not depend on timing.
+//
+// Inside a CTA the warps take groups of kGroup pages in turn. Each warp has its
+// own ring of stages and fills it itself: one bulk copy per page brings K and V
+// of the kv head (18 hd bytes, contiguous), counted on the stage's mbarrier, and
+// the block-table entries are read one group ahead. No barrier joins the warps
+// before the end of a chunk (a CTA's part of one segment).
+//
+// Products, mma.sync m16n8k16 with fp16 operands and fp32 sums:
+//     S^T[16 tokens x 8 columns] = K[16 x hd] . Q^T
+//     O^T[hd x 8 columns]       += V^T[hd x 16] . P^T
+// K and V unpack in registers, straight into the operand layout: e2m1 to fp16
+// is one conversion per pair, the scale one multiplication per pair, both exact
+// (kv4.cuh), so only p is rounded (to fp16, 2^-11) on its way into a product. q
+// is scaled to [1, 2) by a power of two per row, so that bf16 fits fp16.
+//  * K: a lane's operand elements are 4 dims per step of 2 tokens. The order of
+//    dims within the sum is free, so lane t of a quad takes the dims hd/4 * t ..
+//    and reads them as one 16-byte (8 at hd 64) load per token.
+//  * V: a lane holds hd/8 consecutive dims of 4 tokens and needs pairs of tokens
+//    per dim: two tokens' words are interleaved by nibbles first, then converted.
+//  * Row r of a 16-token tile is token pi(r): pi(2t) = t, pi(2t + 1) = 7 - t (and
+//    8 more for r >= 8). Any order does; this one spreads the 64-byte token rows
+//    over the banks for the K loads and the V loads alike.
+#include <algorithm>
 #include <climits>
+#include <cmath>
 
 #include "kv4.cuh"
 #include "lc_host.h"
@@ -10,7 +44,11 @@
 namespace lc {
 namespace {
 
-constexpr int kSimpleWarps = 4;
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+constexpr int kGroup = 2;             // pages of one warp at a time
+constexpr int kMinPages = kWarps * kGroup;  // pages per CTA at least
+constexpr float kLazy = 8.f;  // p may reach 2^8 before O and l are rescaled
 
 struct DecodeKv4Params {
     bf16 *out;
@@ -24,72 +62,729 @@ struct DecodeKv4Params {
     int table_stride;
     const int *ctx_lens;
     int len_offset, batch, tokens;
-    float scale_log2, v_scale;
+    int group;        // query heads per kv head
+    int cols;         // tokens * group
+    int slices;       // ceil(cols / kCols)
+    int seg_per_seq;  // num_kv_heads * slices
+    float scale_log2;  // |sm_scale| * k_scale * log2(e)
+    uint32_t q_sign;   // sign of sm_scale, on both halves of an fp16 pair
+    float v_scale;
+    int pdl_mode;
+    int *ws_cnt;    // [batch * seg_per_seq] arrivals
+    float *ws_ml;   // [pieces][2][kCols] m, l
+    float *ws_o;    // [pieces][kCols][hd]
     int *status;
 };
 
-template <int HD>
-__global__ void __launch_bounds__(kSimpleWarps * 32) decode_kv4_simple_kernel(DecodeKv4Params p) {
-    constexpr int kDims = HD / 32;
-    __shared__ float s_m[kSimpleWarps], s_l[kSimpleWarps], s_o[kSimpleWarps][HD];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int row = blockIdx.x, h = blockIdx.y, b = row / p.tokens;
-    const int kvh = h / (p.num_q_heads / p.num_kv_heads);
-    int n = p.ctx_lens[b] + p.len_offset;
-    if (n > p.table_stride * kBlockSize) {
-        if (lane == 0) set_status(p.status, LC_DEV_BAD_POS);
-        n = p.table_stride * kBlockSize;
+template <int HD, int NT>
+struct Cfg {
+    static constexpr int kCols = 8 * NT;
+    static constexpr int kPage = 18 * HD;  // K and V of one kv head
+    static constexpr int kStage = kGroup * kPage;
+    static constexpr int kStages = HD == 64 ? 4 : 2;
+    static constexpr int kRow = HD + 4;  // floats between columns of a merge slot
+    static constexpr int kSlots = kWarps / 2;
+    static constexpr int kRing = kWarps * kStages * kStage;
+    static constexpr int kSmem = kRing + kSlots * kCols * kRow * 4;
+    static constexpr int kCtasPerSm = NT == 1 ? 2 : 1;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+    const __half2 r = __hmul2(*reinterpret_cast<__half2 *>(&a), *reinterpret_cast<__half2 *>(&b));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                        uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
+        "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes,
+                                          uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+        ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ int tokens_of(const DecodeKv4Params &p, int b, bool report) {
+    const long long n = (long long)__ldg(p.ctx_lens + b) + p.len_offset;
+    const int cap = p.table_stride * kBlockSize;
+    if (n > cap) {
+        if (report) set_status(p.status, LC_DEV_BAD_POS);
+        return cap;
     }
-    n -= p.tokens - 1 - row % p.tokens;
-    float q[kDims], o[kDims] = {}, m = -INFINITY, l = 0.f;
-    for (int i = 0; i < kDims; ++i)
-        q[i] = __bfloat162float(p.q[row * p.q_stride + h * HD + lane * kDims + i]);
-    for (int t = warp; t < n; t += kSimpleWarps) {
-        const int phys = p.tables[(int64_t)b * p.table_stride + t / kBlockSize];
-        const bool ok = phys >= 0 && phys < p.num_blocks;
-        if (!ok && lane == 0) set_status(p.status, LC_DEV_BAD_BLOCK);
-        const uint8_t *page = p.kv_pool + kv4_offset(ok ? phys : 0, p.layer, kvh, p.num_layers,
-                                                     p.num_kv_heads, HD);
-        float kv[2][kDims];
-        for (int half = 0; half < 2; ++half) {
-            const uint8_t *src = page + half * kv4_half_bytes(HD);
-            const int d0 = lane * kDims, tt = t % kBlockSize;
-            const float s = e4m3_to_float(src[kv4_code_bytes(HD) + tt * (HD / 16) + d0 / 16]);
-            const uint32_t w = reinterpret_cast<const uint32_t *>(src)[(tt * (HD / 2) + d0 / 2) / 4]
-                               >> (d0 / 2 % 4 * 8);
-            uint32_t hh[4];
-            e2m1x8_to_half(w, hh);
-            for (int i = 0; i < kDims; ++i) {
-                const __half2 v = *reinterpret_cast<__half2 *>(&hh[i / 2]);
-                kv[half][i] = ok ? (i & 1 ? __high2float(v) : __low2float(v)) * s : 0.f;
+    return n < 0 ? 0 : (int)n;
+}
+__device__ __forceinline__ int pages_of(int tokens) {
+    return (tokens + kBlockSize - 1) / kBlockSize;
+}
+
+// Where a walk over a CTA's range of the page stream stands: the chunk (b, seg)
+// pages [p0, p0 + take), its sequence's tokens and the stream index of its start.
+struct Walk {
+    int b, seg, p0, take, n;
+    long long at;  // stream index of page p0
+    int next_page;  // page of (b, seg) that the next chunk starts with
+
+    __device__ __forceinline__ void start(const DecodeKv4Params &p, long long first, int b0,
+                                          long long before_b0) {
+        b = b0;
+        n = tokens_of(p, b, false);
+        const long long off = first - before_b0;
+        const int pages = pages_of(n);
+        seg = pages ? (int)(off / pages) : 0;
+        next_page = pages ? (int)(off - (long long)seg * pages) : 0;
+        at = first;
+        p0 = take = 0;
+    }
+    // Moves to the next chunk of [.., end); false when there is none.
+    __device__ __forceinline__ bool next(const DecodeKv4Params &p, long long end) {
+        at += take;
+        if (at >= end) return false;
+        int pages = pages_of(n);
+        while (next_page >= pages) {  // the segment is done (or the sequence is empty)
+            next_page = 0;
+            if (pages == 0 || ++seg == p.seg_per_seq) {
+                seg = 0;
+                n = tokens_of(p, ++b, false);
+                pages = pages_of(n);
             }
         }
-        float x = 0.f;
-        for (int i = 0; i < kDims; ++i) x += q[i] * kv[0][i];
-        for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-        x *= p.scale_log2;
-        const float m2 = fmaxf(m, x);
-        const float base = m2 == -INFINITY ? 0.f : m2;
-        const float f = exp2f(m - base), e = exp2f(x - base);
-        l = l * f + e;
-        for (int i = 0; i < kDims; ++i) o[i] = o[i] * f + e * kv[1][i];
-        m = m2;
+        p0 = next_page;
+        take = (int)min((long long)(pages - p0), end - at);
+        next_page = p0 + take;
+        return true;
     }
-    if (lane == 0) s_m[warp] = m, s_l[warp] = l;
-    for (int i = 0; i < kDims; ++i) s_o[warp][lane * kDims + i] = o[i];
-    __syncthreads();
-    for (int d = threadIdx.x; d < HD; d += kSimpleWarps * 32) {
-        float mm = -INFINITY, ll = 0.f, oo = 0.f;
-        for (int w = 0; w < kSimpleWarps; ++w) mm = fmaxf(mm, s_m[w]);
-        const float base = mm == -INFINITY ? 0.f : mm;
-        for (int w = 0; w < kSimpleWarps; ++w) {
-            const float f = exp2f(s_m[w] - base);
-            ll += s_l[w] * f;
-            oo += s_o[w][d] * f;
+};
+
+// The groups of one warp, in stream order: group k of a chunk is warp k % kWarps's.
+struct GroupWalk {
+    Walk w;
+    int page, np;  // first page and pages of the group
+    int base;      // next group's first page within the chunk
+    bool more;
+
+    __device__ __forceinline__ bool next(const DecodeKv4Params &p, long long end, int warp) {
+        while (more) {
+            if (base < w.take) {
+                page = w.p0 + base;
+                np = min(kGroup, w.take - base);
+                base += kGroup * kWarps;
+                return true;
+            }
+            more = w.next(p, end);
+            base = warp * kGroup;
         }
-        p.out[row * p.out_stride + h * HD + d] =
-            __float2bfloat16(ll == 0.f ? 0.f : oo / ll * p.v_scale);
+        return false;
     }
+};
+
+template <int HD, int NT>
+__global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
+    decode_kv4_kernel(const DecodeKv4Params p) {
+    using C = Cfg<HD, NT>;
+    constexpr int kCols = C::kCols;
+    constexpr int kSteps = HD / 16;   // k-steps of S, m-tiles of O
+    constexpr int kWords = HD / 32;   // code words per token and lane (K)
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ __align__(8) uint64_t bars[kWarps][C::kStages];
+    __shared__ float s_m[kWarps][kCols], s_l[kWarps][kCols];
+    __shared__ long long s_sum[kWarps];
+    __shared__ long long s_before;
+    __shared__ int s_b0, s_last, s_abort;
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int g = lane >> 2, t = lane & 3;
+    if (p.pdl_mode > 0) {
+        griddep_launch_dependents();
+        if (p.pdl_mode == 1) griddep_wait();
+    }
+    if (lane < C::kStages) mbar_init(&bars[warp][lane], 1);
+    if (tid == 0) s_abort = 0;
+    fence_barrier_init();
+
+    // ---- the stream: its length, this CTA's range, the sequence it starts in
+    const int per = (p.batch + kThreads - 1) / kThreads;
+    const int q0 = min(p.batch, tid * per), q1 = min(p.batch, q0 + per);
+    long long mine = 0;
+    for (int b = q0; b < q1; ++b) mine += pages_of(tokens_of(p, b, blockIdx.x == 0));
+    mine *= p.seg_per_seq;
+    long long upto = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const long long u = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += u;
+    }
+    if (lane == 31) s_sum[warp] = upto;
+    __syncthreads();
+    long long total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) upto += s_sum[w];
+        total += s_sum[w];
+    }
+    const int ctas = (int)max(1ll, min((long long)gridDim.x, (total + kMinPages - 1) / kMinPages));
+    const int cta = blockIdx.x;
+    const long long first = cta < ctas ? total * cta / ctas : total;
+    const long long end = cta < ctas ? total * (cta + 1) / ctas : total;
+    if (first < end && upto - mine <= first && first < upto) {
+        long long before = upto - mine;
+        int b = q0;
+        for (;; ++b) {
+            const long long k = (long long)pages_of(tokens_of(p, b, false)) * p.seg_per_seq;
+            if (first < before + k) break;
+            before += k;
+        }
+        s_b0 = b;
+        s_before = before;
+    }
+    __syncthreads();
+    if (p.pdl_mode == 2) griddep_wait();
+
+    // ---- rows of sequences without tokens are zeros
+    for (int b = cta; b < p.batch; b += gridDim.x) {
+        if (tokens_of(p, b, false) > 0) continue;
+        const int width = p.num_q_heads * HD;
+        for (int i = tid; i < p.tokens * width; i += kThreads)
+            p.out[((int64_t)b * p.tokens + i / width) * p.out_stride + i % width] =
+                __float2bfloat16(0.f);
+    }
+    if (first >= end) return;
+
+    // ---- loads
+    uint8_t *ring = smem + warp * C::kStages * C::kStage;
+    const uint32_t ring_addr = smem_u32(ring);
+    GroupWalk gw;
+    gw.w.start(p, first, s_b0, s_before);
+    gw.more = gw.w.next(p, end);
+    gw.base = warp * kGroup;
+    int phys = 0;
+    auto look_up = [&]() {  // block-table entries of the group that is loaded next
+        if (lane < gw.np) phys = __ldg(p.tables + (int64_t)gw.w.b * p.table_stride + gw.page + lane);
+    };
+    bool pending = gw.next(p, end, warp);
+    if (pending) look_up();
+    uint32_t issued = 0;
+    auto issue = [&]() {
+        if (!pending) return;
+        const int stage = issued % C::kStages;
+        uint64_t *bar = &bars[warp][stage];
+        const bool bad = lane < gw.np && (phys < 0 || phys >= p.num_blocks);
+        const uint32_t bads = __ballot_sync(0xffffffffu, bad);
+        if (bads) {  // a table entry outside the pool reads as zeros
+            if (bad) set_status(p.status, LC_DEV_BAD_BLOCK);
+#pragma unroll
+            for (int k = 0; k < kGroup; ++k)
+                if (bads >> k & 1)
+                    for (int i = lane; i < C::kPage / 16; i += 32)
+                        reinterpret_cast<uint4 *>(ring + stage * C::kStage + k * C::kPage)[i] =
+                            make_uint4(0, 0, 0, 0);
+            // these stores before the copies that fill the stage later
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+        }
+        if (lane == 0) mbar_arrive_expect_tx(bar, (gw.np - __popc(bads)) * C::kPage);
+        __syncwarp();
+        if (lane < gw.np && !bad)
+            bulk_load(ring_addr + stage * C::kStage + lane * C::kPage,
+                      p.kv_pool + kv4_offset(phys, p.layer, gw.w.seg / p.slices, p.num_layers,
+                                             p.num_kv_heads, HD),
+                      C::kPage, bar);
+        ++issued;
+        pending = gw.next(p, end, warp);
+        if (pending) look_up();
+    };
+#pragma unroll
+    for (int s = 0; s < C::kStages; ++s) issue();
+
+    // ---- chunks
+    const int pi0 = g & 1 ? 7 - (g >> 1) : g >> 1;  // token of tile row g
+    uint32_t used = 0;
+    Walk cw;
+    cw.start(p, first, s_b0, s_before);
+    while (cw.next(p, end)) {
+        const int kvh = cw.seg / p.slices, col0 = (cw.seg - kvh * p.slices) * kCols;
+        const int ncols = min(kCols, p.cols - col0);
+
+        // q: column c of the slice is query row b * tokens + c / group, head c % group
+        uint32_t qf[NT][kSteps][2];
+        float f[NT][2];
+        int lim[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int c = nt * 8 + g;
+            float fc = 0.f;
+            uint4 raw[HD / 32];
+            if (c < ncols) {
+                const int i = (col0 + c) / p.group, h = (col0 + c) - i * p.group;
+                const bf16 *src = p.q + ((int64_t)cw.b * p.tokens + i) * p.q_stride +
+                                  (int64_t)(kvh * p.group + h) * HD + t * (HD / 4);
+#pragma unroll
+                for (int k = 0; k < HD / 32; ++k) raw[k] = __ldg(reinterpret_cast<const uint4 *>(src) + k);
+            } else {
+#pragma unroll
+                for (int k = 0; k < HD / 32; ++k) raw[k] = make_uint4(0, 0, 0, 0);
+            }
+            const uint32_t *r = reinterpret_cast<const uint32_t *>(raw);
+            uint32_t top = 0;  // largest magnitude, as bf16 bits
+#pragma unroll
+            for (int k = 0; k < HD / 8; ++k)
+                top = max(top, max(r[k] & 0x7fffu, (r[k] >> 16) & 0x7fffu));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int e = top ? (int)(top >> 7) - 127 : 0;
+            const float down = ldexpf(1.f, -e);
+            fc = p.scale_log2 * ldexpf(1.f, e);
+#pragma unroll
+            for (int k = 0; k < HD / 8; ++k) {
+                const float lo = __uint_as_float(r[k] << 16) * down;
+                const float hi = __uint_as_float(r[k] & 0xffff0000u) * down;
+                const __half2 v = __floats2half2_rn(lo, hi);
+                qf[nt][k / 2][k & 1] = *reinterpret_cast<const uint32_t *>(&v) ^ p.q_sign;
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                f[nt][k] = __shfl_sync(0xffffffffu, fc, (2 * t + k) * 4);
+                const int cc = col0 + nt * 8 + 2 * t + k;
+                lim[nt][k] = cw.n - (p.tokens - 1 - min(cc, p.cols - 1) / p.group);
+            }
+        }
+        // tokens that every column sees
+        const int all = cw.n - (p.tokens - 1 - col0 / p.group);
+
+        float o[kSteps][NT][4];
+        float m[NT][2], l[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[j][nt][k] = 0.f;
+        }
+
+        for (int base = warp * kGroup; base < cw.take; base += kGroup * kWarps) {
+            const int np = min(kGroup, cw.take - base);
+            const int tok0 = (cw.p0 + base) * kBlockSize;
+            const int stage = used % C::kStages;
+            uint64_t *bar = &bars[warp][stage];
+            if (!mbar_wait_bounded(bar, used / C::kStages & 1, &s_abort, p.status))
+                mbar_wait_drain(bar, used / C::kStages & 1);
+            __syncwarp();
+            const uint8_t *st = ring + stage * C::kStage;
+
+            // S^T = K . Q^T
+            float s[kGroup][NT][4];
+#pragma unroll
+            for (int pg = 0; pg < kGroup; ++pg) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) s[pg][nt][k] = pg < np ? 0.f : -INFINITY;
+                if (pg >= np) continue;
+                const uint8_t *kp = st + pg * C::kPage;
+                uint32_t wa[kWords], wb[kWords], sa[2], sb[2];
+                if constexpr (HD == 128) {
+                    const uint4 a = *reinterpret_cast<const uint4 *>(kp + pi0 * 64 + t * 16);
+                    const uint4 b = *reinterpret_cast<const uint4 *>(kp + (pi0 + 8) * 64 + t * 16);
+                    wa[0] = a.x, wa[1] = a.y, wa[2] = a.z, wa[3] = a.w;
+                    wb[0] = b.x, wb[1] = b.y, wb[2] = b.z, wb[3] = b.w;
+                    const uint8_t *sc = kp + kv4_code_bytes(HD) + pi0 * 8 + t * 2;
+                    const uint32_t ha = e4m3x2_to_half(*reinterpret_cast<const uint16_t *>(sc));
+                    const uint32_t hb = e4m3x2_to_half(*reinterpret_cast<const uint16_t *>(sc + 64));
+                    sa[0] = __byte_perm(ha, 0, 0x1010), sa[1] = __byte_perm(ha, 0, 0x3232);
+                    sb[0] = __byte_perm(hb, 0, 0x1010), sb[1] = __byte_perm(hb, 0, 0x3232);
+                } else {
+                    const uint2 a = *reinterpret_cast<const uint2 *>(kp + pi0 * 32 + t * 8);
+                    const uint2 b = *reinterpret_cast<const uint2 *>(kp + (pi0 + 8) * 32 + t * 8);
+                    wa[0] = a.x, wa[1] = a.y;
+                    wb[0] = b.x, wb[1] = b.y;
+                    const uint8_t *sc = kp + kv4_code_bytes(HD) + pi0 * 4 + t;
+                    const uint32_t h = e4m3x2_to_half(sc[0] | sc[32] << 8);
+                    sa[0] = __byte_perm(h, 0, 0x1010);
+                    sb[0] = __byte_perm(h, 0, 0x3232);
+                }
+#pragma unroll
+                for (int w = 0; w < kWords; ++w) {
+                    uint32_t ha[4], hb[4];
+                    e2m1x8_to_half(wa[w], ha);
+                    e2m1x8_to_half(wb[w], hb);
+                    const uint32_t fa = sa[w / 2], fb = sb[w / 2];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const uint32_t a0 = hmul2(ha[2 * k], fa), a2 = hmul2(ha[2 * k + 1], fa);
+                        const uint32_t a1 = hmul2(hb[2 * k], fb), a3 = hmul2(hb[2 * k + 1], fb);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+                            mma_f16(s[pg][nt], a0, a1, a2, a3, qf[nt][2 * w + k][0],
+                                    qf[nt][2 * w + k][1]);
+                    }
+                }
+            }
+            const bool tail = tok0 + np * kBlockSize > all;
+            if (tail) {
+#pragma unroll
+                for (int pg = 0; pg < kGroup; ++pg)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (tok0 + pg * kBlockSize + pi0 + (k >> 1) * 8 >= lim[nt][k & 1])
+                                s[pg][nt][k] = -INFINITY;
+            }
+
+            // running maximum: raised only where some p would pass 2^kLazy
+            bool raise = false;
+            float top[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    float x = fmaxf(s[0][nt][k], s[0][nt][k + 2]);
+#pragma unroll
+                    for (int pg = 1; pg < kGroup; ++pg)
+                        x = fmaxf(x, fmaxf(s[pg][nt][k], s[pg][nt][k + 2]));
+                    top[nt][k] = x == -INFINITY ? x : x * f[nt][k];
+                    raise |= top[nt][k] > m[nt][k] + kLazy;
+                }
+            if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        float x = top[nt][k];
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1)
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                        x = fmaxf(x, m[nt][k]);
+                        const float r = m[nt][k] == -INFINITY ? 0.f : ex2(m[nt][k] - x);
+                        m[nt][k] = x;
+                        l[nt][k] *= r;
+#pragma unroll
+                        for (int j = 0; j < kSteps; ++j) {
+                            o[j][nt][k] *= r;
+                            o[j][nt][k + 2] *= r;
+                        }
+                    }
+            }
+            uint32_t pf[kGroup][NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const float b0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0];
+                const float b1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+#pragma unroll
+                for (int pg = 0; pg < kGroup; ++pg)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        // a masked score stays -inf whatever the factor is
+                        const float x0 = s[pg][nt][2 * k], x1 = s[pg][nt][2 * k + 1];
+                        const float p0 = x0 == -INFINITY ? 0.f : ex2(fmaf(x0, f[nt][0], -b0));
+                        const float p1 = x1 == -INFINITY ? 0.f : ex2(fmaf(x1, f[nt][1], -b1));
+                        l[nt][0] += p0;
+                        l[nt][1] += p1;
+                        const __half2 v = __floats2half2_rn(p0, p1);
+                        pf[pg][nt][k] = movmatrix_trans(*reinterpret_cast<const uint32_t *>(&v));
+                    }
+            }
+
+            // O^T += V^T . P^T
+#pragma unroll
+            for (int pg = 0; pg < kGroup; ++pg) {
+                if (pg >= np) continue;
+                const uint8_t *vp = st + pg * C::kPage + kv4_half_bytes(HD);
+                const uint8_t *sc = vp + kv4_code_bytes(HD);
+                constexpr int kRowBytes = HD / 2, kRowScales = HD / 16;
+                const int sg = g * (HD / 8) / kKv4Group;  // scale of this lane's dims
+                uint32_t s01 = sc[t * kRowScales + sg] | sc[(7 - t) * kRowScales + sg] << 8;
+                uint32_t s23 = sc[(8 + t) * kRowScales + sg] | sc[(15 - t) * kRowScales + sg] << 8;
+                if (tail) {
+                    // tokens past the end hold anything: their scales become zero
+                    const int left = cw.n - tok0 - pg * kBlockSize;
+                    if (t >= left) s01 &= 0xff00u;
+                    if (7 - t >= left) s01 &= 0x00ffu;
+                    if (8 + t >= left) s23 &= 0xff00u;
+                    if (15 - t >= left) s23 &= 0x00ffu;
+                    if (p.tokens > 1) {
+                        // Of the last tokens, which not every column sees, a NaN scale must
+                        // reach the columns that see it only, not as 0 * NaN the others.
+                        const int common = all - tok0 - pg * kBlockSize;
+                        uint32_t nan = 0;  // by token of the page
+                        auto drop = [&](uint32_t &sc2, int sh, int tok) {
+                            if ((sc2 >> sh & 0x7fu) == kKv4NanScale && tok >= common) {
+                                sc2 &= ~(0xffu << sh);
+                                nan |= 1u << tok;
+                            }
+                        };
+                        drop(s01, 0, t);
+                        drop(s01, 8, 7 - t);
+                        drop(s23, 0, 8 + t);
+                        drop(s23, 8, 15 - t);
+                        nan |= __shfl_xor_sync(0xffffffffu, nan, 1);
+                        nan |= __shfl_xor_sync(0xffffffffu, nan, 2);
+                        if (nan)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int k = 0; k < 2; ++k)
+                                    if (lim[nt][k] - tok0 - pg * kBlockSize > __ffs(nan) - 1)
+#pragma unroll
+                                        for (int j = 0; j < kSteps; ++j)
+                                            o[j][nt][k] = o[j][nt][k + 2] = NAN;
+                    }
+                }
+                const uint32_t h01 = e4m3x2_to_half(s01), h23 = e4m3x2_to_half(s23);
+                uint32_t v[4][HD / 64];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = (i & 1 ? 7 - t : t) + (i >> 1) * 8;
+                    if constexpr (HD == 128) {
+                        const uint2 x = *reinterpret_cast<const uint2 *>(vp + row * kRowBytes + g * 8);
+                        v[i][0] = x.x, v[i][1] = x.y;
+                    } else {
+                        v[i][0] = *reinterpret_cast<const uint32_t *>(vp + row * kRowBytes + g * 4);
+                    }
+                }
+#pragma unroll
+                for (int w = 0; w < HD / 64; ++w) {
+                    constexpr uint32_t kLow = 0x0f0f0f0fu;
+                    uint32_t e01[4], d01[4], e23[4], d23[4];  // even and odd dims
+                    e2m1x8_to_half((v[0][w] & kLow) | (v[1][w] << 4 & ~kLow), e01);
+                    e2m1x8_to_half((v[0][w] >> 4 & kLow) | (v[1][w] & ~kLow), d01);
+                    e2m1x8_to_half((v[2][w] & kLow) | (v[3][w] << 4 & ~kLow), e23);
+                    e2m1x8_to_half((v[2][w] >> 4 & kLow) | (v[3][w] & ~kLow), d23);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t a0 = hmul2(e01[k], h01), a1 = hmul2(d01[k], h01);
+                        const uint32_t a2 = hmul2(e23[k], h23), a3 = hmul2(d23[k], h23);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+                            mma_f16(o[4 * w + k][nt], a0, a1, a2, a3, pf[pg][nt][0], pf[pg][nt][1]);
+                    }
+                }
+            }
+            __syncwarp();
+            ++used;
+            issue();
+        }
+
+        // ---- the chunk's end: join the warps
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) l[nt][k] += __shfl_xor_sync(0xffffffffu, l[nt][k], d);
+                if (g == 0) {
+                    s_m[warp][nt * 8 + 2 * t + k] = m[nt][k];
+                    s_l[warp][nt * 8 + 2 * t + k] = l[nt][k];
+                }
+            }
+        __syncthreads();
+        float *slots = reinterpret_cast<float *>(smem + C::kRing);
+        float *slot = slots + (warp % C::kSlots) * kCols * C::kRow;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w][nt * 8 + 2 * t + k]);
+                const float r = m[nt][k] == -INFINITY ? 0.f : ex2(m[nt][k] - top);
+#pragma unroll
+                for (int j = 0; j < kSteps; ++j) {
+                    // a column that saw nothing here adds nothing, whatever o holds
+                    o[j][nt][k] = m[nt][k] == -INFINITY ? 0.f : o[j][nt][k] * r;
+                    o[j][nt][k + 2] = m[nt][k] == -INFINITY ? 0.f : o[j][nt][k + 2] * r;
+                }
+            }
+        auto each = [&](auto &&fn) {  // 4 consecutive dims of one column at a time
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int j = 0; j < kSteps; j += 2)
+                        fn(reinterpret_cast<float4 *>(slot + (nt * 8 + 2 * t + k) * C::kRow +
+                                                      g * (HD / 8) + 2 * j),
+                           o[j][nt][k], o[j][nt][k + 2], o[j + 1][nt][k], o[j + 1][nt][k + 2]);
+        };
+        if (warp >= C::kSlots)
+            each([](float4 *d, float a, float b, float c, float e) { *d = make_float4(a, b, c, e); });
+        __syncthreads();
+        if (warp < C::kSlots)
+            each([](float4 *d, float a, float b, float c, float e) {
+                const float4 x = *d;
+                *d = make_float4(x.x + a, x.y + b, x.z + c, x.w + e);
+            });
+        __syncthreads();
+
+        const long long seg = (long long)cw.b * p.seg_per_seq + cw.seg;
+        const int pages = pages_of(cw.n);
+        const bool whole = cw.take == pages;
+        // CTA c starts at total * c / ctas; CTAs of the segment's first and last page
+        auto owner = [&](long long x) {
+            int c = (int)min((long long)ctas - 1, x * ctas / total);
+            while (c + 1 < ctas && total * (c + 1) / ctas <= x) ++c;
+            while (total * c / ctas > x) --c;
+            return c;
+        };
+        const long long seg_at = cw.at - cw.p0;
+        constexpr int kQuads = kCols * HD / 4;
+        constexpr int kTurns = kQuads / kThreads > 0 ? kQuads / kThreads : 1;
+        float4 acc[kTurns];
+        float cm[kTurns], cl[kTurns];
+#pragma unroll
+        for (int u = 0; u < kTurns; ++u) {
+            const int i = tid + u * kThreads;
+            if (i >= kQuads) break;
+            const int c = i / (HD / 4), d = i % (HD / 4) * 4;
+            float top = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w][c]);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w)
+                sum += s_m[w][c] == -INFINITY ? 0.f : s_l[w][c] * ex2(s_m[w][c] - top);
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < C::kSlots; ++k) {
+                const float4 x = *reinterpret_cast<const float4 *>(slots + (k * kCols + c) * C::kRow + d);
+                a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
+            }
+            acc[u] = a, cm[u] = top, cl[u] = sum;
+        }
+        if (!whole) {
+            float *po = p.ws_o + (seg + cta) * kCols * HD;
+            float *pml = p.ws_ml + (seg + cta) * 2 * kCols;
+#pragma unroll
+            for (int u = 0; u < kTurns; ++u) {
+                const int i = tid + u * kThreads;
+                if (i >= kQuads) break;
+                reinterpret_cast<float4 *>(po)[i] = acc[u];
+                if (i % (HD / 4) == 0) {
+                    pml[i / (HD / 4)] = cm[u];
+                    pml[kCols + i / (HD / 4)] = cl[u];
+                }
+            }
+            __threadfence();
+            __syncthreads();
+            const int c0 = owner(seg_at), pieces = owner(seg_at + pages - 1) - c0 + 1;
+            if (tid == 0) {
+                s_last = atomicAdd(p.ws_cnt + seg, 1) == pieces - 1;
+                if (s_last) p.ws_cnt[seg] = 0;  // ready for the next call
+            }
+            __syncthreads();
+            if (!s_last) continue;
+            __threadfence();
+            const float *bo = p.ws_o + (seg + c0) * kCols * HD;
+            const float *bml = p.ws_ml + (seg + c0) * 2 * kCols;
+#pragma unroll
+            for (int u = 0; u < kTurns; ++u) {
+                const int i = tid + u * kThreads;
+                if (i >= kQuads) break;
+                const int c = i / (HD / 4);
+                float top = -INFINITY;
+                for (int k = 0; k < pieces; ++k) top = fmaxf(top, __ldcg(bml + k * 2 * kCols + c));
+                float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+                float sum = 0.f;
+#pragma unroll 4
+                for (int k = 0; k < pieces; ++k) {
+                    const float pm = __ldcg(bml + k * 2 * kCols + c);
+                    const float pl = __ldcg(bml + k * 2 * kCols + kCols + c);
+                    const float4 x = __ldcg(reinterpret_cast<const float4 *>(bo + (int64_t)k * kCols * HD) + i);
+                    const float r = pm == -INFINITY ? 0.f : ex2(pm - top);
+                    sum += pl * r;
+                    a.x += x.x * r, a.y += x.y * r, a.z += x.z * r, a.w += x.w * r;
+                }
+                acc[u] = a, cl[u] = sum;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kTurns; ++u) {
+            const int i = tid + u * kThreads;
+            if (i >= kQuads) break;
+            const int c = i / (HD / 4), d = i % (HD / 4) * 4;
+            if (c >= ncols) continue;
+            const int qi = (col0 + c) / p.group, h = col0 + c - qi * p.group;
+            // a row without tokens gets zeros
+            const float r = cl[u] == 0.f ? 0.f : p.v_scale / cl[u];
+            bf16 *dst = p.out + ((int64_t)cw.b * p.tokens + qi) * p.out_stride +
+                        (int64_t)(kvh * p.group + h) * HD + d;
+            const uint32_t lo = pack_bf16(acc[u].x * r, acc[u].y * r);
+            const uint32_t hi = pack_bf16(acc[u].z * r, acc[u].w * r);
+            if ((reinterpret_cast<uintptr_t>(dst) & 7) == 0) {
+                *reinterpret_cast<uint2 *>(dst) = make_uint2(lo, hi);
+            } else {
+                uint16_t *e = reinterpret_cast<uint16_t *>(dst);
+                e[0] = (uint16_t)lo, e[1] = (uint16_t)(lo >> 16);
+                e[2] = (uint16_t)hi, e[3] = (uint16_t)(hi >> 16);
+            }
+        }
+        // the slots and s_m are free again after the next chunk's first barrier; a
+        // warp may write s_m before that, so join here
+        __syncthreads();
+    }
+}
+
+size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+
+// counters [segments] int32 | m, l [pieces][2][cols] | o [pieces][cols][hd], with
+// pieces = segments + CTAs (a piece's place is its segment + its CTA).
+struct WsLayout {
+    size_t cnt, ml, o;
+    size_t total() const { return cnt + ml + o; }
+};
+
+int tiles(int cols) { return cols <= 8 ? 1 : 2; }
+
+WsLayout ws_layout(int64_t batch, int hq, int hkv, int hd, int tokens) {
+    const int64_t cols = (int64_t)(hq / hkv) * tokens;
+    const int nc = 8 * tiles((int)(cols < 64 ? cols : 64));
+    const int64_t segs = batch * hkv * ((cols + nc - 1) / nc);
+    const int64_t pieces = segs + (int64_t)sm_count() * (nc == 8 ? 2 : 1);
+    return {align256(segs * 4), align256(pieces * 2 * nc * 4), (size_t)pieces * nc * hd * 4};
+}
+
+template <int HD, int NT>
+int launch(DecodeKv4Params p, int max_context_len, cudaStream_t stream) {
+    using C = Cfg<HD, NT>;
+    auto kern = decode_kv4_kernel<HD, NT>;
+    const int rc = ensure_smem_attr((const void *)kern, C::kSmem);
+    if (rc) return rc;
+    p.slices = (p.cols + C::kCols - 1) / C::kCols;
+    p.seg_per_seq = p.num_kv_heads * p.slices;
+    int64_t grid = (int64_t)sm_count() * C::kCtasPerSm;
+    if (max_context_len > 0) {  // less work than kMinPages pages per CTA
+        const int64_t pages = (int64_t)p.batch * p.seg_per_seq *
+                              (((int64_t)max_context_len + kBlockSize - 1) / kBlockSize);
+        grid = std::min<int64_t>(grid, (pages + kMinPages - 1) / kMinPages);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)std::max<int64_t>(grid, 1));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = C::kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    p.pdl_mode = dependent_launch_mode();
+    cfg.numAttrs = p.pdl_mode > 0 ? 1 : 0;
+    if (cudaLaunchKernelEx(&cfg, kern, p) != cudaSuccess) {
+        cudaGetLastError();
+        return LC_ERR_CUDA;
+    }
+    return LC_OK;
 }
 
 }  // namespace
@@ -102,7 +797,7 @@ extern "C" size_t lc_paged_decode_kv4_workspace_size(int batch, int num_q_heads,
     if (batch <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads ||
         tokens_per_seq <= 0 || (head_dim != 64 && head_dim != 128))
         return 0;
-    return 256;
+    return ws_layout(batch, num_q_heads, num_kv_heads, head_dim, tokens_per_seq).total();
 }
 
 extern "C" int lc_paged_decode_kv4(void *out, int64_t out_stride, const void *q, int64_t q_stride,
@@ -123,19 +818,16 @@ extern "C" int lc_paged_decode_kv4(void *out, int64_t out_stride, const void *q,
         return LC_ERR_INVALID_ARGUMENT;
     if (num_q_heads % num_kv_heads) return LC_ERR_UNSUPPORTED_SHAPE;
     if (table_stride > INT_MAX / kBlockSize ||
-        (int64_t)batch * tokens_per_seq > INT_MAX)
+        (int64_t)batch * tokens_per_seq > INT_MAX / num_q_heads / head_dim)
         return LC_ERR_INVALID_ARGUMENT;
     if (q_stride < (int64_t)num_q_heads * head_dim || out_stride < (int64_t)num_q_heads * head_dim)
         return LC_ERR_INVALID_ARGUMENT;
     if (!aligned16(kv_pool) || !aligned16(q) || (q_stride & 7) || ((uintptr_t)out & 1))
         return LC_ERR_MISALIGNED;
     if (batch == 0) return LC_OK;
-    if (!workspace || workspace_bytes < lc_paged_decode_kv4_workspace_size(
-                                            batch, num_q_heads, num_kv_heads, head_dim,
-                                            tokens_per_seq))
-        return LC_ERR_WORKSPACE_TOO_SMALL;
+    const WsLayout wl = ws_layout(batch, num_q_heads, num_kv_heads, head_dim, tokens_per_seq);
+    if (!workspace || workspace_bytes < wl.total()) return LC_ERR_WORKSPACE_TOO_SMALL;
     if (!aligned16(workspace)) return LC_ERR_MISALIGNED;
-    if (num_q_heads > 65535) return LC_ERR_UNSUPPORTED_SHAPE;
     DecodeKv4Params p{};
     p.out = (bf16 *)out;
     p.out_stride = out_stride;
@@ -153,13 +845,20 @@ extern "C" int lc_paged_decode_kv4(void *out, int64_t out_stride, const void *q,
     p.len_offset = len_offset;
     p.batch = batch;
     p.tokens = tokens_per_seq;
-    p.scale_log2 = sm_scale * k_scale * 1.4426950408889634f;
+    p.group = num_q_heads / num_kv_heads;
+    p.cols = p.group * tokens_per_seq;
+    p.scale_log2 = std::fabs(sm_scale) * k_scale * 1.4426950408889634f;
+    p.q_sign = std::signbit(sm_scale) ? 0x80008000u : 0u;
     p.v_scale = v_scale;
+    uint8_t *ws = (uint8_t *)workspace;
+    p.ws_cnt = (int *)ws;
+    p.ws_ml = (float *)(ws + wl.cnt);
+    p.ws_o = (float *)(ws + wl.cnt + wl.ml);
     p.status = dev_status;
-    const dim3 grid(batch * tokens_per_seq, num_q_heads);
-    if (head_dim == 64)
-        decode_kv4_simple_kernel<64><<<grid, kSimpleWarps * 32, 0, as_stream(stream)>>>(p);
-    else
-        decode_kv4_simple_kernel<128><<<grid, kSimpleWarps * 32, 0, as_stream(stream)>>>(p);
-    return launch_status();
+    cudaStream_t s = as_stream(stream);
+    if (tiles(p.cols) == 1)
+        return head_dim == 64 ? launch<64, 1>(p, max_context_len, s)
+                              : launch<128, 1>(p, max_context_len, s);
+    return head_dim == 64 ? launch<64, 2>(p, max_context_len, s)
+                          : launch<128, 2>(p, max_context_len, s);
 }
