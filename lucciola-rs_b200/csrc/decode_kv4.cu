@@ -13,11 +13,15 @@
 // (arrival counter) joins them in the order of the stream, so the result does
 // not depend on timing.
 //
-// Inside a CTA the warps take groups of kGroup pages in turn. Each warp has its
-// own ring of stages and fills it itself: one bulk copy per page brings K and V
-// of the kv head (18 hd bytes, contiguous), counted on the stage's mbarrier, and
-// the block-table entries are read one group ahead. No barrier joins the warps
-// before the end of a chunk (a CTA's part of one segment).
+// Inside a CTA eight warps compute, taking groups of kGroup pages in turn, each
+// from a ring of its own; a ninth loads, one lane per page of a group: one bulk
+// copy brings K and V of the kv head (18 hd bytes, contiguous). Full and empty
+// mbarriers per stage join a warp to its lanes of the loading warp and nothing
+// joins the warps until the end of a chunk (a CTA's part of one segment). There
+// each warp leaves its O, m and l in shared memory and goes on with the next
+// chunk; after its first group of that it joins the eight states for one column
+// and writes the row, or the piece, so the latency of that end (shared memory,
+// a fence, the arrival counter, the other pieces) runs beside the next chunk.
 //
 // Products, mma.sync m16n8k16 with fp16 operands and fp32 sums:
 //     S^T[16 tokens x 8 columns] = K[16 x hd] . Q^T
@@ -35,6 +39,7 @@
 //    8 more for r >= 8). Any order does; this one spreads the 64-byte token rows
 //    over the banks for the K loads and the V loads alike.
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 
@@ -44,8 +49,8 @@
 namespace lc {
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
+constexpr int kWarps = 8;  // computing; one more loads
+constexpr int kThreads = (kWarps + 1) * 32;
 constexpr int kGroup = 2;             // pages of one warp at a time
 constexpr int kMinPages = kWarps * kGroup;  // pages per CTA at least
 constexpr float kLazy = 8.f;  // p may reach 2^8 before O and l are rescaled
@@ -70,8 +75,8 @@ struct DecodeKv4Params {
     uint32_t q_sign;   // sign of sm_scale, on both halves of an fp16 pair
     float v_scale;
     int pdl_mode;
-    int *ws_cnt;    // [batch * seg_per_seq] arrivals
-    float *ws_ml;   // [pieces][2][kCols] m, l
+    int *ws_cnt;    // [batch * seg_per_seq][kCols] arrivals
+    float2 *ws_ml;  // [pieces][kCols] m, l
     float *ws_o;    // [pieces][kCols][hd]
     int *status;
 };
@@ -82,10 +87,9 @@ struct Cfg {
     static constexpr int kPage = 18 * HD;  // K and V of one kv head
     static constexpr int kStage = kGroup * kPage;
     static constexpr int kStages = HD == 64 ? 4 : 2;
-    static constexpr int kRow = HD + 4;  // floats between columns of a merge slot
-    static constexpr int kSlots = kWarps / 2;
+    static constexpr int kRow = HD + 4;  // floats between columns of a warp's state
     static constexpr int kRing = kWarps * kStages * kStage;
-    static constexpr int kSmem = kRing + kSlots * kCols * kRow * 4;
+    static constexpr int kSmem = kRing + kWarps * kCols * kRow * 4;
     static constexpr int kCtasPerSm = NT == 1 ? 2 : 1;
 };
 
@@ -102,11 +106,19 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                         uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
         "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The same without a sum to add to.
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                              uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
+        "{%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes,
@@ -114,6 +126,18 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
     asm volatile(
         "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
         ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ bool test_wait(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 q, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
 }
 
 __device__ __forceinline__ int tokens_of(const DecodeKv4Params &p, int b, bool report) {
@@ -129,26 +153,40 @@ __device__ __forceinline__ int pages_of(int tokens) {
     return (tokens + kBlockSize - 1) / kBlockSize;
 }
 
-// Where a walk over a CTA's range of the page stream stands: the chunk (b, seg)
-// pages [p0, p0 + take), its sequence's tokens and the stream index of its start.
+// The stream of `total` pages over `ctas` CTAs: the first `extra` of them take
+// `share` + 1 pages, the others `share`.
+struct Cut {
+    int ctas, share, extra;
+    __device__ __forceinline__ Cut(int total, int max_ctas) {
+        ctas = max(1, min(max_ctas, (total + kMinPages - 1) / kMinPages));
+        share = total / ctas;
+        extra = total - share * ctas;
+    }
+    __device__ __forceinline__ int start(int cta) const { return cta * share + min(cta, extra); }
+    __device__ __forceinline__ int owner(int page) const {
+        const int wide = extra * (share + 1);
+        return page < wide ? page / (share + 1) : extra + (page - wide) / share;
+    }
+};
+
+// Where a walk over a CTA's range of the stream stands: the chunk, pages
+// [p0, p0 + take) of segment seg of sequence b, which holds n tokens.
 struct Walk {
     int b, seg, p0, take, n;
-    long long at;  // stream index of page p0
+    int at;         // stream index of page p0
     int next_page;  // page of (b, seg) that the next chunk starts with
 
-    __device__ __forceinline__ void start(const DecodeKv4Params &p, long long first, int b0,
-                                          long long before_b0) {
+    __device__ __forceinline__ void start(const DecodeKv4Params &p, int first, int b0, int before_b0) {
         b = b0;
         n = tokens_of(p, b, false);
-        const long long off = first - before_b0;
-        const int pages = pages_of(n);
-        seg = pages ? (int)(off / pages) : 0;
-        next_page = pages ? (int)(off - (long long)seg * pages) : 0;
+        const int off = first - before_b0, pages = max(pages_of(n), 1);
+        seg = off / pages;
+        next_page = off - seg * pages;
         at = first;
         p0 = take = 0;
     }
     // Moves to the next chunk of [.., end); false when there is none.
-    __device__ __forceinline__ bool next(const DecodeKv4Params &p, long long end) {
+    __device__ __forceinline__ bool next(const DecodeKv4Params &p, int end) {
         at += take;
         if (at >= end) return false;
         int pages = pages_of(n);
@@ -161,31 +199,9 @@ struct Walk {
             }
         }
         p0 = next_page;
-        take = (int)min((long long)(pages - p0), end - at);
+        take = min(pages - p0, end - at);
         next_page = p0 + take;
         return true;
-    }
-};
-
-// The groups of one warp, in stream order: group k of a chunk is warp k % kWarps's.
-struct GroupWalk {
-    Walk w;
-    int page, np;  // first page and pages of the group
-    int base;      // next group's first page within the chunk
-    bool more;
-
-    __device__ __forceinline__ bool next(const DecodeKv4Params &p, long long end, int warp) {
-        while (more) {
-            if (base < w.take) {
-                page = w.p0 + base;
-                np = min(kGroup, w.take - base);
-                base += kGroup * kWarps;
-                return true;
-            }
-            more = w.next(p, end);
-            base = warp * kGroup;
-        }
-        return false;
     }
 };
 
@@ -197,11 +213,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
     constexpr int kSteps = HD / 16;   // k-steps of S, m-tiles of O
     constexpr int kWords = HD / 32;   // code words per token and lane (K)
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ __align__(8) uint64_t bars[kWarps][C::kStages];
-    __shared__ float s_m[kWarps][kCols], s_l[kWarps][kCols];
-    __shared__ long long s_sum[kWarps];
-    __shared__ long long s_before;
-    __shared__ int s_b0, s_last, s_abort;
+    __shared__ __align__(8) uint64_t full[kWarps][C::kStages], empty[kWarps][C::kStages];
+    __shared__ __align__(8) uint64_t states_full, states_empty;
+    __shared__ float2 s_ml[kWarps][kCols];
+    __shared__ int s_sum[kWarps + 1], s_b0, s_before, s_abort;
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3;
@@ -209,39 +224,44 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
         griddep_launch_dependents();
         if (p.pdl_mode == 1) griddep_wait();
     }
-    if (lane < C::kStages) mbar_init(&bars[warp][lane], 1);
-    if (tid == 0) s_abort = 0;
-    fence_barrier_init();
-
     // ---- the stream: its length, this CTA's range, the sequence it starts in
     const int per = (p.batch + kThreads - 1) / kThreads;
     const int q0 = min(p.batch, tid * per), q1 = min(p.batch, q0 + per);
-    long long mine = 0;
+    int mine = 0;
     for (int b = q0; b < q1; ++b) mine += pages_of(tokens_of(p, b, blockIdx.x == 0));
+    if (warp < kWarps && lane < C::kStages) {
+        mbar_init(&full[warp][lane], kGroup);
+        mbar_init(&empty[warp][lane], 1);
+    }
+    if (tid == 0) {
+        mbar_init(&states_full, kWarps);
+        mbar_init(&states_empty, kWarps);
+        s_abort = 0;
+    }
+    fence_barrier_init();
     mine *= p.seg_per_seq;
-    long long upto = mine;
+    int upto = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const long long u = __shfl_up_sync(0xffffffffu, upto, d);
+        const int u = __shfl_up_sync(0xffffffffu, upto, d);
         if (lane >= d) upto += u;
     }
     if (lane == 31) s_sum[warp] = upto;
     __syncthreads();
-    long long total = 0;
+    int total = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w <= kWarps; ++w) {
         if (w < warp) upto += s_sum[w];
         total += s_sum[w];
     }
-    const int ctas = (int)max(1ll, min((long long)gridDim.x, (total + kMinPages - 1) / kMinPages));
+    const Cut cut(total, gridDim.x);
     const int cta = blockIdx.x;
-    const long long first = cta < ctas ? total * cta / ctas : total;
-    const long long end = cta < ctas ? total * (cta + 1) / ctas : total;
+    const int first = cta < cut.ctas ? cut.start(cta) : total;
+    const int end = cta < cut.ctas ? cut.start(cta + 1) : total;
     if (first < end && upto - mine <= first && first < upto) {
-        long long before = upto - mine;
-        int b = q0;
+        int before = upto - mine, b = q0;
         for (;; ++b) {
-            const long long k = (long long)pages_of(tokens_of(p, b, false)) * p.seg_per_seq;
+            const int k = pages_of(tokens_of(p, b, false)) * p.seg_per_seq;
             if (first < before + k) break;
             before += k;
         }
@@ -261,56 +281,202 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
     }
     if (first >= end) return;
 
-    // ---- loads
-    uint8_t *ring = smem + warp * C::kStages * C::kStage;
-    const uint32_t ring_addr = smem_u32(ring);
-    GroupWalk gw;
-    gw.w.start(p, first, s_b0, s_before);
-    gw.more = gw.w.next(p, end);
-    gw.base = warp * kGroup;
-    int phys = 0;
-    auto look_up = [&]() {  // block-table entries of the group that is loaded next
-        if (lane < gw.np) phys = __ldg(p.tables + (int64_t)gw.w.b * p.table_stride + gw.page + lane);
-    };
-    bool pending = gw.next(p, end, warp);
-    if (pending) look_up();
-    uint32_t issued = 0;
-    auto issue = [&]() {
-        if (!pending) return;
-        const int stage = issued % C::kStages;
-        uint64_t *bar = &bars[warp][stage];
-        const bool bad = lane < gw.np && (phys < 0 || phys >= p.num_blocks);
-        const uint32_t bads = __ballot_sync(0xffffffffu, bad);
-        if (bads) {  // a table entry outside the pool reads as zeros
-            if (bad) set_status(p.status, LC_DEV_BAD_BLOCK);
-#pragma unroll
-            for (int k = 0; k < kGroup; ++k)
-                if (bads >> k & 1)
-                    for (int i = lane; i < C::kPage / 16; i += 32)
-                        reinterpret_cast<uint4 *>(ring + stage * C::kStage + k * C::kPage)[i] =
-                            make_uint4(0, 0, 0, 0);
-            // these stores before the copies that fill the stage later
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
+    if (warp == kWarps) {
+        // ---- loads: lane 2 w + k brings page k of each of warp w's groups, which are
+        // group w, w + kWarps, ... of every chunk
+        static_assert(kGroup * kWarps <= 32);
+        const int w = lane / kGroup, k = lane % kGroup;
+        const int64_t page_stride = kv4_offset(1, 0, 0, p.num_layers, p.num_kv_heads, HD);
+        const uint32_t dst0 = smem_u32(smem) + w * C::kStages * C::kStage + k * C::kPage;
+        Walk lw;
+        lw.start(p, first, s_b0, s_before);
+        bool more = lane < kGroup * kWarps && lw.next(p, end);
+        int base = w * kGroup;  // first page of the next group, within its chunk
+        int phys = -1;          // this lane's table entry in it, -1: no page
+        const uint8_t *head = nullptr;
+        auto advance = [&]() {
+            while (more && base >= lw.take) {
+                more = lw.next(p, end);
+                base = w * kGroup;
+            }
+            phys = -1;
+            if (more && base + k < lw.take) {
+                phys = __ldg(p.tables + (int64_t)lw.b * p.table_stride + lw.p0 + base + k);
+                if (phys < 0) phys = INT_MAX;  // a bad entry, reported when it is loaded
+            }
+            head = p.kv_pool + kv4_offset(0, p.layer, lw.seg / p.slices, p.num_layers,
+                                          p.num_kv_heads, HD);
+        };
+        advance();
+        int stage = 0, issued = 0;
+        uint32_t phase = 1;  // the first round finds every stage free
+        uint64_t since = 0;
+        for (uint32_t it = 0; __any_sync(0xffffffffu, more); ++it) {
+            const bool ready = more && test_wait(&empty[w][stage], phase);
+            if (ready) {
+                uint64_t *bar = &full[w][stage];
+                const uint32_t dst = dst0 + stage * C::kStage;
+                if ((uint32_t)phys < p.num_blocks) {
+                    mbar_arrive_expect_tx(bar, C::kPage);
+                    bulk_load(dst, head + phys * page_stride, C::kPage, bar);
+                } else {
+                    if (phys != -1) {  // a table entry outside the pool reads as zeros
+                        set_status(p.status, LC_DEV_BAD_BLOCK);
+                        for (int i = 0; i < C::kPage / 16; ++i)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst + 16 * i),
+                                         "r"(0) : "memory");
+                        // before the copies that fill the stage later
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    }
+                    mbar_arrive(bar);
+                }
+                ++issued;
+                if (++stage == C::kStages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+                base += kGroup * kWarps;
+                advance();
+            }
+            if (__any_sync(0xffffffffu, ready)) {
+                since = 0;
+                continue;
+            }
+            // nothing to do: wait a little, for 2 s at most
+            __nanosleep(40);
+            if ((it & 63) == 0) {
+                const uint64_t now = global_timer_ns();
+                if (since == 0) since = now;
+                if (now - since > kWaitLimitNs) {
+                    s_abort = 1;
+                    set_status(p.status, LC_DEV_TIMEOUT);
+                }
+                if (*(volatile int *)&s_abort) break;
+            }
         }
-        if (lane == 0) mbar_arrive_expect_tx(bar, (gw.np - __popc(bads)) * C::kPage);
+        // After a timeout the consumers may leave stages unread: no copy may land in
+        // a CTA that is gone.
         __syncwarp();
-        if (lane < gw.np && !bad)
-            bulk_load(ring_addr + stage * C::kStage + lane * C::kPage,
-                      p.kv_pool + kv4_offset(phys, p.layer, gw.w.seg / p.slices, p.num_layers,
-                                             p.num_kv_heads, HD),
-                      C::kPage, bar);
-        ++issued;
-        pending = gw.next(p, end, warp);
-        if (pending) look_up();
-    };
-#pragma unroll
-    for (int s = 0; s < C::kStages; ++s) issue();
+        if (*(volatile int *)&s_abort && lane < kGroup * kWarps)
+            for (int i = max(0, issued - C::kStages); i < issued; ++i)
+                mbar_wait_drain(&full[w][i % C::kStages], i / C::kStages & 1);
+        return;
+    }
 
     // ---- chunks
     const int pi0 = g & 1 ? 7 - (g >> 1) : g >> 1;  // token of tile row g
-    uint32_t used = 0;
-    Walk cw;
+    const uint8_t *ring = smem + warp * C::kStages * C::kStage;
+    float *states = reinterpret_cast<float *>(smem + C::kRing);  // [kWarps][kCols][kRow]
+    int stage = 0;
+    uint32_t phase = 0;
+    Walk cw, done{};  // the current chunk, and the one whose end is not written yet
+    bool open = false;
+    uint32_t chunk = 0;
+
+    // Joins the warps' states of chunk `done` for this warp's columns and writes the
+    // rows, or pieces of them.
+    auto finish = [&]() {
+        const bool ok = mbar_wait_bounded(&states_full, (chunk - 1) & 1, &s_abort, p.status);
+        constexpr int kPer = HD / 32;  // dims per lane
+        const int kvh = done.seg / p.slices, col0 = (done.seg - kvh * p.slices) * kCols;
+        float top[NT], sum[NT], acc[NT][kPer];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int c = nt * 8 + warp;
+            float2 ml[kWarps];
+            top[nt] = -INFINITY, sum[nt] = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                ml[w] = s_ml[w][c];
+                top[nt] = fmaxf(top[nt], ml[w].x);
+            }
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) acc[nt][i] = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                if (ml[w].x == -INFINITY) continue;  // saw nothing of this column
+                const float r = ex2(ml[w].x - top[nt]);
+                sum[nt] = fmaf(ml[w].y, r, sum[nt]);
+                const float *src = states + (w * kCols + c) * C::kRow + lane * kPer;
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) acc[nt][i] = fmaf(src[i], r, acc[nt][i]);
+            }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&states_empty);
+        if (!ok) return;
+
+        const int seg = done.b * p.seg_per_seq + done.seg, pages = pages_of(done.n);
+        const int seg_at = done.at - done.p0;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int c = nt * 8 + warp;
+            if (col0 + c >= p.cols) continue;
+            if (done.take != pages) {
+                float *po = p.ws_o + ((int64_t)(seg + cta) * kCols + c) * HD + lane * kPer;
+                if constexpr (kPer == 4)
+                    *reinterpret_cast<float4 *>(po) =
+                        make_float4(acc[nt][0], acc[nt][1], acc[nt][2], acc[nt][3]);
+                else
+                    *reinterpret_cast<float2 *>(po) = make_float2(acc[nt][0], acc[nt][1]);
+                if (lane == 0) p.ws_ml[(int64_t)(seg + cta) * kCols + c] = make_float2(top[nt], sum[nt]);
+                const int c0 = cut.owner(seg_at), pieces = cut.owner(seg_at + pages - 1) - c0 + 1;
+                __syncwarp();
+                int last = 0;
+                if (lane == 0) {
+                    int *cnt = p.ws_cnt + (int64_t)seg * kCols + c;
+                    last = atom_add_acq_rel_gpu(cnt, 1) == pieces - 1;
+                    if (last) *cnt = 0;  // ready for the next call
+                }
+                last = __shfl_sync(0xffffffffu, last, 0);
+                if (!last) continue;
+                const float2 *bml = p.ws_ml + (int64_t)(seg + c0) * kCols + c;
+                const float *bo = p.ws_o + ((int64_t)(seg + c0) * kCols + c) * HD + lane * kPer;
+                float high = -INFINITY;
+                for (int k = lane; k < pieces; k += 32) high = fmaxf(high, __ldcg(&bml[k * kCols].x));
+#pragma unroll
+                for (int d = 16; d; d >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, d));
+                sum[nt] = 0.f;
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) acc[nt][i] = 0.f;
+#pragma unroll 4
+                for (int k = 0; k < pieces; ++k) {
+                    const float2 ml = __ldcg(&bml[k * kCols]);
+                    float x[kPer];
+                    if constexpr (kPer == 4) {
+                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(bo + (int64_t)k * kCols * HD));
+                        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+                    } else {
+                        const float2 v = __ldcg(reinterpret_cast<const float2 *>(bo + (int64_t)k * kCols * HD));
+                        x[0] = v.x, x[1] = v.y;
+                    }
+                    const float r = ml.x == -INFINITY ? 0.f : ex2(ml.x - high);
+                    sum[nt] = fmaf(ml.y, r, sum[nt]);
+#pragma unroll
+                    for (int i = 0; i < kPer; ++i) acc[nt][i] = fmaf(x[i], r, acc[nt][i]);
+                }
+            }
+            const int qi = (col0 + c) / p.group, h = col0 + c - qi * p.group;
+            // a row without tokens gets zeros
+            const float r = sum[nt] == 0.f ? 0.f : p.v_scale / sum[nt];
+            bf16 *dst = p.out + ((int64_t)done.b * p.tokens + qi) * p.out_stride +
+                        (int64_t)(kvh * p.group + h) * HD + lane * kPer;
+            uint32_t v[kPer / 2];
+#pragma unroll
+            for (int i = 0; i < kPer / 2; ++i) v[i] = pack_bf16(acc[nt][2 * i] * r, acc[nt][2 * i + 1] * r);
+            if ((reinterpret_cast<uintptr_t>(dst) & (2 * kPer - 1)) == 0) {
+                if constexpr (kPer == 4)
+                    *reinterpret_cast<uint2 *>(dst) = make_uint2(v[0], v[1]);
+                else
+                    *reinterpret_cast<uint32_t *>(dst) = v[0];
+            } else {
+                uint16_t *e = reinterpret_cast<uint16_t *>(dst);
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) e[i] = (uint16_t)(v[i / 2] >> (i % 2 * 16));
+            }
+        }
+    };
+
     cw.start(p, first, s_b0, s_before);
     while (cw.next(p, end)) {
         const int kvh = cw.seg / p.slices, col0 = (cw.seg - kvh * p.slices) * kCols;
@@ -323,7 +489,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int c = nt * 8 + g;
-            float fc = 0.f;
             uint4 raw[HD / 32];
             if (c < ncols) {
                 const int i = (col0 + c) / p.group, h = (col0 + c) - i * p.group;
@@ -344,7 +509,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const int e = top ? (int)(top >> 7) - 127 : 0;
             const float down = ldexpf(1.f, -e);
-            fc = p.scale_log2 * ldexpf(1.f, e);
+            // never zero, so that a masked score stays -inf
+            const float fc = fmaxf(p.scale_log2 * ldexpf(1.f, e), FLT_MIN);
 #pragma unroll
             for (int k = 0; k < HD / 8; ++k) {
                 const float lo = __uint_as_float(r[k] << 16) * down;
@@ -364,10 +530,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
 
         float o[kSteps][NT][4];
         float m[NT][2], l[NT][2];
+        float off[NT][2];  // m, or 0 while it is -inf
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             m[nt][0] = m[nt][1] = -INFINITY;
-            l[nt][0] = l[nt][1] = 0.f;
+            l[nt][0] = l[nt][1] = off[nt][0] = off[nt][1] = 0.f;
 #pragma unroll
             for (int j = 0; j < kSteps; ++j)
 #pragma unroll
@@ -375,24 +542,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
         }
 
         for (int base = warp * kGroup; base < cw.take; base += kGroup * kWarps) {
-            const int np = min(kGroup, cw.take - base);
             const int tok0 = (cw.p0 + base) * kBlockSize;
-            const int stage = used % C::kStages;
-            uint64_t *bar = &bars[warp][stage];
-            if (!mbar_wait_bounded(bar, used / C::kStages & 1, &s_abort, p.status))
-                mbar_wait_drain(bar, used / C::kStages & 1);
-            __syncwarp();
+            // after a timeout the stage holds anything; the status word says so
+            mbar_wait_bounded(&full[warp][stage], phase, &s_abort, p.status);
             const uint8_t *st = ring + stage * C::kStage;
 
             // S^T = K . Q^T
             float s[kGroup][NT][4];
 #pragma unroll
             for (int pg = 0; pg < kGroup; ++pg) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) s[pg][nt][k] = pg < np ? 0.f : -INFINITY;
-                if (pg >= np) continue;
                 const uint8_t *kp = st + pg * C::kPage;
                 uint32_t wa[kWords], wb[kWords], sa[2], sb[2];
                 if constexpr (HD == 128) {
@@ -427,12 +585,18 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
                         const uint32_t a1 = hmul2(hb[2 * k], fb), a3 = hmul2(hb[2 * k + 1], fb);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
-                            mma_f16(s[pg][nt], a0, a1, a2, a3, qf[nt][2 * w + k][0],
-                                    qf[nt][2 * w + k][1]);
+                            if (w + k == 0)
+                                mma_f16_first(s[pg][nt], a0, a1, a2, a3, qf[nt][0][0], qf[nt][0][1]);
+                            else
+                                mma_f16(s[pg][nt], a0, a1, a2, a3, qf[nt][2 * w + k][0],
+                                        qf[nt][2 * w + k][1]);
                     }
                 }
             }
-            const bool tail = tok0 + np * kBlockSize > all;
+            // A group that reaches past the tokens that all columns see. A page past
+            // the chunk is masked as well; its stage holds anything.
+            const int held = min(cw.n, (cw.p0 + cw.take) * kBlockSize);
+            const bool tail = tok0 + kGroup * kBlockSize > min(all, held);
             if (tail) {
 #pragma unroll
                 for (int pg = 0; pg < kGroup; ++pg)
@@ -440,7 +604,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            if (tok0 + pg * kBlockSize + pi0 + (k >> 1) * 8 >= lim[nt][k & 1])
+                            if (tok0 + pg * kBlockSize + pi0 + (k >> 1) * 8 >=
+                                min(lim[nt][k & 1], held))
                                 s[pg][nt][k] = -INFINITY;
             }
 
@@ -455,7 +620,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
 #pragma unroll
                     for (int pg = 1; pg < kGroup; ++pg)
                         x = fmaxf(x, fmaxf(s[pg][nt][k], s[pg][nt][k + 2]));
-                    top[nt][k] = x == -INFINITY ? x : x * f[nt][k];
+                    top[nt][k] = x * f[nt][k];
                     raise |= top[nt][k] > m[nt][k] + kLazy;
                 }
             if (__any_sync(0xffffffffu, raise)) {
@@ -470,6 +635,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
                         x = fmaxf(x, m[nt][k]);
                         const float r = m[nt][k] == -INFINITY ? 0.f : ex2(m[nt][k] - x);
                         m[nt][k] = x;
+                        off[nt][k] = x == -INFINITY ? 0.f : x;
                         l[nt][k] *= r;
 #pragma unroll
                         for (int j = 0; j < kSteps; ++j) {
@@ -481,16 +647,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
             uint32_t pf[kGroup][NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                const float b0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0];
-                const float b1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
 #pragma unroll
                 for (int pg = 0; pg < kGroup; ++pg)
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        // a masked score stays -inf whatever the factor is
-                        const float x0 = s[pg][nt][2 * k], x1 = s[pg][nt][2 * k + 1];
-                        const float p0 = x0 == -INFINITY ? 0.f : ex2(fmaf(x0, f[nt][0], -b0));
-                        const float p1 = x1 == -INFINITY ? 0.f : ex2(fmaf(x1, f[nt][1], -b1));
+                        const float p0 = ex2(fmaf(s[pg][nt][2 * k], f[nt][0], -off[nt][0]));
+                        const float p1 = ex2(fmaf(s[pg][nt][2 * k + 1], f[nt][1], -off[nt][1]));
                         l[nt][0] += p0;
                         l[nt][1] += p1;
                         const __half2 v = __floats2half2_rn(p0, p1);
@@ -501,7 +663,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
             // O^T += V^T . P^T
 #pragma unroll
             for (int pg = 0; pg < kGroup; ++pg) {
-                if (pg >= np) continue;
                 const uint8_t *vp = st + pg * C::kPage + kv4_half_bytes(HD);
                 const uint8_t *sc = vp + kv4_code_bytes(HD);
                 constexpr int kRowBytes = HD / 2, kRowScales = HD / 16;
@@ -510,7 +671,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
                 uint32_t s23 = sc[(8 + t) * kRowScales + sg] | sc[(15 - t) * kRowScales + sg] << 8;
                 if (tail) {
                     // tokens past the end hold anything: their scales become zero
-                    const int left = cw.n - tok0 - pg * kBlockSize;
+                    const int left = held - tok0 - pg * kBlockSize;
                     if (t >= left) s01 &= 0xff00u;
                     if (7 - t >= left) s01 &= 0x00ffu;
                     if (8 + t >= left) s23 &= 0xff00u;
@@ -521,7 +682,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
                         const int common = all - tok0 - pg * kBlockSize;
                         uint32_t nan = 0;  // by token of the page
                         auto drop = [&](uint32_t &sc2, int sh, int tok) {
-                            if ((sc2 >> sh & 0x7fu) == kKv4NanScale && tok >= common) {
+                            if ((sc2 >> sh & 0x7fu) == kKv4NanScale && tok >= common && tok < left) {
                                 sc2 &= ~(0xffu << sh);
                                 nan |= 1u << tok;
                             }
@@ -574,171 +735,46 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
                 }
             }
             __syncwarp();
-            ++used;
-            issue();
+            if (lane == 0) mbar_arrive(&empty[warp][stage]);
+            if (++stage == C::kStages) {
+                stage = 0;
+                phase ^= 1;
+            }
+            if (open) {
+                finish();
+                open = false;
+            }
         }
 
-        // ---- the chunk's end: join the warps
+        // ---- the chunk's end: leave this warp's state for the join
+        if (open) finish();
+        if (chunk > 0) mbar_wait_bounded(&states_empty, (chunk - 1) & 1, &s_abort, p.status);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) l[nt][k] += __shfl_xor_sync(0xffffffffu, l[nt][k], d);
-                if (g == 0) {
-                    s_m[warp][nt * 8 + 2 * t + k] = m[nt][k];
-                    s_l[warp][nt * 8 + 2 * t + k] = l[nt][k];
-                }
+                const int c = nt * 8 + 2 * t + k;
+                if (g == 0) s_ml[warp][c] = make_float2(m[nt][k], l[nt][k]);
+                float *dst = states + (warp * kCols + c) * C::kRow + g * (HD / 8);
+#pragma unroll
+                for (int j = 0; j < kSteps; j += 2)
+                    *reinterpret_cast<float4 *>(dst + 2 * j) = make_float4(
+                        o[j][nt][k], o[j][nt][k + 2], o[j + 1][nt][k], o[j + 1][nt][k + 2]);
             }
-        __syncthreads();
-        float *slots = reinterpret_cast<float *>(smem + C::kRing);
-        float *slot = slots + (warp % C::kSlots) * kCols * C::kRow;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                float top = -INFINITY;
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w][nt * 8 + 2 * t + k]);
-                const float r = m[nt][k] == -INFINITY ? 0.f : ex2(m[nt][k] - top);
-#pragma unroll
-                for (int j = 0; j < kSteps; ++j) {
-                    // a column that saw nothing here adds nothing, whatever o holds
-                    o[j][nt][k] = m[nt][k] == -INFINITY ? 0.f : o[j][nt][k] * r;
-                    o[j][nt][k + 2] = m[nt][k] == -INFINITY ? 0.f : o[j][nt][k + 2] * r;
-                }
-            }
-        auto each = [&](auto &&fn) {  // 4 consecutive dims of one column at a time
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int k = 0; k < 2; ++k)
-#pragma unroll
-                    for (int j = 0; j < kSteps; j += 2)
-                        fn(reinterpret_cast<float4 *>(slot + (nt * 8 + 2 * t + k) * C::kRow +
-                                                      g * (HD / 8) + 2 * j),
-                           o[j][nt][k], o[j][nt][k + 2], o[j + 1][nt][k], o[j + 1][nt][k + 2]);
-        };
-        if (warp >= C::kSlots)
-            each([](float4 *d, float a, float b, float c, float e) { *d = make_float4(a, b, c, e); });
-        __syncthreads();
-        if (warp < C::kSlots)
-            each([](float4 *d, float a, float b, float c, float e) {
-                const float4 x = *d;
-                *d = make_float4(x.x + a, x.y + b, x.z + c, x.w + e);
-            });
-        __syncthreads();
-
-        const long long seg = (long long)cw.b * p.seg_per_seq + cw.seg;
-        const int pages = pages_of(cw.n);
-        const bool whole = cw.take == pages;
-        // CTA c starts at total * c / ctas; CTAs of the segment's first and last page
-        auto owner = [&](long long x) {
-            int c = (int)min((long long)ctas - 1, x * ctas / total);
-            while (c + 1 < ctas && total * (c + 1) / ctas <= x) ++c;
-            while (total * c / ctas > x) --c;
-            return c;
-        };
-        const long long seg_at = cw.at - cw.p0;
-        constexpr int kQuads = kCols * HD / 4;
-        constexpr int kTurns = kQuads / kThreads > 0 ? kQuads / kThreads : 1;
-        float4 acc[kTurns];
-        float cm[kTurns], cl[kTurns];
-#pragma unroll
-        for (int u = 0; u < kTurns; ++u) {
-            const int i = tid + u * kThreads;
-            if (i >= kQuads) break;
-            const int c = i / (HD / 4), d = i % (HD / 4) * 4;
-            float top = -INFINITY, sum = 0.f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w][c]);
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w)
-                sum += s_m[w][c] == -INFINITY ? 0.f : s_l[w][c] * ex2(s_m[w][c] - top);
-            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int k = 0; k < C::kSlots; ++k) {
-                const float4 x = *reinterpret_cast<const float4 *>(slots + (k * kCols + c) * C::kRow + d);
-                a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
-            }
-            acc[u] = a, cm[u] = top, cl[u] = sum;
-        }
-        if (!whole) {
-            float *po = p.ws_o + (seg + cta) * kCols * HD;
-            float *pml = p.ws_ml + (seg + cta) * 2 * kCols;
-#pragma unroll
-            for (int u = 0; u < kTurns; ++u) {
-                const int i = tid + u * kThreads;
-                if (i >= kQuads) break;
-                reinterpret_cast<float4 *>(po)[i] = acc[u];
-                if (i % (HD / 4) == 0) {
-                    pml[i / (HD / 4)] = cm[u];
-                    pml[kCols + i / (HD / 4)] = cl[u];
-                }
-            }
-            __threadfence();
-            __syncthreads();
-            const int c0 = owner(seg_at), pieces = owner(seg_at + pages - 1) - c0 + 1;
-            if (tid == 0) {
-                s_last = atomicAdd(p.ws_cnt + seg, 1) == pieces - 1;
-                if (s_last) p.ws_cnt[seg] = 0;  // ready for the next call
-            }
-            __syncthreads();
-            if (!s_last) continue;
-            __threadfence();
-            const float *bo = p.ws_o + (seg + c0) * kCols * HD;
-            const float *bml = p.ws_ml + (seg + c0) * 2 * kCols;
-#pragma unroll
-            for (int u = 0; u < kTurns; ++u) {
-                const int i = tid + u * kThreads;
-                if (i >= kQuads) break;
-                const int c = i / (HD / 4);
-                float top = -INFINITY;
-                for (int k = 0; k < pieces; ++k) top = fmaxf(top, __ldcg(bml + k * 2 * kCols + c));
-                float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-                float sum = 0.f;
-#pragma unroll 4
-                for (int k = 0; k < pieces; ++k) {
-                    const float pm = __ldcg(bml + k * 2 * kCols + c);
-                    const float pl = __ldcg(bml + k * 2 * kCols + kCols + c);
-                    const float4 x = __ldcg(reinterpret_cast<const float4 *>(bo + (int64_t)k * kCols * HD) + i);
-                    const float r = pm == -INFINITY ? 0.f : ex2(pm - top);
-                    sum += pl * r;
-                    a.x += x.x * r, a.y += x.y * r, a.z += x.z * r, a.w += x.w * r;
-                }
-                acc[u] = a, cl[u] = sum;
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < kTurns; ++u) {
-            const int i = tid + u * kThreads;
-            if (i >= kQuads) break;
-            const int c = i / (HD / 4), d = i % (HD / 4) * 4;
-            if (c >= ncols) continue;
-            const int qi = (col0 + c) / p.group, h = col0 + c - qi * p.group;
-            // a row without tokens gets zeros
-            const float r = cl[u] == 0.f ? 0.f : p.v_scale / cl[u];
-            bf16 *dst = p.out + ((int64_t)cw.b * p.tokens + qi) * p.out_stride +
-                        (int64_t)(kvh * p.group + h) * HD + d;
-            const uint32_t lo = pack_bf16(acc[u].x * r, acc[u].y * r);
-            const uint32_t hi = pack_bf16(acc[u].z * r, acc[u].w * r);
-            if ((reinterpret_cast<uintptr_t>(dst) & 7) == 0) {
-                *reinterpret_cast<uint2 *>(dst) = make_uint2(lo, hi);
-            } else {
-                uint16_t *e = reinterpret_cast<uint16_t *>(dst);
-                e[0] = (uint16_t)lo, e[1] = (uint16_t)(lo >> 16);
-                e[2] = (uint16_t)hi, e[3] = (uint16_t)(hi >> 16);
-            }
-        }
-        // the slots and s_m are free again after the next chunk's first barrier; a
-        // warp may write s_m before that, so join here
-        __syncthreads();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&states_full);
+        ++chunk;
+        done = cw;
+        open = true;
     }
+    if (open) finish();
 }
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
-// counters [segments] int32 | m, l [pieces][2][cols] | o [pieces][cols][hd], with
+// counters [segments][cols] int32 | m, l [pieces][cols] | o [pieces][cols][hd], with
 // pieces = segments + CTAs (a piece's place is its segment + its CTA).
 struct WsLayout {
     size_t cnt, ml, o;
@@ -752,7 +788,7 @@ WsLayout ws_layout(int64_t batch, int hq, int hkv, int hd, int tokens) {
     const int nc = 8 * tiles((int)(cols < 64 ? cols : 64));
     const int64_t segs = batch * hkv * ((cols + nc - 1) / nc);
     const int64_t pieces = segs + (int64_t)sm_count() * (nc == 8 ? 2 : 1);
-    return {align256(segs * 4), align256(pieces * 2 * nc * 4), (size_t)pieces * nc * hd * 4};
+    return {align256(segs * nc * 4), align256(pieces * nc * 8), (size_t)pieces * nc * hd * 4};
 }
 
 template <int HD, int NT>
@@ -763,6 +799,8 @@ int launch(DecodeKv4Params p, int max_context_len, cudaStream_t stream) {
     if (rc) return rc;
     p.slices = (p.cols + C::kCols - 1) / C::kCols;
     p.seg_per_seq = p.num_kv_heads * p.slices;
+    // the stream's indexes are int32
+    if ((int64_t)p.batch * p.table_stride > INT_MAX / p.seg_per_seq) return LC_ERR_UNSUPPORTED_SHAPE;
     int64_t grid = (int64_t)sm_count() * C::kCtasPerSm;
     if (max_context_len > 0) {  // less work than kMinPages pages per CTA
         const int64_t pages = (int64_t)p.batch * p.seg_per_seq *
@@ -817,7 +855,7 @@ extern "C" int lc_paged_decode_kv4(void *out, int64_t out_stride, const void *q,
         max_context_len < 0 || len_offset < 0 || len_offset > 1)
         return LC_ERR_INVALID_ARGUMENT;
     if (num_q_heads % num_kv_heads) return LC_ERR_UNSUPPORTED_SHAPE;
-    if (table_stride > INT_MAX / kBlockSize ||
+    if (table_stride > INT_MAX / kBlockSize || num_blocks > INT_MAX ||
         (int64_t)batch * tokens_per_seq > INT_MAX / num_q_heads / head_dim)
         return LC_ERR_INVALID_ARGUMENT;
     if (q_stride < (int64_t)num_q_heads * head_dim || out_stride < (int64_t)num_q_heads * head_dim)
@@ -852,7 +890,7 @@ extern "C" int lc_paged_decode_kv4(void *out, int64_t out_stride, const void *q,
     p.v_scale = v_scale;
     uint8_t *ws = (uint8_t *)workspace;
     p.ws_cnt = (int *)ws;
-    p.ws_ml = (float *)(ws + wl.cnt);
+    p.ws_ml = (float2 *)(ws + wl.cnt);
     p.ws_o = (float *)(ws + wl.cnt + wl.ml);
     p.status = dev_status;
     cudaStream_t s = as_stream(stream);
