@@ -14,14 +14,15 @@
 // not depend on timing.
 //
 // Inside a CTA eight warps compute, taking groups of kGroup pages in turn, each
-// from a ring of its own; a ninth loads, one lane per page of a group: one bulk
-// copy brings K and V of the kv head (18 hd bytes, contiguous). Full and empty
-// mbarriers per stage join a warp to its lanes of the loading warp and nothing
-// joins the warps until the end of a chunk (a CTA's part of one segment). There
-// each warp leaves its O, m and l in shared memory and goes on with the next
-// chunk; after its first group of that it joins the eight states for one column
-// and writes the row, or the piece, so the latency of that end (shared memory,
-// a fence, the arrival counter, the other pieces) runs beside the next chunk.
+// from a ring of its own. A loading warp fills the rings, one lane per page of a
+// group: one bulk copy brings K and V of the kv head (18 hd bytes, contiguous),
+// and full and empty mbarriers per stage join a computing warp to its lanes. An
+// edge warp works a chunk (a CTA's part of one segment) ahead and behind: it
+// prepares the next chunk's q as mma operands in shared memory, and joins the
+// eight states (O, m, l) that the computing warps leave at a chunk's end, so the
+// latency of that end (shared memory, the stores, the arrival counter, the other
+// pieces) runs beside the next chunk. The computing warps touch no global memory
+// until the CTA's last chunk, whose columns they join themselves, one per warp.
 //
 // Products, mma.sync m16n8k16 with fp16 operands and fp32 sums:
 //     S^T[16 tokens x 8 columns] = K[16 x hd] . Q^T
@@ -42,6 +43,7 @@
 #include <cfloat>
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 #include "kv4.cuh"
 #include "lc_host.h"
@@ -49,8 +51,10 @@
 namespace lc {
 namespace {
 
-constexpr int kWarps = 8;  // computing; one more loads
-constexpr int kThreads = (kWarps + 1) * 32;
+constexpr int kWarps = 8;             // computing
+constexpr int kLoadWarp = kWarps;     // one that loads
+constexpr int kEdgeWarp = kWarps + 1;  // one for the chunks' ends
+constexpr int kThreads = (kWarps + 2) * 32;
 constexpr int kGroup = 2;             // pages of one warp at a time
 constexpr int kMinPages = kWarps * kGroup;  // pages per CTA at least
 constexpr float kLazy = 8.f;  // p may reach 2^8 before O and l are rescaled
@@ -89,7 +93,9 @@ struct Cfg {
     static constexpr int kStages = HD == 64 ? 4 : 2;
     static constexpr int kRow = HD + 4;  // floats between columns of a warp's state
     static constexpr int kRing = kWarps * kStages * kStage;
-    static constexpr int kSmem = kRing + kWarps * kCols * kRow * 4;
+    static constexpr int kStates = kWarps * kCols * kRow * 4;
+    static constexpr int kQ = kCols * HD * 2;  // a chunk's q, fp16 operands
+    static constexpr int kSmem = kRing + kStates + 2 * kQ;
     static constexpr int kCtasPerSm = NT == 1 ? 2 : 1;
 };
 
@@ -101,6 +107,16 @@ __device__ __forceinline__ float ex2(float x) {
 
 __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
     const __half2 r = __hmul2(*reinterpret_cast<__half2 *>(&a), *reinterpret_cast<__half2 *>(&b));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+
+// Both halves of `a` replaced by its low or its high one.
+__device__ __forceinline__ uint32_t both_low(uint32_t a) {
+    const __half2 r = __low2half2(*reinterpret_cast<__half2 *>(&a));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+__device__ __forceinline__ uint32_t both_high(uint32_t a) {
+    const __half2 r = __high2half2(*reinterpret_cast<__half2 *>(&a));
     return *reinterpret_cast<const uint32_t *>(&r);
 }
 
@@ -153,19 +169,22 @@ __device__ __forceinline__ int pages_of(int tokens) {
     return (tokens + kBlockSize - 1) / kBlockSize;
 }
 
-// The stream of `total` pages over `ctas` CTAs: the first `extra` of them take
-// `share` + 1 pages, the others `share`.
+// The stream of `total` pages over `ctas` CTAs: CTA c takes the pages from
+// total * c / ctas on.
 struct Cut {
-    int ctas, share, extra;
-    __device__ __forceinline__ Cut(int total, int max_ctas) {
+    int total, ctas;
+    __device__ __forceinline__ Cut(const DecodeKv4Params &p, int pages, int max_ctas) {
+        total = pages;
         ctas = max(1, min(max_ctas, (total + kMinPages - 1) / kMinPages));
-        share = total / ctas;
-        extra = total - share * ctas;
+        // One sequence on part of the GPU: whole CTAs per segment, so that none of them
+        // joins two segments in turn.
+        if (p.batch == 1 && ctas < max_ctas && ctas > p.seg_per_seq) ctas -= ctas % p.seg_per_seq;
     }
-    __device__ __forceinline__ int start(int cta) const { return cta * share + min(cta, extra); }
+    __device__ __forceinline__ int start(int cta) const {
+        return (int)((long long)total * cta / ctas);
+    }
     __device__ __forceinline__ int owner(int page) const {
-        const int wide = extra * (share + 1);
-        return page < wide ? page / (share + 1) : extra + (page - wide) / share;
+        return (int)((((long long)page + 1) * ctas - 1) / total);
     }
 };
 
@@ -205,6 +224,133 @@ struct Walk {
     }
 };
 
+// What the edge warp tells the computing warps about a chunk.
+struct ChunkInfo {
+    int b, seg, p0, take, n, at, last;
+};
+
+template <int HD, int NT>
+struct Joined {  // one column of a chunk, this lane's dims
+    static constexpr int kPer = HD / 32;
+    float m, l, o[kPer];
+};
+
+// Joins the warps' states for column c of a chunk.
+template <int HD, int NT>
+__device__ __forceinline__ void join_states(const float2 (*ml_of)[Cfg<HD, NT>::kCols],
+                                            const float *states, int c, int lane,
+                                            Joined<HD, NT> &j) {
+    using C = Cfg<HD, NT>;
+    float2 ml[kWarps];
+    j.m = -INFINITY, j.l = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        ml[w] = ml_of[w][c];
+        j.m = fmaxf(j.m, ml[w].x);
+    }
+#pragma unroll
+    for (int i = 0; i < j.kPer; ++i) j.o[i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (ml[w].x == -INFINITY) continue;  // saw nothing of this column
+        const float r = ex2(ml[w].x - j.m);
+        j.l = fmaf(ml[w].y, r, j.l);
+        const float *src = states + (w * C::kCols + c) * C::kRow + lane * j.kPer;
+#pragma unroll
+        for (int i = 0; i < j.kPer; ++i) j.o[i] = fmaf(src[i], r, j.o[i]);
+    }
+}
+
+// The output row of column c of a chunk from its joined state.
+template <int HD, int NT>
+__device__ __forceinline__ void write_row(const DecodeKv4Params &p, const ChunkInfo &ch, int c,
+                                          int lane, const Joined<HD, NT> &j) {
+    constexpr int kPer = HD / 32;
+    const int kvh = ch.seg / p.slices, col = (ch.seg - kvh * p.slices) * Cfg<HD, NT>::kCols + c;
+    if (col >= p.cols) return;
+    const int qi = col / p.group, h = col - qi * p.group;
+    // a row without tokens gets zeros
+    const float r = j.l == 0.f ? 0.f : p.v_scale / j.l;
+    bf16 *dst = p.out + ((int64_t)ch.b * p.tokens + qi) * p.out_stride +
+                (int64_t)(kvh * p.group + h) * HD + lane * kPer;
+    uint32_t v[kPer / 2];
+#pragma unroll
+    for (int i = 0; i < kPer / 2; ++i) v[i] = pack_bf16(j.o[2 * i] * r, j.o[2 * i + 1] * r);
+    if ((reinterpret_cast<uintptr_t>(dst) & (2 * kPer - 1)) == 0) {
+        if constexpr (kPer == 4)
+            *reinterpret_cast<uint2 *>(dst) = make_uint2(v[0], v[1]);
+        else
+            *reinterpret_cast<uint32_t *>(dst) = v[0];
+    } else {
+        uint16_t *e = reinterpret_cast<uint16_t *>(dst);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) e[i] = (uint16_t)(v[i / 2] >> (i % 2 * 16));
+    }
+}
+
+// A chunk that is a part of its segment leaves a piece per column, at the place
+// of its segment and CTA.
+template <int HD, int NT>
+__device__ __forceinline__ void store_piece(const DecodeKv4Params &p, int64_t place, int c, int lane,
+                                            const Joined<HD, NT> &j) {
+    constexpr int kCols = Cfg<HD, NT>::kCols, kPer = HD / 32;
+    float *po = p.ws_o + (place * kCols + c) * HD + lane * kPer;
+    if constexpr (kPer == 4)
+        *reinterpret_cast<float4 *>(po) = make_float4(j.o[0], j.o[1], j.o[2], j.o[3]);
+    else
+        *reinterpret_cast<float2 *>(po) = make_float2(j.o[0], j.o[1]);
+    if (lane == 0) p.ws_ml[place * kCols + c] = make_float2(j.m, j.l);
+}
+
+// Counts a piece of column c; true for the segment's last one. One lane, after
+// the warp's stores and a __syncwarp.
+template <int kCols>
+__device__ __forceinline__ bool last_piece(const DecodeKv4Params &p, int64_t seg, int c, int pieces) {
+    int *cnt = p.ws_cnt + seg * kCols + c;
+    if (atom_add_acq_rel_gpu(cnt, 1) != pieces - 1) return false;
+    *cnt = 0;  // ready for the next call
+    return true;
+}
+
+// Joins the pieces of column c, the first of which lies at `place`, in order.
+template <int HD, int NT>
+__device__ __forceinline__ void join_pieces(const DecodeKv4Params &p, int64_t place, int pieces, int c,
+                                            int lane, Joined<HD, NT> &j) {
+    constexpr int kCols = Cfg<HD, NT>::kCols, kPer = HD / 32;
+    const float2 *bml = p.ws_ml + place * kCols + c;
+    const float *bo = p.ws_o + (place * kCols + c) * HD + lane * kPer;
+    j.m = -INFINITY;
+    for (int k = lane; k < pieces; k += 32) j.m = fmaxf(j.m, __ldcg(&bml[k * kCols].x));
+#pragma unroll
+    for (int d = 16; d; d >>= 1) j.m = fmaxf(j.m, __shfl_xor_sync(0xffffffffu, j.m, d));
+    j.l = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) j.o[i] = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < pieces; ++k) {
+        const float2 ml = __ldcg(&bml[k * kCols]);
+        float x[kPer];
+        if constexpr (kPer == 4) {
+            const float4 v = __ldcg(reinterpret_cast<const float4 *>(bo + (int64_t)k * kCols * HD));
+            x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+        } else {
+            const float2 v = __ldcg(reinterpret_cast<const float2 *>(bo + (int64_t)k * kCols * HD));
+            x[0] = v.x, x[1] = v.y;
+        }
+        const float r = ml.x == -INFINITY ? 0.f : ex2(ml.x - j.m);
+        j.l = fmaf(ml.y, r, j.l);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) j.o[i] = fmaf(x[i], r, j.o[i]);
+    }
+}
+
+// The pieces of a chunk's segment: the CTA of the first one, and how many.
+__device__ __forceinline__ int pieces_of(const Cut &cut, const ChunkInfo &ch, int &c0) {
+    const int seg_at = ch.at - ch.p0;
+    c0 = cut.owner(seg_at);
+    return cut.owner(seg_at + pages_of(ch.n) - 1) - c0 + 1;
+}
+
 template <int HD, int NT>
 __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
     decode_kv4_kernel(const DecodeKv4Params p) {
@@ -214,82 +360,84 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
     constexpr int kWords = HD / 32;   // code words per token and lane (K)
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(8) uint64_t full[kWarps][C::kStages], empty[kWarps][C::kStages];
-    __shared__ __align__(8) uint64_t states_full, states_empty;
+    __shared__ __align__(8) uint64_t q_full[2], states_full, states_empty, edge_done;
+    __shared__ ChunkInfo s_chunk[2];
+    // Columns of the CTA's first chunk whose last piece it was, to be joined at the end.
+    __shared__ ChunkInfo s_left;
+    __shared__ uint32_t s_left_cols;
+    __shared__ float s_f[2][kCols];
     __shared__ float2 s_ml[kWarps][kCols];
-    __shared__ int s_sum[kWarps + 1], s_b0, s_before, s_abort;
+    __shared__ int s_abort, s_total;
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3;
+    const int cta = blockIdx.x;
+    float *states = reinterpret_cast<float *>(smem + C::kRing);  // [kWarps][kCols][kRow]
+    uint8_t *q_ops = smem + C::kRing + C::kStates;               // [2][NT][kSteps][32 lanes] 8 bytes
     if (p.pdl_mode > 0) {
         griddep_launch_dependents();
         if (p.pdl_mode == 1) griddep_wait();
     }
-    // ---- the stream: its length, this CTA's range, the sequence it starts in
-    const int per = (p.batch + kThreads - 1) / kThreads;
-    const int q0 = min(p.batch, tid * per), q1 = min(p.batch, q0 + per);
-    int mine = 0;
-    for (int b = q0; b < q1; ++b) mine += pages_of(tokens_of(p, b, blockIdx.x == 0));
     if (warp < kWarps && lane < C::kStages) {
         mbar_init(&full[warp][lane], kGroup);
         mbar_init(&empty[warp][lane], 1);
     }
     if (tid == 0) {
+        mbar_init(&q_full[0], 1);
+        mbar_init(&q_full[1], 1);
         mbar_init(&states_full, kWarps);
-        mbar_init(&states_empty, kWarps);
+        mbar_init(&states_empty, 1);
+        mbar_init(&edge_done, 1);
         s_abort = 0;
+        s_left_cols = 0;
     }
     fence_barrier_init();
-    mine *= p.seg_per_seq;
-    int upto = mine;
+
+    // ---- the two side warps: the stream's length, this CTA's range of it and the
+    // sequence that it starts in
+    int total = 0, first = 0, end = 0, b0 = 0, before = 0;
+    if (warp >= kWarps) {
+        const int per = (p.batch + 31) / 32;
+        const int q0 = min(p.batch, lane * per), q1 = min(p.batch, q0 + per);
+        int mine = 0;
+        for (int b = q0; b < q1; ++b)
+            mine += pages_of(tokens_of(p, b, cta == 0 && warp == kEdgeWarp));
+        mine *= p.seg_per_seq;
+        int upto = mine;
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, upto, d);
-        if (lane >= d) upto += u;
-    }
-    if (lane == 31) s_sum[warp] = upto;
-    __syncthreads();
-    int total = 0;
-#pragma unroll
-    for (int w = 0; w <= kWarps; ++w) {
-        if (w < warp) upto += s_sum[w];
-        total += s_sum[w];
-    }
-    const Cut cut(total, gridDim.x);
-    const int cta = blockIdx.x;
-    const int first = cta < cut.ctas ? cut.start(cta) : total;
-    const int end = cta < cut.ctas ? cut.start(cta + 1) : total;
-    if (first < end && upto - mine <= first && first < upto) {
-        int before = upto - mine, b = q0;
-        for (;; ++b) {
-            const int k = pages_of(tokens_of(p, b, false)) * p.seg_per_seq;
-            if (first < before + k) break;
-            before += k;
+        for (int d = 1; d < 32; d <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += u;
         }
-        s_b0 = b;
-        s_before = before;
+        total = __shfl_sync(0xffffffffu, upto, 31);
+        const Cut cut(p, total, gridDim.x);
+        if (cta < cut.ctas) {
+            first = cut.start(cta);
+            end = cut.start(cta + 1);
+        }
+        if (first < end) {
+            const int at = __ffs(__ballot_sync(0xffffffffu, upto > first)) - 1;
+            before = __shfl_sync(0xffffffffu, upto - mine, at);
+            for (b0 = at * per;; ++b0) {
+                const int k = pages_of(tokens_of(p, b0, false)) * p.seg_per_seq;
+                if (first < before + k) break;
+                before += k;
+            }
+        }
     }
     __syncthreads();
     if (p.pdl_mode == 2) griddep_wait();
 
-    // ---- rows of sequences without tokens are zeros
-    for (int b = cta; b < p.batch; b += gridDim.x) {
-        if (tokens_of(p, b, false) > 0) continue;
-        const int width = p.num_q_heads * HD;
-        for (int i = tid; i < p.tokens * width; i += kThreads)
-            p.out[((int64_t)b * p.tokens + i / width) * p.out_stride + i % width] =
-                __float2bfloat16(0.f);
-    }
-    if (first >= end) return;
-
-    if (warp == kWarps) {
+    if (warp == kLoadWarp) {
         // ---- loads: lane 2 w + k brings page k of each of warp w's groups, which are
         // group w, w + kWarps, ... of every chunk
+        if (first >= end) return;
         static_assert(kGroup * kWarps <= 32);
         const int w = lane / kGroup, k = lane % kGroup;
         const int64_t page_stride = kv4_offset(1, 0, 0, p.num_layers, p.num_kv_heads, HD);
         const uint32_t dst0 = smem_u32(smem) + w * C::kStages * C::kStage + k * C::kPage;
         Walk lw;
-        lw.start(p, first, s_b0, s_before);
+        lw.start(p, first, b0, before);
         bool more = lane < kGroup * kWarps && lw.next(p, end);
         int base = w * kGroup;  // first page of the next group, within its chunk
         int phys = -1;          // this lane's table entry in it, -1: no page
@@ -354,8 +502,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
                 if (*(volatile int *)&s_abort) break;
             }
         }
-        // After a timeout the consumers may leave stages unread: no copy may land in
-        // a CTA that is gone.
+        // After a timeout the computing warps may leave stages unread: no copy may land
+        // in a CTA that is gone.
         __syncwarp();
         if (*(volatile int *)&s_abort && lane < kGroup * kWarps)
             for (int i = max(0, issued - C::kStages); i < issued; ++i)
@@ -363,170 +511,143 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
         return;
     }
 
-    // ---- chunks
-    const int pi0 = g & 1 ? 7 - (g >> 1) : g >> 1;  // token of tile row g
-    const uint8_t *ring = smem + warp * C::kStages * C::kStage;
-    float *states = reinterpret_cast<float *>(smem + C::kRing);  // [kWarps][kCols][kRow]
-    int stage = 0;
-    uint32_t phase = 0;
-    Walk cw, done{};  // the current chunk, and the one whose end is not written yet
-    bool open = false;
-    uint32_t chunk = 0;
-
-    // Joins the warps' states of chunk `done` for this warp's columns and writes the
-    // rows, or pieces of them.
-    auto finish = [&]() {
-        const bool ok = mbar_wait_bounded(&states_full, (chunk - 1) & 1, &s_abort, p.status);
-        constexpr int kPer = HD / 32;  // dims per lane
-        const int kvh = done.seg / p.slices, col0 = (done.seg - kvh * p.slices) * kCols;
-        float top[NT], sum[NT], acc[NT][kPer];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int c = nt * 8 + warp;
-            float2 ml[kWarps];
-            top[nt] = -INFINITY, sum[nt] = 0.f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                ml[w] = s_ml[w][c];
-                top[nt] = fmaxf(top[nt], ml[w].x);
-            }
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) acc[nt][i] = 0.f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                if (ml[w].x == -INFINITY) continue;  // saw nothing of this column
-                const float r = ex2(ml[w].x - top[nt]);
-                sum[nt] = fmaf(ml[w].y, r, sum[nt]);
-                const float *src = states + (w * kCols + c) * C::kRow + lane * kPer;
-#pragma unroll
-                for (int i = 0; i < kPer; ++i) acc[nt][i] = fmaf(src[i], r, acc[nt][i]);
-            }
+    if (warp == kEdgeWarp) {
+        // ---- rows of sequences without tokens are zeros
+        for (int b = cta; b < p.batch; b += gridDim.x) {
+            if (tokens_of(p, b, false) > 0) continue;
+            const int width = p.num_q_heads * HD;
+            for (int i = lane; i < p.tokens * width; i += 32)
+                p.out[((int64_t)b * p.tokens + i / width) * p.out_stride + i % width] =
+                    __float2bfloat16(0.f);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&states_empty);
-        if (!ok) return;
-
-        const int seg = done.b * p.seg_per_seq + done.seg, pages = pages_of(done.n);
-        const int seg_at = done.at - done.p0;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int c = nt * 8 + warp;
-            if (col0 + c >= p.cols) continue;
-            if (done.take != pages) {
-                float *po = p.ws_o + ((int64_t)(seg + cta) * kCols + c) * HD + lane * kPer;
-                if constexpr (kPer == 4)
-                    *reinterpret_cast<float4 *>(po) =
-                        make_float4(acc[nt][0], acc[nt][1], acc[nt][2], acc[nt][3]);
-                else
-                    *reinterpret_cast<float2 *>(po) = make_float2(acc[nt][0], acc[nt][1]);
-                if (lane == 0) p.ws_ml[(int64_t)(seg + cta) * kCols + c] = make_float2(top[nt], sum[nt]);
-                const int c0 = cut.owner(seg_at), pieces = cut.owner(seg_at + pages - 1) - c0 + 1;
-                __syncwarp();
-                int last = 0;
-                if (lane == 0) {
-                    int *cnt = p.ws_cnt + (int64_t)seg * kCols + c;
-                    last = atom_add_acq_rel_gpu(cnt, 1) == pieces - 1;
-                    if (last) *cnt = 0;  // ready for the next call
-                }
-                last = __shfl_sync(0xffffffffu, last, 0);
-                if (!last) continue;
-                const float2 *bml = p.ws_ml + (int64_t)(seg + c0) * kCols + c;
-                const float *bo = p.ws_o + ((int64_t)(seg + c0) * kCols + c) * HD + lane * kPer;
-                float high = -INFINITY;
-                for (int k = lane; k < pieces; k += 32) high = fmaxf(high, __ldcg(&bml[k * kCols].x));
-#pragma unroll
-                for (int d = 16; d; d >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, d));
-                sum[nt] = 0.f;
-#pragma unroll
-                for (int i = 0; i < kPer; ++i) acc[nt][i] = 0.f;
-#pragma unroll 4
-                for (int k = 0; k < pieces; ++k) {
-                    const float2 ml = __ldcg(&bml[k * kCols]);
-                    float x[kPer];
-                    if constexpr (kPer == 4) {
-                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(bo + (int64_t)k * kCols * HD));
-                        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-                    } else {
-                        const float2 v = __ldcg(reinterpret_cast<const float2 *>(bo + (int64_t)k * kCols * HD));
-                        x[0] = v.x, x[1] = v.y;
-                    }
-                    const float r = ml.x == -INFINITY ? 0.f : ex2(ml.x - high);
-                    sum[nt] = fmaf(ml.y, r, sum[nt]);
-#pragma unroll
-                    for (int i = 0; i < kPer; ++i) acc[nt][i] = fmaf(x[i], r, acc[nt][i]);
-                }
-            }
-            const int qi = (col0 + c) / p.group, h = col0 + c - qi * p.group;
-            // a row without tokens gets zeros
-            const float r = sum[nt] == 0.f ? 0.f : p.v_scale / sum[nt];
-            bf16 *dst = p.out + ((int64_t)done.b * p.tokens + qi) * p.out_stride +
-                        (int64_t)(kvh * p.group + h) * HD + lane * kPer;
-            uint32_t v[kPer / 2];
-#pragma unroll
-            for (int i = 0; i < kPer / 2; ++i) v[i] = pack_bf16(acc[nt][2 * i] * r, acc[nt][2 * i + 1] * r);
-            if ((reinterpret_cast<uintptr_t>(dst) & (2 * kPer - 1)) == 0) {
-                if constexpr (kPer == 4)
-                    *reinterpret_cast<uint2 *>(dst) = make_uint2(v[0], v[1]);
-                else
-                    *reinterpret_cast<uint32_t *>(dst) = v[0];
-            } else {
-                uint16_t *e = reinterpret_cast<uint16_t *>(dst);
-#pragma unroll
-                for (int i = 0; i < kPer; ++i) e[i] = (uint16_t)(v[i / 2] >> (i % 2 * 16));
-            }
+        const Cut cut(p, total, gridDim.x);
+        if (lane == 0) s_total = total;  // seen with the first chunk's barrier
+        Walk cw;
+        bool more = first < end;
+        if (more) {
+            cw.start(p, first, b0, before);
+            more = cw.next(p, end);
         }
-    };
-
-    cw.start(p, first, s_b0, s_before);
-    while (cw.next(p, end)) {
-        const int kvh = cw.seg / p.slices, col0 = (cw.seg - kvh * p.slices) * kCols;
-        const int ncols = min(kCols, p.cols - col0);
-
-        // q: column c of the slice is query row b * tokens + c / group, head c % group
-        uint32_t qf[NT][kSteps][2];
-        float f[NT][2];
-        int lim[NT][2];
+        if (!more) {
+            if (lane == 0) {
+                s_chunk[0].take = 0;
+                mbar_arrive(&q_full[0]);
+            }
+            return;
+        }
+        ChunkInfo prev{};
+        for (uint32_t chunk = 0; more; ++chunk) {
+            // Buffer chunk & 1 is free: chunk - 2 was joined here in the turn before.
+            const int buf = chunk & 1;
+            ChunkInfo ch{cw.b, cw.seg, cw.p0, cw.take, cw.n, cw.at, 0};
+            const int kvh = ch.seg / p.slices, col0 = (ch.seg - kvh * p.slices) * kCols;
+            // q: column c of the slice is query token c / group, head c % group. Lane
+            // (g, t) holds dims t * hd/4 .. of column g, as the products need them.
+            uint4 raw[NT][HD / 32];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int c = nt * 8 + g;
-            uint4 raw[HD / 32];
-            if (c < ncols) {
-                const int i = (col0 + c) / p.group, h = (col0 + c) - i * p.group;
-                const bf16 *src = p.q + ((int64_t)cw.b * p.tokens + i) * p.q_stride +
+            for (int nt = 0; nt < NT; ++nt) {
+                const int col = col0 + nt * 8 + g;
+                const int i = col / p.group, h = col - i * p.group;
+                const bf16 *src = p.q + ((int64_t)ch.b * p.tokens + i) * p.q_stride +
                                   (int64_t)(kvh * p.group + h) * HD + t * (HD / 4);
 #pragma unroll
-                for (int k = 0; k < HD / 32; ++k) raw[k] = __ldg(reinterpret_cast<const uint4 *>(src) + k);
-            } else {
-#pragma unroll
-                for (int k = 0; k < HD / 32; ++k) raw[k] = make_uint4(0, 0, 0, 0);
+                for (int k = 0; k < HD / 32; ++k)
+                    raw[nt][k] = col < p.cols ? __ldg(reinterpret_cast<const uint4 *>(src) + k)
+                                              : make_uint4(0, 0, 0, 0);
             }
-            const uint32_t *r = reinterpret_cast<const uint32_t *>(raw);
-            uint32_t top = 0;  // largest magnitude, as bf16 bits
+            more = cw.next(p, end);
+            ch.last = !more;
 #pragma unroll
-            for (int k = 0; k < HD / 8; ++k)
-                top = max(top, max(r[k] & 0x7fffu, (r[k] >> 16) & 0x7fffu));
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const int e = top ? (int)(top >> 7) - 127 : 0;
-            const float down = ldexpf(1.f, -e);
-            // never zero, so that a masked score stays -inf
-            const float fc = fmaxf(p.scale_log2 * ldexpf(1.f, e), FLT_MIN);
+            for (int nt = 0; nt < NT; ++nt) {
+                const uint32_t *r = reinterpret_cast<const uint32_t *>(raw[nt]);
+                uint32_t top = 0;  // largest magnitude, as bf16 bits
 #pragma unroll
-            for (int k = 0; k < HD / 8; ++k) {
-                const float lo = __uint_as_float(r[k] << 16) * down;
-                const float hi = __uint_as_float(r[k] & 0xffff0000u) * down;
-                const __half2 v = __floats2half2_rn(lo, hi);
-                qf[nt][k / 2][k & 1] = *reinterpret_cast<const uint32_t *>(&v) ^ p.q_sign;
+                for (int k = 0; k < HD / 8; ++k)
+                    top = max(top, max(r[k] & 0x7fffu, (r[k] >> 16) & 0x7fffu));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const int e = top ? (int)(top >> 7) - 127 : 0;
+                const float down = ldexpf(1.f, -e);
+                // never zero, so that a masked score stays -inf
+                if (t == 0)
+                    s_f[buf][nt * 8 + g] = fmaxf(p.scale_log2 * ldexpf(1.f, e), FLT_MIN);
+                uint2 *dst = reinterpret_cast<uint2 *>(q_ops + buf * C::kQ) + nt * kSteps * 32 + lane;
+#pragma unroll
+                for (int k = 0; k < HD / 16; ++k) {
+                    uint32_t v[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t x = r[2 * k + i];
+                        const __half2 y = __floats2half2_rn(__uint_as_float(x << 16) * down,
+                                                            __uint_as_float(x & 0xffff0000u) * down);
+                        v[i] = *reinterpret_cast<const uint32_t *>(&y) ^ p.q_sign;
+                    }
+                    dst[k * 32] = make_uint2(v[0], v[1]);
+                }
             }
+            if (lane == 0) s_chunk[buf] = ch;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full[buf]);
+
+            if (chunk > 0) {
+                if (!mbar_wait_bounded(&states_full, (chunk - 1) & 1, &s_abort, p.status)) return;
+                const bool whole = prev.take == pages_of(prev.n);
+                const int64_t seg = (int64_t)prev.b * p.seg_per_seq + prev.seg;
+#pragma unroll 2
+                for (int c = 0; c < kCols; ++c) {
+                    Joined<HD, NT> j;
+                    join_states<HD, NT>(s_ml, states, c, lane, j);
+                    if (whole)
+                        write_row<HD, NT>(p, prev, c, lane, j);
+                    else
+                        store_piece<HD, NT>(p, seg + cta, c, lane, j);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&states_empty);
+                if (!whole) {  // the CTA's first chunk, the end of a segment
+                    int c0;
+                    const int pieces = pieces_of(cut, prev, c0);
+                    const bool mine = lane < kCols && last_piece<kCols>(p, seg, lane, pieces);
+                    const uint32_t cols = __ballot_sync(0xffffffffu, mine);
+                    if (lane == 0 && cols) {
+                        s_left = prev;
+                        s_left_cols = cols;
+                    }
+                }
+            }
+            prev = ch;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&edge_done);
+        return;
+    }
+
+    // ---- computing warps
+    const int pi0 = g & 1 ? 7 - (g >> 1) : g >> 1;  // token of tile row g
+    const uint8_t *ring = smem + warp * C::kStages * C::kStage;
+    int stage = 0;
+    uint32_t phase = 0;
+    for (uint32_t chunk = 0;; ++chunk) {
+        const int buf = chunk & 1;
+        if (!mbar_wait_bounded(&q_full[buf], chunk >> 1 & 1, &s_abort, p.status)) return;
+        const ChunkInfo &info = s_chunk[buf];
+        const int take = info.take, p0 = info.p0, n = info.n;
+        if (take == 0) return;
+        const uint2 *qs = reinterpret_cast<const uint2 *>(q_ops + buf * C::kQ) + lane;
+        float f[NT][2];
+        int lim[NT][2];  // tokens that a column sees
+        // Tokens that every column sees, and those of the chunk's pages.
+        const int col0 = info.seg % p.slices * kCols;
+        const int all = n - (p.tokens - 1 - col0 / p.group);
+        const int held = min(n, (p0 + take) * kBlockSize);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                f[nt][k] = __shfl_sync(0xffffffffu, fc, (2 * t + k) * 4);
-                const int cc = col0 + nt * 8 + 2 * t + k;
-                lim[nt][k] = cw.n - (p.tokens - 1 - min(cc, p.cols - 1) / p.group);
+                const int c = nt * 8 + 2 * t + k;
+                f[nt][k] = s_f[buf][c];
+                lim[nt][k] = min(held, n - (p.tokens - 1 - min(col0 + c, p.cols - 1) / p.group));
             }
-        }
-        // tokens that every column sees
-        const int all = cw.n - (p.tokens - 1 - col0 / p.group);
 
         float o[kSteps][NT][4];
         float m[NT][2], l[NT][2];
@@ -541,44 +662,55 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
                 for (int k = 0; k < 4; ++k) o[j][nt][k] = 0.f;
         }
 
-        for (int base = warp * kGroup; base < cw.take; base += kGroup * kWarps) {
-            const int tok0 = (cw.p0 + base) * kBlockSize;
+        // One group. kTail: it reaches past the tokens that every column sees, or past
+        // the chunk (a page that was not loaded is masked; its stage holds anything).
+        auto group = [&](auto tail_c, int base) {
+            constexpr bool kTail = decltype(tail_c)::value;
+            const int tok0 = (p0 + base) * kBlockSize;
             // after a timeout the stage holds anything; the status word says so
             mbar_wait_bounded(&full[warp][stage], phase, &s_abort, p.status);
             const uint8_t *st = ring + stage * C::kStage;
 
             // S^T = K . Q^T
             float s[kGroup][NT][4];
+            uint32_t wa[kGroup][kWords], wb[kGroup][kWords], sa[kGroup][2], sb[kGroup][2];
 #pragma unroll
             for (int pg = 0; pg < kGroup; ++pg) {
                 const uint8_t *kp = st + pg * C::kPage;
-                uint32_t wa[kWords], wb[kWords], sa[2], sb[2];
                 if constexpr (HD == 128) {
                     const uint4 a = *reinterpret_cast<const uint4 *>(kp + pi0 * 64 + t * 16);
                     const uint4 b = *reinterpret_cast<const uint4 *>(kp + (pi0 + 8) * 64 + t * 16);
-                    wa[0] = a.x, wa[1] = a.y, wa[2] = a.z, wa[3] = a.w;
-                    wb[0] = b.x, wb[1] = b.y, wb[2] = b.z, wb[3] = b.w;
+                    wa[pg][0] = a.x, wa[pg][1] = a.y, wa[pg][2] = a.z, wa[pg][3] = a.w;
+                    wb[pg][0] = b.x, wb[pg][1] = b.y, wb[pg][2] = b.z, wb[pg][3] = b.w;
                     const uint8_t *sc = kp + kv4_code_bytes(HD) + pi0 * 8 + t * 2;
                     const uint32_t ha = e4m3x2_to_half(*reinterpret_cast<const uint16_t *>(sc));
                     const uint32_t hb = e4m3x2_to_half(*reinterpret_cast<const uint16_t *>(sc + 64));
-                    sa[0] = __byte_perm(ha, 0, 0x1010), sa[1] = __byte_perm(ha, 0, 0x3232);
-                    sb[0] = __byte_perm(hb, 0, 0x1010), sb[1] = __byte_perm(hb, 0, 0x3232);
+                    sa[pg][0] = both_low(ha), sa[pg][1] = both_high(ha);
+                    sb[pg][0] = both_low(hb), sb[pg][1] = both_high(hb);
                 } else {
                     const uint2 a = *reinterpret_cast<const uint2 *>(kp + pi0 * 32 + t * 8);
                     const uint2 b = *reinterpret_cast<const uint2 *>(kp + (pi0 + 8) * 32 + t * 8);
-                    wa[0] = a.x, wa[1] = a.y;
-                    wb[0] = b.x, wb[1] = b.y;
+                    wa[pg][0] = a.x, wa[pg][1] = a.y;
+                    wb[pg][0] = b.x, wb[pg][1] = b.y;
                     const uint8_t *sc = kp + kv4_code_bytes(HD) + pi0 * 4 + t;
                     const uint32_t h = e4m3x2_to_half(sc[0] | sc[32] << 8);
-                    sa[0] = __byte_perm(h, 0, 0x1010);
-                    sb[0] = __byte_perm(h, 0, 0x3232);
+                    sa[pg][0] = both_low(h);
+                    sb[pg][0] = both_high(h);
                 }
+            }
 #pragma unroll
-                for (int w = 0; w < kWords; ++w) {
+            for (int w = 0; w < kWords; ++w) {
+                uint2 qf[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) qf[nt][k] = qs[(nt * kSteps + 2 * w + k) * 32];
+#pragma unroll
+                for (int pg = 0; pg < kGroup; ++pg) {
                     uint32_t ha[4], hb[4];
-                    e2m1x8_to_half(wa[w], ha);
-                    e2m1x8_to_half(wb[w], hb);
-                    const uint32_t fa = sa[w / 2], fb = sb[w / 2];
+                    e2m1x8_to_half(wa[pg][w], ha);
+                    e2m1x8_to_half(wb[pg][w], hb);
+                    const uint32_t fa = sa[pg][w / 2], fb = sb[pg][w / 2];
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
                         const uint32_t a0 = hmul2(ha[2 * k], fa), a2 = hmul2(ha[2 * k + 1], fa);
@@ -586,18 +718,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
                             if (w + k == 0)
-                                mma_f16_first(s[pg][nt], a0, a1, a2, a3, qf[nt][0][0], qf[nt][0][1]);
+                                mma_f16_first(s[pg][nt], a0, a1, a2, a3, qf[nt][k].x, qf[nt][k].y);
                             else
-                                mma_f16(s[pg][nt], a0, a1, a2, a3, qf[nt][2 * w + k][0],
-                                        qf[nt][2 * w + k][1]);
+                                mma_f16(s[pg][nt], a0, a1, a2, a3, qf[nt][k].x, qf[nt][k].y);
                     }
                 }
             }
-            // A group that reaches past the tokens that all columns see. A page past
-            // the chunk is masked as well; its stage holds anything.
-            const int held = min(cw.n, (cw.p0 + cw.take) * kBlockSize);
-            const bool tail = tok0 + kGroup * kBlockSize > min(all, held);
-            if (tail) {
+            if constexpr (kTail) {
 #pragma unroll
                 for (int pg = 0; pg < kGroup; ++pg)
 #pragma unroll
@@ -605,7 +732,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             if (tok0 + pg * kBlockSize + pi0 + (k >> 1) * 8 >=
-                                min(lim[nt][k & 1], held))
+                                lim[nt][k & 1])
                                 s[pg][nt][k] = -INFINITY;
             }
 
@@ -669,7 +796,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
                 const int sg = g * (HD / 8) / kKv4Group;  // scale of this lane's dims
                 uint32_t s01 = sc[t * kRowScales + sg] | sc[(7 - t) * kRowScales + sg] << 8;
                 uint32_t s23 = sc[(8 + t) * kRowScales + sg] | sc[(15 - t) * kRowScales + sg] << 8;
-                if (tail) {
+                if constexpr (kTail) {
                     // tokens past the end hold anything: their scales become zero
                     const int left = held - tok0 - pg * kBlockSize;
                     if (t >= left) s01 &= 0xff00u;
@@ -740,14 +867,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
                 stage = 0;
                 phase ^= 1;
             }
-            if (open) {
-                finish();
-                open = false;
-            }
-        }
+        };
+        int base = warp * kGroup;
+        const int plain = (min(all, held) / kBlockSize - p0) - kGroup;  // last base without a tail
+        for (; base <= plain; base += kGroup * kWarps) group(std::false_type(), base);
+        for (; base < take; base += kGroup * kWarps) group(std::true_type(), base);
 
         // ---- the chunk's end: leave this warp's state for the join
-        if (open) finish();
         if (chunk > 0) mbar_wait_bounded(&states_empty, (chunk - 1) & 1, &s_abort, p.status);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -763,13 +889,48 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
                     *reinterpret_cast<float4 *>(dst + 2 * j) = make_float4(
                         o[j][nt][k], o[j][nt][k + 2], o[j + 1][nt][k], o[j + 1][nt][k + 2]);
             }
+        const bool last = info.last;
         __syncwarp();
         if (lane == 0) mbar_arrive(&states_full);
-        ++chunk;
-        done = cw;
-        open = true;
+        if (!last) continue;
+        if (!mbar_wait_bounded(&states_full, chunk & 1, &s_abort, p.status)) return;
+        const ChunkInfo ch = s_chunk[buf];
+        const Cut cut(p, s_total, gridDim.x);
+        const bool whole = ch.take == pages_of(ch.n);
+        const int64_t seg = (int64_t)ch.b * p.seg_per_seq + ch.seg;
+        int c0 = 0, pieces = 0;
+        if (!whole) pieces = pieces_of(cut, ch, c0);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int c = nt * 8 + warp;
+            Joined<HD, NT> j;
+            join_states<HD, NT>(s_ml, states, c, lane, j);
+            if (!whole) {
+                store_piece<HD, NT>(p, seg + cta, c, lane, j);
+                __syncwarp();
+                const int mine = lane == 0 && last_piece<kCols>(p, seg, c, pieces);
+                if (!__shfl_sync(0xffffffffu, mine, 0)) continue;
+                join_pieces<HD, NT>(p, seg + c0, pieces, c, lane, j);
+            }
+            write_row<HD, NT>(p, ch, c, lane, j);
+        }
+        if (chunk == 0 || !mbar_wait_bounded(&edge_done, 0, &s_abort, p.status)) return;
+        const uint32_t left = s_left_cols;
+        if (!left) return;
+        const ChunkInfo lc = s_left;
+        pieces = pieces_of(cut, lc, c0);
+        __syncwarp();
+        __threadfence();  // the edge warp's count saw the pieces; now this warp's reads do
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int c = nt * 8 + warp;
+            if (!(left >> c & 1)) continue;
+            Joined<HD, NT> j;
+            join_pieces<HD, NT>(p, (int64_t)lc.b * p.seg_per_seq + lc.seg + c0, pieces, c, lane, j);
+            write_row<HD, NT>(p, lc, c, lane, j);
+        }
+        return;
     }
-    if (open) finish();
 }
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
