@@ -57,6 +57,7 @@ constexpr int kEdgeWarp = kWarps + 1;  // one for the chunks' ends
 constexpr int kThreads = (kWarps + 2) * 32;
 constexpr int kGroup = 2;             // pages of one warp at a time
 constexpr int kMinPages = kWarps * kGroup;  // pages per CTA at least
+constexpr int kEdgeUnits = 24;
 constexpr float kLazy = 8.f;  // p may reach 2^8 before O and l are rescaled
 
 struct DecodeKv4Params {
@@ -169,12 +170,22 @@ __device__ __forceinline__ int pages_of(int tokens) {
     return (tokens + kBlockSize - 1) / kBlockSize;
 }
 
-// The stream of `total` pages over `ctas` CTAs: CTA c takes the pages from
-// total * c / ctas on.
+// Units of one segment in the stream: its pages and, before them, kEdgeUnits
+// without a page, about what a chunk's two ends cost in page times; without them
+// a CTA whose pages lie in many short segments takes longer than the others. A
+// single sequence fills no CTA with several segments and has none.
+__device__ __forceinline__ int edge_units(const DecodeKv4Params &p) {
+    return p.batch > 1 ? kEdgeUnits : 0;
+}
+__device__ __forceinline__ int units_of(const DecodeKv4Params &p, int tokens) {
+    return tokens > 0 ? pages_of(tokens) + edge_units(p) : 0;
+}
+
+// The stream over `ctas` CTAs: CTA c takes the units from total * c / ctas on.
 struct Cut {
     int total, ctas;
-    __device__ __forceinline__ Cut(const DecodeKv4Params &p, int pages, int max_ctas) {
-        total = pages;
+    __device__ __forceinline__ Cut(const DecodeKv4Params &p, int units, int max_ctas) {
+        total = units;
         ctas = max(1, min(max_ctas, (total + kMinPages - 1) / kMinPages));
         // One sequence on part of the GPU: whole CTAs per segment, so that none of them
         // joins two segments in turn.
@@ -183,50 +194,53 @@ struct Cut {
     __device__ __forceinline__ int start(int cta) const {
         return (int)((long long)total * cta / ctas);
     }
-    __device__ __forceinline__ int owner(int page) const {
-        return (int)((((long long)page + 1) * ctas - 1) / total);
+    __device__ __forceinline__ int owner(int unit) const {
+        return (int)((((long long)unit + 1) * ctas - 1) / total);
     }
 };
 
 // Where a walk over a CTA's range of the stream stands: the chunk, pages
-// [p0, p0 + take) of segment seg of sequence b, which holds n tokens.
+// [p0, p0 + take) of segment seg of sequence b, which holds n tokens and starts
+// at unit seg_at.
 struct Walk {
     int b, seg, p0, take, n;
-    int at;         // stream index of page p0
-    int next_page;  // page of (b, seg) that the next chunk starts with
+    int seg_at;
+    int unit;  // next unit of the stream
 
     __device__ __forceinline__ void start(const DecodeKv4Params &p, int first, int b0, int before_b0) {
         b = b0;
         n = tokens_of(p, b, false);
-        const int off = first - before_b0, pages = max(pages_of(n), 1);
-        seg = off / pages;
-        next_page = off - seg * pages;
-        at = first;
+        const int units = units_of(p, n);  // not zero
+        seg = (first - before_b0) / units;
+        seg_at = before_b0 + seg * units;
+        unit = first;
         p0 = take = 0;
     }
     // Moves to the next chunk of [.., end); false when there is none.
     __device__ __forceinline__ bool next(const DecodeKv4Params &p, int end) {
-        at += take;
-        if (at >= end) return false;
-        int pages = pages_of(n);
-        while (next_page >= pages) {  // the segment is done (or the sequence is empty)
-            next_page = 0;
-            if (pages == 0 || ++seg == p.seg_per_seq) {
-                seg = 0;
-                n = tokens_of(p, ++b, false);
-                pages = pages_of(n);
+        while (unit < end) {
+            const int units = units_of(p, n);
+            if (unit >= seg_at + units) {  // the segment is done (or the sequence is empty)
+                seg_at += units;
+                if (units == 0 || ++seg == p.seg_per_seq) {
+                    seg = 0;
+                    n = tokens_of(p, ++b, false);
+                }
+                continue;
             }
+            const int pages_at = seg_at + edge_units(p), stop = min(seg_at + units, end);
+            p0 = max(unit - pages_at, 0);
+            take = stop - pages_at - p0;
+            unit = stop;
+            if (take > 0) return true;
         }
-        p0 = next_page;
-        take = min(pages - p0, end - at);
-        next_page = p0 + take;
-        return true;
+        return false;
     }
 };
 
 // What the edge warp tells the computing warps about a chunk.
 struct ChunkInfo {
-    int b, seg, p0, take, n, at, last;
+    int b, seg, p0, take, n, seg_at, last;
 };
 
 template <int HD, int NT>
@@ -345,10 +359,10 @@ __device__ __forceinline__ void join_pieces(const DecodeKv4Params &p, int64_t pl
 }
 
 // The pieces of a chunk's segment: the CTA of the first one, and how many.
-__device__ __forceinline__ int pieces_of(const Cut &cut, const ChunkInfo &ch, int &c0) {
-    const int seg_at = ch.at - ch.p0;
-    c0 = cut.owner(seg_at);
-    return cut.owner(seg_at + pages_of(ch.n) - 1) - c0 + 1;
+__device__ __forceinline__ int pieces_of(const DecodeKv4Params &p, const Cut &cut, const ChunkInfo &ch, int &c0) {
+    const int first = ch.seg_at + edge_units(p);
+    c0 = cut.owner(first);
+    return cut.owner(first + pages_of(ch.n) - 1) - c0 + 1;
 }
 
 template <int HD, int NT>
@@ -401,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
         const int q0 = min(p.batch, lane * per), q1 = min(p.batch, q0 + per);
         int mine = 0;
         for (int b = q0; b < q1; ++b)
-            mine += pages_of(tokens_of(p, b, cta == 0 && warp == kEdgeWarp));
+            mine += units_of(p, tokens_of(p, b, cta == 0 && warp == kEdgeWarp));
         mine *= p.seg_per_seq;
         int upto = mine;
 #pragma unroll
@@ -419,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
             const int at = __ffs(__ballot_sync(0xffffffffu, upto > first)) - 1;
             before = __shfl_sync(0xffffffffu, upto - mine, at);
             for (b0 = at * per;; ++b0) {
-                const int k = pages_of(tokens_of(p, b0, false)) * p.seg_per_seq;
+                const int k = units_of(p, tokens_of(p, b0, false)) * p.seg_per_seq;
                 if (first < before + k) break;
                 before += k;
             }
@@ -535,26 +549,30 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
             }
             return;
         }
-        ChunkInfo prev{};
-        for (uint32_t chunk = 0; more; ++chunk) {
-            // Buffer chunk & 1 is free: chunk - 2 was joined here in the turn before.
-            const int buf = chunk & 1;
-            ChunkInfo ch{cw.b, cw.seg, cw.p0, cw.take, cw.n, cw.at, 0};
-            const int kvh = ch.seg / p.slices, col0 = (ch.seg - kvh * p.slices) * kCols;
-            // q: column c of the slice is query token c / group, head c % group. Lane
-            // (g, t) holds dims t * hd/4 .. of column g, as the products need them.
-            uint4 raw[NT][HD / 32];
+        // q: column c of the slice is query token c / group, head c % group. Lane (g, t)
+        // holds dims t * hd/4 .. of column g, as the products need them. A chunk's rows
+        // are read while the chunk before it is prepared and the one before that joined.
+        uint4 raw[NT][HD / 32];
+        auto read_q = [&]() {
+            const int kvh = cw.seg / p.slices, col0 = (cw.seg - kvh * p.slices) * kCols;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 const int col = col0 + nt * 8 + g;
                 const int i = col / p.group, h = col - i * p.group;
-                const bf16 *src = p.q + ((int64_t)ch.b * p.tokens + i) * p.q_stride +
+                const bf16 *src = p.q + ((int64_t)cw.b * p.tokens + i) * p.q_stride +
                                   (int64_t)(kvh * p.group + h) * HD + t * (HD / 4);
 #pragma unroll
                 for (int k = 0; k < HD / 32; ++k)
                     raw[nt][k] = col < p.cols ? __ldg(reinterpret_cast<const uint4 *>(src) + k)
                                               : make_uint4(0, 0, 0, 0);
             }
+        };
+        read_q();
+        ChunkInfo prev{};
+        for (uint32_t chunk = 0; more; ++chunk) {
+            // Buffer chunk & 1 is free: chunk - 2 was joined here in the turn before.
+            const int buf = chunk & 1;
+            ChunkInfo ch{cw.b, cw.seg, cw.p0, cw.take, cw.n, cw.seg_at, 0};
             more = cw.next(p, end);
             ch.last = !more;
 #pragma unroll
@@ -588,6 +606,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
             if (lane == 0) s_chunk[buf] = ch;
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_full[buf]);
+            if (more) read_q();
 
             if (chunk > 0) {
                 if (!mbar_wait_bounded(&states_full, (chunk - 1) & 1, &s_abort, p.status)) return;
@@ -606,7 +625,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
                 if (lane == 0) mbar_arrive(&states_empty);
                 if (!whole) {  // the CTA's first chunk, the end of a segment
                     int c0;
-                    const int pieces = pieces_of(cut, prev, c0);
+                    const int pieces = pieces_of(p, cut, prev, c0);
                     const bool mine = lane < kCols && last_piece<kCols>(p, seg, lane, pieces);
                     const uint32_t cols = __ballot_sync(0xffffffffu, mine);
                     if (lane == 0 && cols) {
@@ -899,7 +918,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
         const bool whole = ch.take == pages_of(ch.n);
         const int64_t seg = (int64_t)ch.b * p.seg_per_seq + ch.seg;
         int c0 = 0, pieces = 0;
-        if (!whole) pieces = pieces_of(cut, ch, c0);
+        if (!whole) pieces = pieces_of(p, cut, ch, c0);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int c = nt * 8 + warp;
@@ -918,7 +937,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
         const uint32_t left = s_left_cols;
         if (!left) return;
         const ChunkInfo lc = s_left;
-        pieces = pieces_of(cut, lc, c0);
+        pieces = pieces_of(p, cut, lc, c0);
         __syncwarp();
         __threadfence();  // the edge warp's count saw the pieces; now this warp's reads do
 #pragma unroll
@@ -961,7 +980,7 @@ int launch(DecodeKv4Params p, int max_context_len, cudaStream_t stream) {
     p.slices = (p.cols + C::kCols - 1) / C::kCols;
     p.seg_per_seq = p.num_kv_heads * p.slices;
     // the stream's indexes are int32
-    if ((int64_t)p.batch * p.table_stride > INT_MAX / p.seg_per_seq) return LC_ERR_UNSUPPORTED_SHAPE;
+    if ((int64_t)p.batch * (p.table_stride + kEdgeUnits) > INT_MAX / p.seg_per_seq) return LC_ERR_UNSUPPORTED_SHAPE;
     int64_t grid = (int64_t)sm_count() * C::kCtasPerSm;
     if (max_context_len > 0) {  // less work than kMinPages pages per CTA
         const int64_t pages = (int64_t)p.batch * p.seg_per_seq *
