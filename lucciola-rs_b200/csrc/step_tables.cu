@@ -12,10 +12,10 @@
 // Every CTA scans the lengths itself (a few KB from L2) instead of waiting for
 // another one, so the call is one launch without a device-wide barrier. The
 // outputs that a caller may let alias inputs (free_count, the context lengths)
-// are written by whichever CTA is last to have read them: a ticket counts the
-// CTAs past their scan. A step of small calls is launch latency; a wide step is
-// bound by the bytes of the step's table rows and of positions and slots, which
-// are written 16 bytes a thread.
+// are written by whichever CTA is last to have read them: each takes a ticket
+// after its scan and looks at it at its end, when the answer has long come. Small
+// steps are launch latency and three dependent reads; a wide step is bound by the
+// bytes of the table rows, positions and slots, which move 16 bytes a lane.
 #include <algorithm>
 
 #include "lc_common.cuh"
@@ -26,8 +26,9 @@ namespace {
 
 constexpr int kStepThreads = 512;
 constexpr int kStepWarps = kStepThreads / 32;
-constexpr int kStepMaxBatch = 8192;  // three ints of shared memory per request
-constexpr int kRowSegment = 1024;    // table entries a warp copies per task
+constexpr int kStepMaxBatch = 8192;  // four ints of shared memory per request
+constexpr int kTokenSegment = 128;   // token rows of a warp's task
+constexpr int kRowSegment = 128;     // table entries of a warp's task: 16 bytes per lane
 
 struct StepParams {
     int *tables;
@@ -39,7 +40,7 @@ struct StepParams {
     int num_blocks;
     int *step_tables;
     int step_stride;
-    int step_vec;  // step rows start 16-byte aligned
+    int table_vec, step_vec;  // rows start 16-byte aligned
     int *positions, *slot_map;
     int max_tokens, tokens_vec;
     int *row_starts, *ctx_out, *count_out;
@@ -85,24 +86,65 @@ __device__ __forceinline__ void block_scan2(int &x, int &y, int *tx, int *ty) {
     *ty = sy;
 }
 
-// True in the one CTA of the grid that comes last here; it leaves the ticket at
-// zero. Every thread of the CTA has made its reads before (barrier).
-__device__ __forceinline__ bool last_past(int *ticket) {
-    __shared__ int last;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        last = 1;
-        if (gridDim.x > 1) {
-            last = atom_add_acq_rel_gpu(ticket, 1) == (int)gridDim.x - 1;
-            if (last) *ticket = 0;
-        }
-    }
-    __syncthreads();
-    return last != 0;
+// One thread, after the CTA's reads of what the last CTA will overwrite (and a
+// barrier): true in the CTA that comes last. It leaves the ticket at zero.
+__device__ __forceinline__ bool take_ticket(int *ticket) {
+    if (gridDim.x == 1) return true;
+    const bool last = atom_add_acq_rel_gpu(ticket, 1) == (int)gridDim.x - 1;
+    if (last) *ticket = 0;
+    return last;
 }
 
 __device__ __forceinline__ int slot_of(const int *slots, int i) {
     return slots ? __ldg(slots + i) : i;
+}
+
+// Positions and slots of the four token rows from r0 on.
+__device__ __forceinline__ void token_rows(const StepParams &p, const int *start, const int *before,
+                                           const int *cached, const int *slots, int count, int tokens,
+                                           int r0) {
+    if (r0 >= p.max_tokens) return;
+    int b = 0;
+    if (r0 < tokens) {  // the request of row r0: start[b] <= r0 < start[b + 1]
+        int hi = p.batch;
+        while (hi - b > 1) {
+            const int mid = (b + hi) >> 1;
+            if (start[mid] <= r0) b = mid; else hi = mid;
+        }
+    }
+    int pos[4], page[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = r0 + i;
+        pos[i] = page[i] = -1;
+        if (r >= tokens) continue;
+        while (start[b + 1] <= r) ++b;
+        const int c = cached[b];
+        pos[i] = (c < 0 ? -1 - c : c) + r - start[b];
+        if (c < 0) continue;
+        const int j = pos[i] / kBlockSize, have = pages_of(c);
+        const int *at = j < have ? p.tables + (int64_t)slots[b] * p.table_stride + j
+                                 : p.free_pages + (count - 1 - before[b] + have - j);
+        page[i] = *at;
+        if (page[i] < 0 || page[i] >= p.num_blocks) page[i] = -2;  // not a page
+    }
+    int slot[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (page[i] == -2) set_status(p.status, LC_DEV_BAD_BLOCK);
+        slot[i] = page[i] < 0 ? -1 : page[i] * kBlockSize + pos[i] % kBlockSize;
+    }
+    if (p.tokens_vec && r0 + 4 <= p.max_tokens) {
+        *reinterpret_cast<int4 *>(p.positions + r0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+        *reinterpret_cast<int4 *>(p.slot_map + r0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (r0 + i < p.max_tokens) {
+                p.positions[r0 + i] = pos[i];
+                p.slot_map[r0 + i] = slot[i];
+            }
+    }
 }
 
 __global__ void __launch_bounds__(kStepThreads) step_tables_kernel(StepParams p) {
@@ -110,6 +152,7 @@ __global__ void __launch_bounds__(kStepThreads) step_tables_kernel(StepParams p)
     int *start = sm;                  // [batch + 1] first token row of a request
     int *before = start + p.batch + 1;  // [batch] pages that earlier requests need
     int *cached = before + p.batch;   // [batch] cached tokens, -1 - them if refused
+    int *slots = cached + p.batch;    // [batch] slot, -1 if invalid
     const int tid = threadIdx.x, lane = tid & 31;
     const bool first_cta = blockIdx.x == 0;
 
@@ -131,63 +174,56 @@ __global__ void __launch_bounds__(kStepThreads) step_tables_kernel(StepParams p)
             m = 0;  // an invalid request has no rows
         }
         cached[b] = c;
+        slots[b] = slot >= 0 && slot < p.num_slots ? slot : -1;
         start[b] = m;  // its length, until the scan is known
         tok += m;
         need += pages_of(c + m) - pages_of(c);
     }
+    __shared__ int most;  // pages taken: the sum up to the last served request that needs one
+    if (tid == 0) most = 0;
     int tokens, needed;
     block_scan2(tok, need, &tokens, &needed);
+    int taken = 0;
     for (int b = b0; b < b1; ++b) {
         const int c = cached[b], m = start[b], k = pages_of(c + m) - pages_of(c);
         start[b] = tok;
         before[b] = need;
         tok += m;
         need += k;
-        if (k > 0 && need > count) cached[b] = -1 - c;
+        if (k > 0) {
+            if (need > count) cached[b] = -1 - c;
+            else taken = need;
+        }
     }
     if (tid == 0) start[p.batch] = tokens;
+    if (taken) atomicMax(&most, taken);
     if (first_cta && tid == 0) {
         if (needed > count) set_status(p.status, LC_DEV_OUT_OF_BLOCKS);
         if (tokens > p.max_tokens) set_status(p.status, LC_DEV_BAD_POS);
     }
-    if (last_past(p.ticket)) {
-        // taken: the sum up to the last served request that needed a page
-        for (int b = tid; b < p.batch; b += kStepThreads) {
-            const int c = cached[b], m = start[b + 1] - start[b];
-            p.ctx_out[b] = c < 0 ? -1 - c : c + m;
-            p.row_starts[b] = start[b];
-        }
-        int taken = 0;
-        for (int b = tid; b < p.batch; b += kStepThreads) {
-            const int c = cached[b], m = start[b + 1] - start[b];
-            if (c >= 0) {
-                const int k = pages_of(c + m) - pages_of(c);
-                if (k > 0) taken = max(taken, before[b] + k);
-            }
-        }
-        __shared__ int most;
-        if (tid == 0) most = 0;
-        __syncthreads();
-        atomicMax(&most, taken);
-        __syncthreads();
-        if (tid == 0) {
-            p.row_starts[p.batch] = tokens;
-            *p.count_out = count - most;
-        }
-    }
+    __syncthreads();
+    bool last = false;
+    if (tid == 0) last = take_ticket(p.ticket);
 
-    // Table rows: tasks of kRowSegment entries, one warp each.
+    // Tasks of one warp: kRowSegment entries of a table row, then kTokenSegment token
+    // rows, so that in a small step the two kinds run side by side.
     const int warps = gridDim.x * kStepWarps, warp = blockIdx.x * kStepWarps + (tid >> 5);
     const int width = p.step_tables ? max(p.step_stride, p.table_stride) : p.table_stride;
-    const int segs = (width + kRowSegment - 1) / kRowSegment;
-    for (int t = warp; t < p.batch * segs; t += warps) {
+    const int segs = (width + kRowSegment - 1) / kRowSegment, row_tasks = p.batch * segs;
+    const int tasks = row_tasks + (p.max_tokens + kTokenSegment - 1) / kTokenSegment;
+    for (int t = warp; t < tasks; t += warps) {
+        if (t >= row_tasks) {
+            token_rows(p, start, before, cached, slots, count, tokens,
+                       (t - row_tasks) * kTokenSegment + 4 * lane);
+            continue;
+        }
         const int b = t / segs, j0 = (t - b * segs) * kRowSegment;
         const int j1 = min(width, j0 + kRowSegment), s1 = min(p.step_stride, j1);
         const int c = cached[b];
         const int n = c < 0 ? -1 - c : c, m = start[b + 1] - start[b];
         const int have = pages_of(n), want = c < 0 ? have : pages_of(n + m);
-        const int slot = slot_of(p.slots, b);
-        if (slot < 0 || slot >= p.num_slots) {
+        const int slot = slots[b];
+        if (slot < 0) {
             if (p.step_tables)
                 for (int j = j0 + lane; j < s1; j += 32)
                     p.step_tables[(int64_t)b * p.step_stride + j] = -1;
@@ -206,60 +242,32 @@ __global__ void __launch_bounds__(kStepThreads) step_tables_kernel(StepParams p)
         auto entry = [&](int j) {
             return j < min(have, p.table_stride) ? row[j] : j < want ? __ldg(top - j) : -1;
         };
-        if (p.step_vec) {
-            for (int j = j0 + 4 * lane; j < s1; j += 128) {
-                const int4 v = make_int4(entry(j), entry(j + 1), entry(j + 2), entry(j + 3));
-                if (j + 4 <= s1) {
-                    *reinterpret_cast<int4 *>(out + j) = v;
-                } else {
-                    out[j] = v.x;
-                    if (j + 1 < s1) out[j + 1] = v.y;
-                    if (j + 2 < s1) out[j + 2] = v.z;
-                }
-            }
+        const int j = j0 + 4 * lane;
+        if (j >= s1) continue;
+        int4 v;
+        if (p.table_vec && j + 4 <= have)
+            v = *reinterpret_cast<const int4 *>(row + j);
+        else
+            v = make_int4(entry(j), entry(j + 1), entry(j + 2), entry(j + 3));
+        if (p.step_vec && j + 4 <= s1) {
+            *reinterpret_cast<int4 *>(out + j) = v;
         } else {
-            for (int j = j0 + lane; j < s1; j += 32) out[j] = entry(j);
+            out[j] = v.x;
+            if (j + 1 < s1) out[j + 1] = v.y;
+            if (j + 2 < s1) out[j + 2] = v.z;
+            if (j + 3 < s1) out[j + 3] = v.w;
         }
     }
 
-    // Token rows: four consecutive ones per thread.
-    const int threads = gridDim.x * kStepThreads;
-    for (int64_t q = blockIdx.x * kStepThreads + tid; q * 4 < p.max_tokens; q += threads) {
-        const int r0 = (int)(q * 4);
-        int pos[4], slt[4];
-        int b = -1;
-        if (r0 < tokens) {  // the request of row r0: start[b] <= r0 < start[b + 1]
-            int lo = 0, hi = p.batch;
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (start[mid] <= r0) lo = mid; else hi = mid;
-            }
-            b = lo;
+    if (__syncthreads_or(last)) {
+        for (int b = tid; b < p.batch; b += kStepThreads) {
+            const int c = cached[b], m = start[b + 1] - start[b];
+            p.ctx_out[b] = c < 0 ? -1 - c : c + m;
+            p.row_starts[b] = start[b];
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = r0 + i;
-            pos[i] = slt[i] = -1;
-            if (r >= tokens || r >= p.max_tokens) continue;
-            while (start[b + 1] <= r) ++b;
-            const int c = cached[b];
-            pos[i] = (c < 0 ? -1 - c : c) + r - start[b];
-            if (c < 0) continue;
-            const int j = pos[i] / kBlockSize, have = pages_of(c);
-            const int page = j < have
-                                 ? p.tables[(int64_t)slot_of(p.slots, b) * p.table_stride + j]
-                                 : __ldg(p.free_pages + (count - 1 - before[b] + have - j));
-            if (page < 0 || page >= p.num_blocks) set_status(p.status, LC_DEV_BAD_BLOCK);
-            else slt[i] = page * kBlockSize + pos[i] % kBlockSize;
-        }
-        if (p.tokens_vec && r0 + 4 <= p.max_tokens) {
-            *reinterpret_cast<int4 *>(p.positions + r0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
-            *reinterpret_cast<int4 *>(p.slot_map + r0) = make_int4(slt[0], slt[1], slt[2], slt[3]);
-        } else {
-            for (int i = 0; i < 4 && r0 + i < p.max_tokens; ++i) {
-                p.positions[r0 + i] = pos[i];
-                p.slot_map[r0 + i] = slt[i];
-            }
+        if (tid == 0) {
+            p.row_starts[p.batch] = tokens;
+            *p.count_out = count - most;
         }
     }
 }
@@ -297,21 +305,34 @@ __global__ void __launch_bounds__(kStepThreads) step_release_kernel(ReleaseParam
     }
     const int room = p.num_blocks - count;
     if (first_cta && tid == 0 && total > room) set_status(p.status, LC_DEV_BAD_BLOCK);
-    if (last_past(p.ticket) && tid == 0) *p.count_out = count + min(total, room);
+    __syncthreads();
+    bool last = false;
+    if (tid == 0) last = take_ticket(p.ticket);
 
+    // Tasks of kRowSegment pages, one warp each; a request's last page first, so that
+    // the stack hands them out again in order.
     const int warps = gridDim.x * kStepWarps, warp = blockIdx.x * kStepWarps + (tid >> 5);
-    for (int b = warp; b < p.count; b += warps) {
+    const int segs = (p.table_stride + kRowSegment - 1) / kRowSegment;
+    for (int t = warp; t < p.count * segs; t += warps) {
+        const int b = t / segs, j0 = (t - b * segs) * kRowSegment;
         const int n = pages[b];
-        if (n == 0) continue;
+        if (j0 >= n) continue;
         const int *row = p.tables + (int64_t)slot_of(p.slots, b) * p.table_stride;
-        // last page first, so that the stack hands them out again in order
-        for (int j = lane; j < n; j += 32) {
-            const int at = before[b] + n - 1 - j;
-            const int page = row[j];
-            if (page < 0 || page >= p.num_blocks) set_status(p.status, LC_DEV_BAD_BLOCK);
-            if (at < room) p.free_pages[count + at] = page;
+        int page[kRowSegment / 32];
+#pragma unroll
+        for (int i = 0; i < kRowSegment / 32; ++i) {
+            const int j = j0 + lane + 32 * i;
+            page[i] = j < n ? row[j] : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < kRowSegment / 32; ++i) {
+            const int j = j0 + lane + 32 * i, at = before[b] + n - 1 - j;
+            if (j >= n) continue;
+            if (page[i] < 0 || page[i] >= p.num_blocks) set_status(p.status, LC_DEV_BAD_BLOCK);
+            if (at < room) p.free_pages[count + at] = page[i];
         }
     }
+    if (last) *p.count_out = count + min(total, room);
 }
 
 bool aligned4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
@@ -358,6 +379,7 @@ extern "C" int lc_step_tables(int *block_tables, int table_stride, int num_slots
     p.num_blocks = (int)num_blocks;
     p.step_tables = step_tables;
     p.step_stride = step_stride;
+    p.table_vec = aligned16(block_tables) && (table_stride & 3) == 0;
     p.step_vec = step_tables && aligned16(step_tables) && (step_stride & 3) == 0;
     p.positions = positions;
     p.slot_map = slot_map;
@@ -368,16 +390,17 @@ extern "C" int lc_step_tables(int *block_tables, int table_stride, int num_slots
     p.count_out = free_count_out;
     p.ticket = (int *)workspace;
     p.status = dev_status;
-    const int smem = (3 * batch + 1) * (int)sizeof(int);
+    const int smem = (4 * batch + 1) * (int)sizeof(int);
     if (smem > 48 * 1024) {
         const int rc = ensure_smem_attr((const void *)step_tables_kernel, smem);
         if (rc) return rc;
     }
-    // Two rounds of every thread's work per CTA at least, two CTAs per SM at most.
+    // A warp per task, two CTAs per SM at most.
     const int64_t width = step_tables ? std::max(step_stride, table_stride) : table_stride;
-    const int64_t work = std::max<int64_t>((int64_t)batch * ((width + kRowSegment - 1) / kRowSegment) * 32,
-                                           max_tokens / 4);
-    const int grid = (int)std::min<int64_t>((work + 2 * kStepThreads - 1) / (2 * kStepThreads) + 1,
+    const int64_t tasks = (int64_t)batch * ((width + kRowSegment - 1) / kRowSegment) +
+                          ((int64_t)max_tokens + kTokenSegment - 1) / kTokenSegment;
+    if (tasks > INT32_MAX / 2) return LC_ERR_UNSUPPORTED_SHAPE;
+    const int grid = (int)std::min<int64_t>(std::max<int64_t>((tasks + kStepWarps - 1) / kStepWarps, 1),
                                             2 * sm_count());
     step_tables_kernel<<<grid, kStepThreads, smem, as_stream(stream)>>>(p);
     return launch_status();
@@ -407,7 +430,8 @@ extern "C" int lc_step_release(int *free_pages, const int *free_count, int64_t n
         const int rc = ensure_smem_attr((const void *)step_release_kernel, smem);
         if (rc) return rc;
     }
-    const int grid = std::min((count + kStepWarps - 1) / kStepWarps, 2 * sm_count());
+    const int64_t tasks = (int64_t)count * ((table_stride + kRowSegment - 1) / kRowSegment);
+    const int grid = (int)std::min<int64_t>((tasks + kStepWarps - 1) / kStepWarps, 2 * sm_count());
     step_release_kernel<<<std::max(grid, 1), kStepThreads, smem, as_stream(stream)>>>(p);
     return launch_status();
 }
