@@ -16,9 +16,11 @@
 //
 // hd/16 lanes share a head, each with 8 dims of the first half and their 8
 // rotation partners: two 16-byte loads, both halves of a rotation in one
-// thread, a reduction of 2 or 3 shuffles. A warp takes kIter times 32 / (hd/16)
-// heads of one row and issues all their loads first; the row's cos and sin are
-// read once per warp.
+// thread, a reduction of 2 or 3 shuffles. A warp takes 32 / (hd/16) heads of one
+// row at a time and loads the next ones before it works on these, so that a
+// read's latency (the row, and the position before the cos and sin) is not paid
+// once per set of warps that fits the GPU.
+#include <algorithm>
 #include <cfloat>
 #include <climits>
 
@@ -29,6 +31,7 @@ namespace lc {
 namespace {
 
 constexpr int kNormRopeThreads = 128;
+constexpr int kNormRopeCtas = 7;  // per SM: up to 72 registers
 
 struct NormRopeParams {
     bf16 *q_out;
@@ -51,43 +54,73 @@ struct NormRopeParams {
     int *status;
 };
 
-__device__ __forceinline__ void unpack8(const uint4 &u, float (&f)[8]) {
-    const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&u);
+// Pairs of fp32 values, each rounded as a single operation would.
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t pair2(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 split2(uint64_t a) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+    return r;
+}
+__device__ __forceinline__ uint64_t neg2(uint64_t a) { return a ^ 0x8000000080000000ull; }
+
+// Eight bf16 values as four pairs, and back with one rounding.
+__device__ __forceinline__ void unpack8(const uint4 &u, uint64_t (&f)[4]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        f[i] = pair2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+}
+__device__ __forceinline__ uint4 pack8(const uint64_t (&f)[4]) {
+    uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        f[2 * i] = __low2float(h[i]);
-        f[2 * i + 1] = __high2float(h[i]);
+        const float2 x = split2(f[i]);
+        w[i] = pack_bf16(x.x, x.y);
     }
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
-
-__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
-    return make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]),
-                      pack_bf16(f[6], f[7]));
+__device__ __forceinline__ void floats8(const uint64_t (&f)[4], float (&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 v = split2(f[i]);
+        x[2 * i] = v.x, x[2 * i + 1] = v.y;
+    }
 }
 
 __device__ __forceinline__ uint4 ldg16(const bf16 *p) {
     return __ldg(reinterpret_cast<const uint4 *>(p));
 }
 
-__device__ __forceinline__ void load8f(const float *p, float (&f)[8]) {
-    const float4 a = __ldg(reinterpret_cast<const float4 *>(p));
-    const float4 b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+__device__ __forceinline__ void load8f(const float *p, uint64_t (&f)[4]) {
+    const ulonglong2 a = __ldg(reinterpret_cast<const ulonglong2 *>(p));
+    const ulonglong2 b = __ldg(reinterpret_cast<const ulonglong2 *>(p) + 1);
+    f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y;
 }
 
 // 1 / sqrt(mean of squares + eps) of a head, x1 and x2 its two 8-dim pieces in
 // this lane. All lanes of the warp call it.
 template <int HD>
-__device__ __forceinline__ float rms_factor(const float (&x1)[8], const float (&x2)[8], float eps) {
-    float s[8];
+__device__ __forceinline__ float rms_factor(const uint64_t (&x1)[4], const uint64_t (&x2)[4], float eps) {
+    uint64_t s[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-        s[e] = __fadd_rn(__fmul_rn(x1[e], x1[e]), __fmul_rn(x2[e], x2[e]));
-#pragma unroll
-    for (int w = 4; w >= 1; w >>= 1)
-#pragma unroll
-        for (int e = 0; e < w; ++e) s[e] = __fadd_rn(s[e], s[e + w]);
-    float t = s[0];
+    for (int e = 0; e < 4; ++e) s[e] = add2(mul2(x1[e], x1[e]), mul2(x2[e], x2[e]));
+    // dims e and e + 4, then e and e + 2, then the last two
+    const float2 r = split2(add2(add2(s[0], s[2]), add2(s[1], s[3])));
+    float t = __fadd_rn(r.x, r.y);
 #pragma unroll
     for (int w = HD / 32; w >= 1; w >>= 1) t = __fadd_rn(t, __shfl_xor_sync(0xffffffffu, t, w));
     return __frcp_rn(__fsqrt_rn(__fadd_rn(__fmul_rn(t, 1.f / HD), eps)));
@@ -102,106 +135,121 @@ __device__ __forceinline__ uint32_t group_amax(const float (&x)[8]) {
     return max(m, __shfl_xor_sync(0xffffffffu, m, 1));
 }
 
-// kIter: heads a lane works on in one task.
-template <int HD, bool KV4, int kIter>
-__global__ void __launch_bounds__(kNormRopeThreads) norm_rope_append_kernel(NormRopeParams p) {
-    constexpr int kLanes = HD / 16;         // lanes per head
-    constexpr int kHeads = 32 / kLanes;     // heads per warp at a time
+template <int HD, bool KV4>
+__global__ void __launch_bounds__(kNormRopeThreads, kNormRopeCtas) norm_rope_append_kernel(NormRopeParams p) {
+    constexpr int kLanes = HD / 16;      // lanes per head
+    constexpr int kHeads = 32 / kLanes;  // heads per warp at a time
     constexpr int kHalf = HD / 2;
     const int lane = threadIdx.x & 31;
-    const int64_t task = (int64_t)blockIdx.x * (kNormRopeThreads / 32) + (threadIdx.x >> 5);
-    if (task >= (int64_t)p.rows * p.groups) return;
-    const int row = (int)(task / p.groups);
-    const int first = (int)(task - (int64_t)row * p.groups) * kHeads * kIter;
     const int hq = p.num_q_heads, hk = hq + p.num_kv_heads, heads = hk + p.num_kv_heads;
     const int c8 = (lane % kLanes) * 8;
-    const int h0 = first + lane / kLanes;
+    const uint32_t tasks = (uint32_t)p.rows * p.groups;  // kHeads heads of one row each
+    const uint32_t step = gridDim.x * (kNormRopeThreads / 32);
 
-    const bf16 *src = p.qkv + (int64_t)row * p.row_stride + c8;
-    uint4 a[kIter], b[kIter];
-#pragma unroll
-    for (int u = 0; u < kIter; ++u) {
-        const int h = h0 + u * kHeads;
+    struct Task {
+        uint4 a, b;  // this lane's dims of both halves
+        int row, first, pos, slot;
+    };
+    auto fetch = [&](uint32_t task, Task &k) {
+        const uint32_t row = task / (uint32_t)p.groups;
+        k.row = (int)row;
+        k.first = (int)(task - row * p.groups) * kHeads;
+        const int h = k.first + lane / kLanes;
+        k.a = k.b = make_uint4(0, 0, 0, 0);
         if (h < heads) {
             // plain loads: q_out may be these rows
-            a[u] = *reinterpret_cast<const uint4 *>(src + (int64_t)h * HD);
-            b[u] = *reinterpret_cast<const uint4 *>(src + (int64_t)h * HD + kHalf);
-        } else {
-            a[u] = b[u] = make_uint4(0, 0, 0, 0);
+            const bf16 *src = p.qkv + (int64_t)k.row * p.row_stride + (int64_t)h * HD + c8;
+            k.a = *reinterpret_cast<const uint4 *>(src);
+            k.b = *reinterpret_cast<const uint4 *>(src + kHalf);
         }
-    }
-    const int pos = __ldg(p.positions + row), slot = __ldg(p.slot_map + row);
-    if (pos < 0 || pos >= p.rope_rows) {  // -1: a padding row
-        if (pos != -1 && first == 0 && lane == 0) set_status(p.status, LC_DEV_BAD_POS);
-        return;
-    }
-    const bool stored = slot >= 0 && slot < p.num_blocks * kBlockSize;
-    if (!stored && slot != -1 && first == 0 && lane == 0) set_status(p.status, LC_DEV_BAD_BLOCK);
-    const int phys = slot / kBlockSize, off = slot % kBlockSize;
-    float cs[8], sn[8];
-    load8f(p.cos_t + (int64_t)pos * kHalf + c8, cs);
-    load8f(p.sin_t + (int64_t)pos * kHalf + c8, sn);
+        k.pos = __ldg(p.positions + k.row);
+        k.slot = __ldg(p.slot_map + k.row);
+    };
 
-#pragma unroll
-    for (int u = 0; u < kIter; ++u) {
-        const int hw = first + u * kHeads;  // the warp's first head of this turn
-        if (hw >= heads) break;
-        const int h = h0 + u * kHeads;
+    uint32_t task = blockIdx.x * (kNormRopeThreads / 32) + (threadIdx.x >> 5);
+    if (task >= tasks) return;
+    Task next;
+    fetch(task, next);
+    for (; task < tasks; task += step) {
+        const Task cur = next;
+        uint64_t cs[4] = {}, sn[4] = {};
+        const bool pos_ok = cur.pos >= 0 && cur.pos < p.rope_rows;
+        if (pos_ok && cur.first < hk) {
+            load8f(p.cos_t + (int64_t)cur.pos * kHalf + c8, cs);
+            load8f(p.sin_t + (int64_t)cur.pos * kHalf + c8, sn);
+        }
+        if (task + step < tasks) fetch(task + step, next);
+        if (!pos_ok) {  // -1: a padding row
+            if (cur.pos != -1 && cur.first == 0 && lane == 0) set_status(p.status, LC_DEV_BAD_POS);
+            continue;
+        }
+        const bool stored = cur.slot >= 0 && cur.slot < p.num_blocks * kBlockSize;
+        if (!stored && cur.slot != -1 && cur.first == 0 && lane == 0)
+            set_status(p.status, LC_DEV_BAD_BLOCK);
+        const int phys = cur.slot / kBlockSize, off = cur.slot % kBlockSize;
+
+        const int h = cur.first + lane / kLanes;
         const bool is_q = h < hq, is_v = h >= hk;
         const int hl = is_q ? h : is_v ? h - hk : h - hq;  // head within its part
-        float x1[8], x2[8];
-        unpack8(a[u], x1);
-        unpack8(b[u], x2);
+        uint64_t x1[4], x2[4];
+        unpack8(cur.a, x1);
+        unpack8(cur.b, x2);
         const bf16 *bias = is_q ? p.q_bias : is_v ? p.v_bias : p.k_bias;
         if (bias && h < heads) {
-            float t1[8], t2[8];
+            uint64_t t1[4], t2[4];
             unpack8(ldg16(bias + (int64_t)hl * HD + c8), t1);
             unpack8(ldg16(bias + (int64_t)hl * HD + c8 + kHalf), t2);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x1[e] = __fadd_rn(x1[e], t1[e]);
-                x2[e] = __fadd_rn(x2[e], t2[e]);
+            for (int e = 0; e < 4; ++e) {
+                x1[e] = add2(x1[e], t1[e]);
+                x2[e] = add2(x2[e], t2[e]);
             }
         }
-        if (hw < hk) {  // warp-uniform: some head of this turn is q or k
-            const float r = rms_factor<HD>(x1, x2, p.eps);
+        if (cur.first < hk) {  // warp-uniform: some head of this turn is q or k
             const bf16 *w = is_q ? p.q_norm : p.k_norm;
-            if (!is_v) {
-                if (w) {
-                    float t1[8], t2[8];
+            if (p.q_norm || p.k_norm) {  // for the whole warp: the sum goes across lanes
+                const float r = rms_factor<HD>(x1, x2, p.eps);
+                if (w && !is_v) {
+                    const uint64_t rr = pair2(r, r);
+                    uint64_t t1[4], t2[4];
                     unpack8(ldg16(w + c8), t1);
                     unpack8(ldg16(w + c8 + kHalf), t2);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        x1[e] = __fmul_rn(__fmul_rn(x1[e], r), t1[e]);
-                        x2[e] = __fmul_rn(__fmul_rn(x2[e], r), t2[e]);
+                    for (int e = 0; e < 4; ++e) {
+                        x1[e] = mul2(mul2(x1[e], rr), t1[e]);
+                        x2[e] = mul2(mul2(x2[e], rr), t2[e]);
                     }
                 }
+            }
+            if (!is_v) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float y1 = x1[e], y2 = x2[e];
-                    x1[e] = __fsub_rn(__fmul_rn(y1, cs[e]), __fmul_rn(y2, sn[e]));
-                    x2[e] = __fadd_rn(__fmul_rn(y1, sn[e]), __fmul_rn(y2, cs[e]));
+                for (int e = 0; e < 4; ++e) {
+                    const uint64_t y1 = x1[e], y2 = x2[e];
+                    x1[e] = add2(mul2(y1, cs[e]), neg2(mul2(y2, sn[e])));
+                    x2[e] = add2(mul2(y1, sn[e]), mul2(y2, cs[e]));
                 }
             }
         }
         if (is_q) {
-            bf16 *dst = p.q_out + (int64_t)row * p.q_out_stride + (int64_t)h * HD + c8;
+            bf16 *dst = p.q_out + (int64_t)cur.row * p.q_out_stride + (int64_t)h * HD + c8;
             *reinterpret_cast<uint4 *>(dst) = pack8(x1);
             *reinterpret_cast<uint4 *>(dst + kHalf) = pack8(x2);
         }
-        if (hw + kHeads <= hq) continue;  // warp-uniform: only queries in this turn
+        if (cur.first + kHeads <= hq) continue;  // warp-uniform: only queries in this turn
         if constexpr (KV4) {
             const float g = is_v ? p.v_scale : p.k_scale;
-            const uint32_t s1 = kv4_scale_byte(group_amax(x1), 6.f * g);
-            const uint32_t s2 = kv4_scale_byte(group_amax(x2), 6.f * g);
+            float f1[8], f2[8];
+            floats8(x1, f1);
+            floats8(x2, f2);
+            const uint32_t s1 = kv4_scale_byte(group_amax(f1), 6.f * g);
+            const uint32_t s2 = kv4_scale_byte(group_amax(f2), 6.f * g);
             if (is_q || h >= heads || !stored) continue;
             uint8_t *page = p.kv_pool + kv4_offset(phys, p.layer, hl, p.num_layers,
                                                    p.num_kv_heads, HD) +
                             (is_v ? kv4_half_bytes(HD) : 0);
             uint32_t *codes = reinterpret_cast<uint32_t *>(page + off * (HD / 2) + c8 / 2);
-            codes[0] = kv4_codes(x1, e4m3_to_float(s1) * g);
-            codes[kHalf / 8] = kv4_codes(x2, e4m3_to_float(s2) * g);
+            codes[0] = kv4_codes(f1, e4m3_to_float(s1) * g);
+            codes[kHalf / 8] = kv4_codes(f2, e4m3_to_float(s2) * g);
             if ((lane & 1) == 0) {
                 uint8_t *sc = page + kv4_code_bytes(HD) + off * (HD / kKv4Group) + c8 / kKv4Group;
                 sc[0] = (uint8_t)s1;
@@ -217,22 +265,21 @@ __global__ void __launch_bounds__(kNormRopeThreads) norm_rope_append_kernel(Norm
     }
 }
 
-template <int HD, bool KV4, int kIter>
-int launch_iter(NormRopeParams p, cudaStream_t stream) {
-    constexpr int kPer = 32 / (HD / 16) * kIter;
-    p.groups = (p.num_q_heads + 2 * p.num_kv_heads + kPer - 1) / kPer;
-    const int64_t blocks = ((int64_t)p.rows * p.groups + kNormRopeThreads / 32 - 1) /
-                           (kNormRopeThreads / 32);
-    if (blocks > INT_MAX) return LC_ERR_INVALID_ARGUMENT;
-    norm_rope_append_kernel<HD, KV4, kIter>
-        <<<(unsigned)blocks, kNormRopeThreads, 0, stream>>>(p);
+template <int HD, bool KV4>
+int launch_dim(NormRopeParams p, cudaStream_t stream) {
+    constexpr int kHeads = 32 / (HD / 16), kWarps = kNormRopeThreads / 32;
+    p.groups = (p.num_q_heads + 2 * p.num_kv_heads + kHeads - 1) / kHeads;
+    const int64_t tasks = (int64_t)p.rows * p.groups;
+    if (tasks > INT_MAX) return LC_ERR_UNSUPPORTED_SHAPE;
+    const int64_t blocks = std::min<int64_t>((tasks + kWarps - 1) / kWarps,
+                                             (int64_t)sm_count() * kNormRopeCtas);
+    norm_rope_append_kernel<HD, KV4><<<(unsigned)blocks, kNormRopeThreads, 0, stream>>>(p);
     return launch_status();
 }
 
 template <bool KV4>
 int launch(const NormRopeParams &p, int head_dim, cudaStream_t stream) {
-    return head_dim == 64 ? launch_iter<64, KV4, 1>(p, stream)
-                          : launch_iter<128, KV4, 1>(p, stream);
+    return head_dim == 64 ? launch_dim<64, KV4>(p, stream) : launch_dim<128, KV4>(p, stream);
 }
 
 // The checks both entries share; fills everything but the pools.
