@@ -179,10 +179,21 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
+_torch_c = None
+
+
 def _stream(stream=None):
-    import torch
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return s.cuda_stream
+    """cudaStream_t of `stream` or of the current device's current stream."""
+    if stream is not None:
+        return stream.cuda_stream
+    global _torch_c
+    if _torch_c is None:
+        import torch
+        torch.cuda.init()
+        _torch_c = torch._C
+    # what torch.cuda.current_stream().cuda_stream is, without building the Stream
+    # object (0.2 us of a call against 3.2)
+    return _torch_c._cuda_getCurrentRawStream(_torch_c._cuda_getDevice())
 
 
 # ----------------------------------------------------------- reference shape --
