@@ -6,20 +6,20 @@
 // when m rises.
 //
 // Split. The T * Hq/Hkv query rows of a kv head are the columns of its products,
-// kCols = 8 or 16 at a time; (sequence, kv head, slice of columns) is a segment.
+// kCols = 8, 16 or 24 at a time; (sequence, kv head, slice of columns) is a segment.
 // The pages of all segments form one stream, cut evenly over a persistent grid:
 // every CTA moves the same bytes whatever the lengths are. A segment cut across
 // CTAs leaves (O, m, l) pieces in the workspace; the CTA that finishes it last
 // (arrival counter) joins them in the order of the stream, so the result does
 // not depend on timing.
 //
-// Inside a CTA eight warps compute, taking groups of kGroup pages in turn, each
+// Inside a CTA eight (ten, six) warps compute, taking groups of kGroup pages in turn, each
 // from a ring of its own. A loading warp fills the rings, one lane per page of a
 // group: one bulk copy brings K and V of the kv head (18 hd bytes, contiguous),
 // and full and empty mbarriers per stage join a computing warp to its lanes. An
 // edge warp works a chunk (a CTA's part of one segment) ahead and behind: it
 // prepares the next chunk's q as mma operands in shared memory, and joins the
-// eight states (O, m, l) that the computing warps leave at a chunk's end, so the
+// states (O, m, l) that the computing warps leave at a chunk's end, so the
 // latency of that end (shared memory, the stores, the arrival counter, the other
 // pieces) runs beside the next chunk. The computing warps touch no global memory
 // until the CTA's last chunk, whose columns they join themselves, one per warp.
@@ -51,12 +51,8 @@
 namespace lc {
 namespace {
 
-constexpr int kWarps = 8;             // computing
-constexpr int kLoadWarp = kWarps;     // one that loads
-constexpr int kEdgeWarp = kWarps + 1;  // one for the chunks' ends
-constexpr int kThreads = (kWarps + 2) * 32;
 constexpr int kGroup = 2;             // pages of one warp at a time
-constexpr int kMinPages = kWarps * kGroup;  // pages per CTA at least
+constexpr int kMinPages = 16;         // pages per CTA at least
 constexpr int kEdgeUnits = 24;
 constexpr float kLazy = 8.f;  // p may reach 2^8 before O and l are rescaled
 
@@ -89,15 +85,23 @@ struct DecodeKv4Params {
 template <int HD, int NT>
 struct Cfg {
     static constexpr int kCols = 8 * NT;
+    // Computing warps per CTA and CTAs per SM, by the registers that O takes: 8 NT for
+    // each 32 dims. One warp that loads and one for the chunks' ends beside them.
+    static constexpr int kWarps = NT == 1 ? 8 : NT == 2 ? 10 : 6;
+    static constexpr int kCtasPerSm = NT == 1 ? 2 : 1;
+    static constexpr int kLoadWarp = kWarps, kEdgeWarp = kWarps + 1;
+    static constexpr int kThreads = (kWarps + 2) * 32;
     static constexpr int kPage = 18 * HD;  // K and V of one kv head
     static constexpr int kStage = kGroup * kPage;
-    static constexpr int kStages = HD == 64 ? 4 : 2;
     static constexpr int kRow = HD + 4;  // floats between columns of a warp's state
-    static constexpr int kRing = kWarps * kStages * kStage;
     static constexpr int kStates = kWarps * kCols * kRow * 4;
     static constexpr int kQ = kCols * HD * 2;  // a chunk's q, fp16 operands
+    // Stages per warp: two groups of the 128-dim pages, more where there is room.
+    static constexpr int kStages = NT == 1 ? (HD == 64 ? 4 : 2)
+                                           : (224 * 1024 - kStates - 2 * kQ) / (kWarps * kStage);
+    static_assert(kStages >= 2 && kGroup * kWarps <= 32);
+    static constexpr int kRing = kWarps * kStages * kStage;
     static constexpr int kSmem = kRing + kStates + 2 * kQ;
-    static constexpr int kCtasPerSm = NT == 1 ? 2 : 1;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -255,6 +259,7 @@ __device__ __forceinline__ void join_states(const float2 (*ml_of)[Cfg<HD, NT>::k
                                             const float *states, int c, int lane,
                                             Joined<HD, NT> &j) {
     using C = Cfg<HD, NT>;
+    constexpr int kWarps = C::kWarps;
     float2 ml[kWarps];
     j.m = -INFINITY, j.l = 0.f;
 #pragma unroll
@@ -366,10 +371,11 @@ __device__ __forceinline__ int pieces_of(const DecodeKv4Params &p, const Cut &cu
 }
 
 template <int HD, int NT>
-__global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
+__global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm)
     decode_kv4_kernel(const DecodeKv4Params p) {
     using C = Cfg<HD, NT>;
-    constexpr int kCols = C::kCols;
+    constexpr int kCols = C::kCols, kWarps = C::kWarps;
+    constexpr int kLoadWarp = C::kLoadWarp, kEdgeWarp = C::kEdgeWarp;
     constexpr int kSteps = HD / 16;   // k-steps of S, m-tiles of O
     constexpr int kWords = HD / 32;   // code words per token and lane (K)
     extern __shared__ __align__(128) uint8_t smem[];
@@ -446,7 +452,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
         // ---- loads: lane 2 w + k brings page k of each of warp w's groups, which are
         // group w, w + kWarps, ... of every chunk
         if (first >= end) return;
-        static_assert(kGroup * kWarps <= 32);
         const int w = lane / kGroup, k = lane % kGroup;
         const int64_t page_stride = kv4_offset(1, 0, 0, p.num_layers, p.num_kv_heads, HD);
         const uint32_t dst0 = smem_u32(smem) + w * C::kStages * C::kStage + k * C::kPage;
@@ -919,9 +924,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
         const int64_t seg = (int64_t)ch.b * p.seg_per_seq + ch.seg;
         int c0 = 0, pieces = 0;
         if (!whole) pieces = pieces_of(p, cut, ch, c0);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int c = nt * 8 + warp;
+#pragma unroll 1
+        for (int c = warp; c < kCols; c += kWarps) {
             Joined<HD, NT> j;
             join_states<HD, NT>(s_ml, states, c, lane, j);
             if (!whole) {
@@ -940,9 +944,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NT>::kCtasPerSm)
         pieces = pieces_of(p, cut, lc, c0);
         __syncwarp();
         __threadfence();  // the edge warp's count saw the pieces; now this warp's reads do
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int c = nt * 8 + warp;
+#pragma unroll 1
+        for (int c = warp; c < kCols; c += kWarps) {
             if (!(left >> c & 1)) continue;
             Joined<HD, NT> j;
             join_pieces<HD, NT>(p, (int64_t)lc.b * p.seg_per_seq + lc.seg + c0, pieces, c, lane, j);
@@ -961,11 +964,18 @@ struct WsLayout {
     size_t total() const { return cnt + ml + o; }
 };
 
-int tiles(int cols) { return cols <= 8 ? 1 : 2; }
+// Tiles of 8 columns that a segment takes at once: K and V unpack once for all of
+// them, so as few slices as three tiles allow, and then no more tiles than needed.
+// (24 columns, 8 sequences of 1024 .. 32768 tokens of 64/8 heads of 128: 86 us with
+// three tiles, 104 us as two slices of two.)
+int tiles(int64_t cols) {
+    if (cols <= 8) return 1;
+    return (cols + 23) / 24 < (cols + 15) / 16 ? 3 : 2;
+}
 
 WsLayout ws_layout(int64_t batch, int hq, int hkv, int hd, int tokens) {
     const int64_t cols = (int64_t)(hq / hkv) * tokens;
-    const int nc = 8 * tiles((int)(cols < 64 ? cols : 64));
+    const int nc = 8 * tiles(cols);
     const int64_t segs = batch * hkv * ((cols + nc - 1) / nc);
     const int64_t pieces = segs + (int64_t)sm_count() * (nc == 8 ? 2 : 1);
     return {align256(segs * nc * 4), align256(pieces * nc * 8), (size_t)pieces * nc * hd * 4};
@@ -989,7 +999,7 @@ int launch(DecodeKv4Params p, int max_context_len, cudaStream_t stream) {
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)std::max<int64_t>(grid, 1));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(C::kThreads);
     cfg.dynamicSmemBytes = C::kSmem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -1074,9 +1084,12 @@ extern "C" int lc_paged_decode_kv4(void *out, int64_t out_stride, const void *q,
     p.ws_o = (float *)(ws + wl.cnt + wl.ml);
     p.status = dev_status;
     cudaStream_t s = as_stream(stream);
-    if (tiles(p.cols) == 1)
-        return head_dim == 64 ? launch<64, 1>(p, max_context_len, s)
-                              : launch<128, 1>(p, max_context_len, s);
-    return head_dim == 64 ? launch<64, 2>(p, max_context_len, s)
-                          : launch<128, 2>(p, max_context_len, s);
+    switch (tiles(p.cols) * 1000 + head_dim) {
+        case 1064: return launch<64, 1>(p, max_context_len, s);
+        case 1128: return launch<128, 1>(p, max_context_len, s);
+        case 2064: return launch<64, 2>(p, max_context_len, s);
+        case 2128: return launch<128, 2>(p, max_context_len, s);
+        case 3064: return launch<64, 3>(p, max_context_len, s);
+        default: return launch<128, 3>(p, max_context_len, s);
+    }
 }
