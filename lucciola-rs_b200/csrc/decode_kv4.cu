@@ -195,10 +195,14 @@ struct Cut {
         // joins two segments in turn.
         if (p.batch == 1 && ctas < max_ctas && ctas > p.seg_per_seq) ctas -= ctas % p.seg_per_seq;
     }
+    // In 32 bits where the products fit: a 64-bit division costs a good part of a
+    // microsecond before the first load.
     __device__ __forceinline__ int start(int cta) const {
+        if (total < (1 << 22)) return (int)((unsigned)total * (unsigned)cta / (unsigned)ctas);
         return (int)((long long)total * cta / ctas);
     }
     __device__ __forceinline__ int owner(int unit) const {
+        if (total < (1 << 22)) return (int)((((unsigned)unit + 1u) * (unsigned)ctas - 1u) / (unsigned)total);
         return (int)((((long long)unit + 1) * ctas - 1) / total);
     }
 };
@@ -345,21 +349,32 @@ __device__ __forceinline__ void join_pieces(const DecodeKv4Params &p, int64_t pl
     j.l = 0.f;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) j.o[i] = 0.f;
-#pragma unroll 4
-    for (int k = 0; k < pieces; ++k) {
-        const float2 ml = __ldcg(&bml[k * kCols]);
-        float x[kPer];
-        if constexpr (kPer == 4) {
-            const float4 v = __ldcg(reinterpret_cast<const float4 *>(bo + (int64_t)k * kCols * HD));
-            x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-        } else {
-            const float2 v = __ldcg(reinterpret_cast<const float2 *>(bo + (int64_t)k * kCols * HD));
-            x[0] = v.x, x[1] = v.y;
-        }
-        const float r = ml.x == -INFINITY ? 0.f : ex2(ml.x - j.m);
-        j.l = fmaf(ml.y, r, j.l);
+    constexpr int kBatch = 8;  // pieces read at once
+    for (int k0 = 0; k0 < pieces; k0 += kBatch) {
+        float2 ml[kBatch];
+        float x[kBatch][kPer];
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) j.o[i] = fmaf(x[i], r, j.o[i]);
+        for (int i = 0; i < kBatch; ++i) {
+            ml[i] = make_float2(-INFINITY, 0.f);
+            if (k0 + i >= pieces) continue;
+            const float *src = bo + (int64_t)(k0 + i) * kCols * HD;
+            ml[i] = __ldcg(&bml[(k0 + i) * kCols]);
+            if constexpr (kPer == 4) {
+                const float4 v = __ldcg(reinterpret_cast<const float4 *>(src));
+                x[i][0] = v.x, x[i][1] = v.y, x[i][2] = v.z, x[i][3] = v.w;
+            } else {
+                const float2 v = __ldcg(reinterpret_cast<const float2 *>(src));
+                x[i][0] = v.x, x[i][1] = v.y;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            if (ml[i].x == -INFINITY) continue;
+            const float r = ex2(ml[i].x - j.m);
+            j.l = fmaf(ml[i].y, r, j.l);
+#pragma unroll
+            for (int d = 0; d < kPer; ++d) j.o[d] = fmaf(x[i][d], r, j.o[d]);
+        }
     }
 }
 
@@ -412,6 +427,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
         s_left_cols = 0;
     }
     fence_barrier_init();
+    __syncthreads();
 
     // ---- the two side warps: the stream's length, this CTA's range of it and the
     // sequence that it starts in
@@ -445,7 +461,6 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
             }
         }
     }
-    __syncthreads();
     if (p.pdl_mode == 2) griddep_wait();
 
     if (warp == kLoadWarp) {
@@ -589,11 +604,13 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
                     top = max(top, max(r[k] & 0x7fffu, (r[k] >> 16) & 0x7fffu));
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const int e = top ? (int)(top >> 7) - 127 : 0;
-                const float down = ldexpf(1.f, -e);
+                // 2^-e and 2^e, kept within the normal numbers
+                const int e = min(max((int)(top >> 7) - 127, -126), 126);
+                const float down = __int_as_float((127 - e) << 23);
                 // never zero, so that a masked score stays -inf
                 if (t == 0)
-                    s_f[buf][nt * 8 + g] = fmaxf(p.scale_log2 * ldexpf(1.f, e), FLT_MIN);
+                    s_f[buf][nt * 8 + g] =
+                        fmaxf(p.scale_log2 * __int_as_float((127 + e) << 23), FLT_MIN);
                 uint2 *dst = reinterpret_cast<uint2 *>(q_ops + buf * C::kQ) + nt * kSteps * 32 + lane;
 #pragma unroll
                 for (int k = 0; k < HD / 16; ++k) {
