@@ -43,6 +43,7 @@ struct NormRopeParams {
     const bf16 *q_bias, *k_bias, *v_bias;
     const bf16 *q_norm, *k_norm;
     float eps;
+    float one;  // 1: see kv4.cuh
     const float *cos_t, *sin_t;
     int rope_rows;
     bf16 *k_pool, *v_pool;  // bf16 pools
@@ -53,29 +54,6 @@ struct NormRopeParams {
     int groups;  // warp tasks per row
     int *status;
 };
-
-// Pairs of fp32 values, each rounded as a single operation would.
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t pair2(float lo, float hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ float2 split2(uint64_t a) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
-    return r;
-}
-__device__ __forceinline__ uint64_t neg2(uint64_t a) { return a ^ 0x8000000080000000ull; }
 
 // Eight bf16 values as four pairs, and back with one rounding.
 __device__ __forceinline__ void unpack8(const uint4 &u, uint64_t (&f)[4]) {
@@ -93,14 +71,6 @@ __device__ __forceinline__ uint4 pack8(const uint64_t (&f)[4]) {
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
-__device__ __forceinline__ void floats8(const uint64_t (&f)[4], float (&x)[8]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 v = split2(f[i]);
-        x[2 * i] = v.x, x[2 * i + 1] = v.y;
-    }
-}
-
 __device__ __forceinline__ uint4 ldg16(const bf16 *p) {
     return __ldg(reinterpret_cast<const uint4 *>(p));
 }
@@ -114,10 +84,11 @@ __device__ __forceinline__ void load8f(const float *p, uint64_t (&f)[4]) {
 // 1 / sqrt(mean of squares + eps) of a head, x1 and x2 its two 8-dim pieces in
 // this lane. All lanes of the warp call it.
 template <int HD>
-__device__ __forceinline__ float rms_factor(const uint64_t (&x1)[4], const uint64_t (&x2)[4], float eps) {
+__device__ __forceinline__ float rms_factor(const uint64_t (&x1)[4], const uint64_t (&x2)[4], float eps,
+                                            uint64_t one) {
     uint64_t s[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[e] = add2(mul2(x1[e], x1[e]), mul2(x2[e], x2[e]));
+    for (int e = 0; e < 4; ++e) s[e] = fma2(mul2(x1[e], x1[e]), one, mul2(x2[e], x2[e]));
     // dims e and e + 4, then e and e + 2, then the last two
     const float2 r = split2(add2(add2(s[0], s[2]), add2(s[1], s[3])));
     float t = __fadd_rn(r.x, r.y);
@@ -128,10 +99,13 @@ __device__ __forceinline__ float rms_factor(const uint64_t (&x1)[4], const uint6
 
 // Largest magnitude of a 16-dim group (this lane's 8 dims and its neighbour's),
 // as float bits: a NaN is larger than every number.
-__device__ __forceinline__ uint32_t group_amax(const float (&x)[8]) {
+__device__ __forceinline__ uint32_t group_amax(const uint64_t (&x)[4]) {
     uint32_t m = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(x[e]) & 0x7fffffffu);
+    for (int e = 0; e < 4; ++e) {
+        const float2 v = split2(x[e]);
+        m = max(m, max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu));
+    }
     return max(m, __shfl_xor_sync(0xffffffffu, m, 1));
 }
 
@@ -143,6 +117,7 @@ __global__ void __launch_bounds__(kNormRopeThreads, kNormRopeCtas) norm_rope_app
     const int lane = threadIdx.x & 31;
     const int hq = p.num_q_heads, hk = hq + p.num_kv_heads, heads = hk + p.num_kv_heads;
     const int c8 = (lane % kLanes) * 8;
+    const uint64_t one = pair2(p.one, p.one), minus_one = pair2(-p.one, -p.one);
     const uint32_t tasks = (uint32_t)p.rows * p.groups;  // kHeads heads of one row each
     const uint32_t step = gridDim.x * (kNormRopeThreads / 32);
 
@@ -208,7 +183,7 @@ __global__ void __launch_bounds__(kNormRopeThreads, kNormRopeCtas) norm_rope_app
         if (cur.first < hk) {  // warp-uniform: some head of this turn is q or k
             const bf16 *w = is_q ? p.q_norm : p.k_norm;
             if (p.q_norm || p.k_norm) {  // for the whole warp: the sum goes across lanes
-                const float r = rms_factor<HD>(x1, x2, p.eps);
+                const float r = rms_factor<HD>(x1, x2, p.eps, one);
                 if (w && !is_v) {
                     const uint64_t rr = pair2(r, r);
                     uint64_t t1[4], t2[4];
@@ -225,8 +200,8 @@ __global__ void __launch_bounds__(kNormRopeThreads, kNormRopeCtas) norm_rope_app
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const uint64_t y1 = x1[e], y2 = x2[e];
-                    x1[e] = add2(mul2(y1, cs[e]), neg2(mul2(y2, sn[e])));
-                    x2[e] = add2(mul2(y1, sn[e]), mul2(y2, cs[e]));
+                    x1[e] = fma2(mul2(y2, sn[e]), minus_one, mul2(y1, cs[e]));
+                    x2[e] = fma2(mul2(y1, sn[e]), one, mul2(y2, cs[e]));
                 }
             }
         }
@@ -238,18 +213,15 @@ __global__ void __launch_bounds__(kNormRopeThreads, kNormRopeCtas) norm_rope_app
         if (cur.first + kHeads <= hq) continue;  // warp-uniform: only queries in this turn
         if constexpr (KV4) {
             const float g = is_v ? p.v_scale : p.k_scale;
-            float f1[8], f2[8];
-            floats8(x1, f1);
-            floats8(x2, f2);
-            const uint32_t s1 = kv4_scale_byte(group_amax(f1), 6.f * g);
-            const uint32_t s2 = kv4_scale_byte(group_amax(f2), 6.f * g);
+            const uint32_t m1 = group_amax(x1), m2 = group_amax(x2);
+            const uint32_t s1 = kv4_scale_byte(m1, 6.f * g), s2 = kv4_scale_byte(m2, 6.f * g);
             if (is_q || h >= heads || !stored) continue;
             uint8_t *page = p.kv_pool + kv4_offset(phys, p.layer, hl, p.num_layers,
                                                    p.num_kv_heads, HD) +
                             (is_v ? kv4_half_bytes(HD) : 0);
             uint32_t *codes = reinterpret_cast<uint32_t *>(page + off * (HD / 2) + c8 / 2);
-            codes[0] = kv4_codes(f1, e4m3_to_float(s1) * g);
-            codes[kHalf / 8] = kv4_codes(f2, e4m3_to_float(s2) * g);
+            codes[0] = kv4_codes(x1, e4m3_to_float(s1) * g, m1);
+            codes[kHalf / 8] = kv4_codes(x2, e4m3_to_float(s2) * g, m2);
             if ((lane & 1) == 0) {
                 uint8_t *sc = page + kv4_code_bytes(HD) + off * (HD / kKv4Group) + c8 / kKv4Group;
                 sc[0] = (uint8_t)s1;
@@ -318,6 +290,7 @@ int fill(NormRopeParams &p, void *q_out, int64_t q_out_stride, const void *qkv,
     p.q_norm = (const bf16 *)q_norm;
     p.k_norm = (const bf16 *)k_norm;
     p.eps = eps;
+    p.one = 1.f;
     p.cos_t = cos_cache;
     p.sin_t = sin_cache;
     p.rope_rows = rope_rows;
