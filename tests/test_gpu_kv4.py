@@ -402,3 +402,54 @@ def test_decode_on_another_stream_and_in_a_graph():
         graph.replay()
     torch.cuda.synchronize()
     assert np.array_equal(R.bf16_f64(from_device(out)).reshape(3, hq, hd), got)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("hq,hkv,tokens", [(14, 2, 1), (16, 2, 2), (8, 1, 3), (16, 2, 5), (3, 3, 11)])
+def test_decode_long_contexts_over_many_ctas(hq, hkv, tokens, hd):
+    """Segments split over CTAs, for 8, 16 and 24 columns at a time and several slices."""
+    check_decode(hq, hkv, hd, [2500, 0, 700, 33, 1601], tokens=tokens, seed=hq + tokens)
+    check_decode(hq, hkv, hd, [3333], tokens=tokens, seed=hq + tokens, hint=3333)
+
+
+def test_decode_many_short_sequences():
+    """CTAs with many segments each."""
+    rng = np.random.default_rng(21)
+    check_decode(4, 2, 64, rng.integers(0, 40, 600), seed=22)
+    check_decode(8, 1, 128, rng.integers(1, 20, 900), seed=23, hint=19)
+
+
+@pytest.mark.parametrize("mode", [1, 2])
+def test_decode_with_dependent_launch(mode):
+    """An append and the decode over it, back to back: the same bits in every launch mode."""
+    hq, hkv, hd, b = 14, 2, 64, 6
+    rng = np.random.default_rng(24)
+    lens = rng.integers(200, 900, b).astype(np.int32)
+    tables, nb = make_tables(np.array([R.ceil16(n) for n in lens]), rng)
+    base = to_device(R.make_pool(rng, nb, 1, hkv, hd, 1.0, 1.0))
+    cos, sin = (to_device(t) for t in O.rope_table(1024, hd, 1e6))
+    qkv = to_device(randn_bf16(rng, (b, (hq + 2 * hkv) * hd)))
+    pos = lens - 1
+    slot = to_device((tables[np.arange(b), pos // 16] * 16 + pos % 16).astype(np.int32))
+    pos, lens_d, tables_d = to_device(pos), to_device(lens), to_device(tables)
+    ws = L.alloc_decode_kv4_workspace(b, hq, hkv, hd)
+
+    def run():
+        pool = base.clone()
+        q = torch.zeros(b, hq * hd, dtype=torch.bfloat16, device="cuda")
+        outs = []
+        for _ in range(4):
+            L.qk_norm_rope_append_kv4(q, qkv, pos, slot, cos, sin, pool, nb, 1, 0, hq, hkv, hd)
+            outs.append(torch.zeros_like(q))
+            L.paged_decode_kv4(outs[-1], q, pool, nb, 1, 0, hq, hkv, hd, tables_d, lens_d, 900,
+                               workspace=ws)
+        torch.cuda.synchronize()
+        return outs
+    want = run()
+    old = L.set_dependent_launch(mode)
+    try:
+        got = run()
+    finally:
+        L.set_dependent_launch(old)
+    for x in got + want:
+        assert torch.equal(x, want[0])

@@ -138,3 +138,55 @@ def test_agrees_with_rope_append():
         # the rotation's terms are below 16; one bf16 step where the last fp32 bit decides
         assert ((x - y).abs() <= torch.maximum(x.abs() * 2.0 ** -7, torch.tensor(16 * 2.0 ** -23))).all()
         assert (x != y).float().mean() < 1e-3
+
+
+def separately_rounded(x, bias, w, eps, cos, sin):
+    """float32 in, float32 out: every product and sum rounded by itself, the squares added
+    in halves (d with d + hd/2, within 8 dims, across the 8-dim chunks)."""
+    f = np.float32
+    u = x if bias is None else x + bias
+    hd = u.shape[-1]
+    if w is not None:
+        q = (u * u).reshape(u.shape[:-1] + (2, hd // 16, 8))
+        q = q[..., 0, :, :] + q[..., 1, :, :]
+        while q.shape[-1] > 1:
+            n = q.shape[-1] // 2
+            q = q[..., :n] + q[..., n:]
+        q = q[..., 0]
+        while q.shape[-1] > 1:
+            n = q.shape[-1] // 2
+            q = q[..., :n] + q[..., n:]
+        u = u * (f(1) / np.sqrt(q * f(1 / hd) + f(eps))) * w
+    a, b = np.split(u, 2, -1)
+    c, s = cos[:, None, :], sin[:, None, :]
+    return np.concatenate([a * c - b * s, a * s + b * c], -1)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("norm,bias", [(True, False), (True, True), (False, True), (False, False)])
+def test_bits_do_not_depend_on_the_kernel(hd, norm, bias):
+    """Compilers like to contract a * b + c * d: a last bit here can be a whole step once a
+    value is held in 4 bits, so the bits are pinned."""
+    hq, hkv, rows = 6, 2, 70
+    rng = np.random.default_rng(hd)
+    qkv = randn_bf16(rng, (rows, (hq + 2 * hkv) * hd))
+    vec = {k: randn_bf16(rng, n * hd) if on else None for k, n, on in (
+        ("q_bias", hq, bias), ("k_bias", hkv, bias), ("v_bias", hkv, bias),
+        ("q_norm", 1, norm), ("k_norm", 1, norm))}
+    cos, sin = O.rope_table(rows, hd, 1e6)
+    pool = [torch.zeros(5, 1, hkv, 16, hd, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    q = torch.zeros(rows, hq * hd, dtype=torch.bfloat16, device="cuda")
+    ids = torch.arange(rows, dtype=torch.int32, device="cuda")
+    L.qk_norm_rope_append(q, to_device(qkv), ids, ids, to_device(cos), to_device(sin), *pool, 5, 1,
+                          0, hq, hkv, hd, **{k: None if v is None else to_device(v)
+                                             for k, v in vec.items()})
+    f = {k: None if v is None else R.bf16_f64(v).astype(np.float32).reshape(-1, hd)
+         for k, v in vec.items()}
+    x = R.bf16_f64(qkv).astype(np.float32).reshape(rows, -1, hd)
+    for got, lo, n, part in ((from_device(q).reshape(rows, hq, hd), 0, hq, "q"),
+                             (from_device(pool[0])[:, 0].transpose(0, 2, 1, 3)
+                              .reshape(80, hkv, hd)[:rows], hq, hkv, "k")):
+        w = f[part + "_norm"]
+        want = separately_rounded(x[:, lo:lo + n], f[part + "_bias"], None if w is None else w[0],
+                                  1e-6, cos, sin)
+        assert np.array_equal(got, O.f32_to_bf16(want))
