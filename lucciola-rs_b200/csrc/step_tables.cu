@@ -28,7 +28,8 @@ constexpr int kStepThreads = 512;
 constexpr int kStepWarps = kStepThreads / 32;
 constexpr int kStepMaxBatch = 8192;  // four ints of shared memory per request
 constexpr int kTokenSegment = 128;   // token rows of a warp's task
-constexpr int kRowSegment = 128;     // table entries of a warp's task: 16 bytes per lane
+constexpr int kRowTurns = 2;
+constexpr int kRowSegment = 128 * kRowTurns;  // table entries of a warp's task: 16 bytes per lane and turn
 
 struct StepParams {
     int *tables;
@@ -242,20 +243,29 @@ __global__ void __launch_bounds__(kStepThreads) step_tables_kernel(StepParams p)
         auto entry = [&](int j) {
             return j < min(have, p.table_stride) ? row[j] : j < want ? __ldg(top - j) : -1;
         };
-        const int j = j0 + 4 * lane;
-        if (j >= s1) continue;
-        int4 v;
-        if (p.table_vec && j + 4 <= have)
-            v = *reinterpret_cast<const int4 *>(row + j);
-        else
-            v = make_int4(entry(j), entry(j + 1), entry(j + 2), entry(j + 3));
-        if (p.step_vec && j + 4 <= s1) {
-            *reinterpret_cast<int4 *>(out + j) = v;
-        } else {
-            out[j] = v.x;
-            if (j + 1 < s1) out[j + 1] = v.y;
-            if (j + 2 < s1) out[j + 2] = v.z;
-            if (j + 3 < s1) out[j + 3] = v.w;
+        int4 v[kRowTurns];
+#pragma unroll
+        for (int i = 0; i < kRowTurns; ++i) {
+            const int j = j0 + 128 * i + 4 * lane;
+            if (p.table_vec && j + 4 <= have)
+                v[i] = *reinterpret_cast<const int4 *>(row + j);
+            else if (j < want)
+                v[i] = make_int4(entry(j), entry(j + 1), entry(j + 2), entry(j + 3));
+            else
+                v[i] = make_int4(-1, -1, -1, -1);
+        }
+#pragma unroll
+        for (int i = 0; i < kRowTurns; ++i) {
+            const int j = j0 + 128 * i + 4 * lane;
+            if (j >= s1) break;
+            if (p.step_vec && j + 4 <= s1) {
+                *reinterpret_cast<int4 *>(out + j) = v[i];
+            } else {
+                out[j] = v[i].x;
+                if (j + 1 < s1) out[j + 1] = v[i].y;
+                if (j + 2 < s1) out[j + 2] = v[i].z;
+                if (j + 3 < s1) out[j + 3] = v[i].w;
+            }
         }
     }
 
