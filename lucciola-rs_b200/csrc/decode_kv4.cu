@@ -13,13 +13,13 @@
 // (arrival counter) joins them in the order of the stream, so the result does
 // not depend on timing.
 //
-// Inside a CTA eight (ten, six) warps compute, taking groups of kGroup pages in turn, each
+// Inside a CTA eight warps compute, taking groups of kGroup pages in turn, each
 // from a ring of its own. A loading warp fills the rings, one lane per page of a
 // group: one bulk copy brings K and V of the kv head (18 hd bytes, contiguous),
-// and full and empty mbarriers per stage join a computing warp to its lanes. An
-// edge warp works a chunk (a CTA's part of one segment) ahead and behind: it
-// prepares the next chunk's q as mma operands in shared memory, and joins the
-// states (O, m, l) that the computing warps leave at a chunk's end, so the
+// and full and empty mbarriers per stage join a computing warp to its lanes. Edge
+// warps, one for each 8 columns, work a chunk (a CTA's part of one segment) ahead
+// and behind: they prepare the next chunk's q as mma operands in shared memory, and
+// join the states (O, m, l) that the computing warps leave at a chunk's end, so the
 // latency of that end (shared memory, the stores, the arrival counter, the other
 // pieces) runs beside the next chunk. The computing warps touch no global memory
 // until the CTA's last chunk, whose columns they join themselves, one per warp.
@@ -85,12 +85,20 @@ struct DecodeKv4Params {
 template <int HD, int NT>
 struct Cfg {
     static constexpr int kCols = 8 * NT;
-    // Computing warps per CTA and CTAs per SM, by the registers that O takes: 8 NT for
-    // each 32 dims. One warp that loads and one for the chunks' ends beside them.
-    static constexpr int kWarps = NT == 1 ? 8 : NT == 2 ? 10 : 6;
+    // Two warps per scheduler, or four (two CTAs) where O takes few registers: 8 NT for
+    // each 32 dims. Ten of 168 registers do not help two tiles (8 sequences of 1024 ..
+    // 32768 tokens, 64/8 heads of 128: 61 us, 59 us with eight): two schedulers have three
+    // then. Beside them one warp that loads and one per tile for the chunks' ends.
+    static constexpr int kWarps = 8;
     static constexpr int kCtasPerSm = NT == 1 ? 2 : 1;
+    static constexpr int kEdges = NT;
     static constexpr int kLoadWarp = kWarps, kEdgeWarp = kWarps + 1;
-    static constexpr int kThreads = (kWarps + 2) * 32;
+    static constexpr int kThreads = (kWarps + 1 + kEdges) * 32;
+    // Three tiles of 128 dims take 210 registers: the four side warps hand theirs over.
+    // (The case above with 24 columns: 69 us, 86 us with six warps of 238.) 0: as launched.
+    static constexpr int kRegs = NT == 3 && HD == 128 ? 216 : 0, kSideRegs = kRegs ? 72 : 24;
+    static_assert(kRegs == 0 || (kEdges == 3 && kWarps * kRegs + 4 * kSideRegs <=
+                                                    12 * (65536 / kThreads / 8 * 8)));
     static constexpr int kPage = 18 * HD;  // K and V of one kv head
     static constexpr int kStage = kGroup * kPage;
     static constexpr int kRow = HD + 4;  // floats between columns of a warp's state
@@ -390,7 +398,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
     decode_kv4_kernel(const DecodeKv4Params p) {
     using C = Cfg<HD, NT>;
     constexpr int kCols = C::kCols, kWarps = C::kWarps;
-    constexpr int kLoadWarp = C::kLoadWarp, kEdgeWarp = C::kEdgeWarp;
+    constexpr int kLoadWarp = C::kLoadWarp, kEdgeWarp = C::kEdgeWarp, kEdges = C::kEdges;
     constexpr int kSteps = HD / 16;   // k-steps of S, m-tiles of O
     constexpr int kWords = HD / 32;   // code words per token and lane (K)
     extern __shared__ __align__(128) uint8_t smem[];
@@ -418,21 +426,23 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
         mbar_init(&empty[warp][lane], 1);
     }
     if (tid == 0) {
-        mbar_init(&q_full[0], 1);
-        mbar_init(&q_full[1], 1);
+        mbar_init(&q_full[0], C::kEdges);
+        mbar_init(&q_full[1], C::kEdges);
         mbar_init(&states_full, kWarps);
-        mbar_init(&states_empty, 1);
-        mbar_init(&edge_done, 1);
+        mbar_init(&states_empty, C::kEdges);
+        mbar_init(&edge_done, C::kEdges);
         s_abort = 0;
         s_left_cols = 0;
     }
     fence_barrier_init();
     __syncthreads();
 
-    // ---- the two side warps: the stream's length, this CTA's range of it and the
+    // ---- the side warps: the stream's length, this CTA's range of it and the
     // sequence that it starts in
-    int total = 0, first = 0, end = 0, b0 = 0, before = 0;
     if (warp >= kWarps) {
+        if constexpr (C::kRegs != 0)
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kSideRegs));
+        int first = 0, end = 0, b0 = 0, before = 0;
         const int per = (p.batch + 31) / 32;
         const int q0 = min(p.batch, lane * per), q1 = min(p.batch, q0 + per);
         int mine = 0;
@@ -445,7 +455,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
             const int u = __shfl_up_sync(0xffffffffu, upto, d);
             if (lane >= d) upto += u;
         }
-        total = __shfl_sync(0xffffffffu, upto, 31);
+        const int total = __shfl_sync(0xffffffffu, upto, 31);
         const Cut cut(p, total, gridDim.x);
         if (cta < cut.ctas) {
             first = cut.start(cta);
@@ -460,102 +470,101 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
                 before += k;
             }
         }
-    }
-    if (p.pdl_mode == 2) griddep_wait();
+        if (p.pdl_mode == 2) griddep_wait();
 
-    if (warp == kLoadWarp) {
-        // ---- loads: lane 2 w + k brings page k of each of warp w's groups, which are
-        // group w, w + kWarps, ... of every chunk
-        if (first >= end) return;
-        const int w = lane / kGroup, k = lane % kGroup;
-        const int64_t page_stride = kv4_offset(1, 0, 0, p.num_layers, p.num_kv_heads, HD);
-        const uint32_t dst0 = smem_u32(smem) + w * C::kStages * C::kStage + k * C::kPage;
-        Walk lw;
-        lw.start(p, first, b0, before);
-        bool more = lane < kGroup * kWarps && lw.next(p, end);
-        int base = w * kGroup;  // first page of the next group, within its chunk
-        int phys = -1;          // this lane's table entry in it, -1: no page
-        const uint8_t *head = nullptr;
-        auto advance = [&]() {
-            while (more && base >= lw.take) {
-                more = lw.next(p, end);
-                base = w * kGroup;
-            }
-            phys = -1;
-            if (more && base + k < lw.take) {
-                phys = __ldg(p.tables + (int64_t)lw.b * p.table_stride + lw.p0 + base + k);
-                if (phys < 0) phys = INT_MAX;  // a bad entry, reported when it is loaded
-            }
-            head = p.kv_pool + kv4_offset(0, p.layer, lw.seg / p.slices, p.num_layers,
-                                          p.num_kv_heads, HD);
-        };
-        advance();
-        int stage = 0, issued = 0;
-        uint32_t phase = 1;  // the first round finds every stage free
-        uint64_t since = 0;
-        for (uint32_t it = 0; __any_sync(0xffffffffu, more); ++it) {
-            const bool ready = more && test_wait(&empty[w][stage], phase);
-            if (ready) {
-                uint64_t *bar = &full[w][stage];
-                const uint32_t dst = dst0 + stage * C::kStage;
-                if ((uint32_t)phys < p.num_blocks) {
-                    mbar_arrive_expect_tx(bar, C::kPage);
-                    bulk_load(dst, head + phys * page_stride, C::kPage, bar);
-                } else {
-                    if (phys != -1) {  // a table entry outside the pool reads as zeros
-                        set_status(p.status, LC_DEV_BAD_BLOCK);
-                        for (int i = 0; i < C::kPage / 16; ++i)
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst + 16 * i),
-                                         "r"(0) : "memory");
-                        // before the copies that fill the stage later
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        if (warp == kLoadWarp) {
+            // ---- loads: lane 2 w + k brings page k of each of warp w's groups, which are
+            // group w, w + kWarps, ... of every chunk
+            if (first >= end) return;
+            const int w = lane / kGroup, k = lane % kGroup;
+            const int64_t page_stride = kv4_offset(1, 0, 0, p.num_layers, p.num_kv_heads, HD);
+            const uint32_t dst0 = smem_u32(smem) + w * C::kStages * C::kStage + k * C::kPage;
+            Walk lw;
+            lw.start(p, first, b0, before);
+            bool more = lane < kGroup * kWarps && lw.next(p, end);
+            int base = w * kGroup;  // first page of the next group, within its chunk
+            int phys = -1;          // this lane's table entry in it, -1: no page
+            const uint8_t *head = nullptr;
+            auto advance = [&]() {
+                while (more && base >= lw.take) {
+                    more = lw.next(p, end);
+                    base = w * kGroup;
+                }
+                phys = -1;
+                if (more && base + k < lw.take) {
+                    phys = __ldg(p.tables + (int64_t)lw.b * p.table_stride + lw.p0 + base + k);
+                    if (phys < 0) phys = INT_MAX;  // a bad entry, reported when it is loaded
+                }
+                head = p.kv_pool + kv4_offset(0, p.layer, lw.seg / p.slices, p.num_layers,
+                                              p.num_kv_heads, HD);
+            };
+            advance();
+            int stage = 0, issued = 0;
+            uint32_t phase = 1;  // the first round finds every stage free
+            uint64_t since = 0;
+            for (uint32_t it = 0; __any_sync(0xffffffffu, more); ++it) {
+                const bool ready = more && test_wait(&empty[w][stage], phase);
+                if (ready) {
+                    uint64_t *bar = &full[w][stage];
+                    const uint32_t dst = dst0 + stage * C::kStage;
+                    if ((uint32_t)phys < p.num_blocks) {
+                        mbar_arrive_expect_tx(bar, C::kPage);
+                        bulk_load(dst, head + phys * page_stride, C::kPage, bar);
+                    } else {
+                        if (phys != -1) {  // a table entry outside the pool reads as zeros
+                            set_status(p.status, LC_DEV_BAD_BLOCK);
+                            for (int i = 0; i < C::kPage / 16; ++i)
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst + 16 * i),
+                                             "r"(0) : "memory");
+                            // before the copies that fill the stage later
+                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        }
+                        mbar_arrive(bar);
                     }
-                    mbar_arrive(bar);
+                    ++issued;
+                    if (++stage == C::kStages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                    base += kGroup * kWarps;
+                    advance();
                 }
-                ++issued;
-                if (++stage == C::kStages) {
-                    stage = 0;
-                    phase ^= 1;
+                if (__any_sync(0xffffffffu, ready)) {
+                    since = 0;
+                    continue;
                 }
-                base += kGroup * kWarps;
-                advance();
-            }
-            if (__any_sync(0xffffffffu, ready)) {
-                since = 0;
-                continue;
-            }
-            // nothing to do: wait a little, for 2 s at most
-            __nanosleep(40);
-            if ((it & 63) == 0) {
-                const uint64_t now = global_timer_ns();
-                if (since == 0) since = now;
-                if (now - since > kWaitLimitNs) {
-                    s_abort = 1;
-                    set_status(p.status, LC_DEV_TIMEOUT);
+                // nothing to do: wait a little, for 2 s at most
+                __nanosleep(40);
+                if ((it & 63) == 0) {
+                    const uint64_t now = global_timer_ns();
+                    if (since == 0) since = now;
+                    if (now - since > kWaitLimitNs) {
+                        s_abort = 1;
+                        set_status(p.status, LC_DEV_TIMEOUT);
+                    }
+                    if (*(volatile int *)&s_abort) break;
                 }
-                if (*(volatile int *)&s_abort) break;
             }
+            // After a timeout the computing warps may leave stages unread: no copy may land
+            // in a CTA that is gone.
+            __syncwarp();
+            if (*(volatile int *)&s_abort && lane < kGroup * kWarps)
+                for (int i = max(0, issued - C::kStages); i < issued; ++i)
+                    mbar_wait_drain(&full[w][i % C::kStages], i / C::kStages & 1);
+            return;
         }
-        // After a timeout the computing warps may leave stages unread: no copy may land
-        // in a CTA that is gone.
-        __syncwarp();
-        if (*(volatile int *)&s_abort && lane < kGroup * kWarps)
-            for (int i = max(0, issued - C::kStages); i < issued; ++i)
-                mbar_wait_drain(&full[w][i % C::kStages], i / C::kStages & 1);
-        return;
-    }
 
-    if (warp == kEdgeWarp) {
-        // ---- rows of sequences without tokens are zeros
-        for (int b = cta; b < p.batch; b += gridDim.x) {
+        // ---- the edge warps
+        const int edge = kEdges == 1 ? 0 : warp - kEdgeWarp;
+        // rows of sequences without tokens are zeros
+        for (int b = cta + edge * gridDim.x; b < p.batch; b += kEdges * gridDim.x) {
             if (tokens_of(p, b, false) > 0) continue;
             const int width = p.num_q_heads * HD;
             for (int i = lane; i < p.tokens * width; i += 32)
                 p.out[((int64_t)b * p.tokens + i / width) * p.out_stride + i % width] =
                     __float2bfloat16(0.f);
         }
-        const Cut cut(p, total, gridDim.x);
-        if (lane == 0) s_total = total;  // seen with the first chunk's barrier
+        if (edge == 0 && lane == 0) s_total = total;  // seen with the first chunk's barrier
         Walk cw;
         bool more = first < end;
         if (more) {
@@ -564,7 +573,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
         }
         if (!more) {
             if (lane == 0) {
-                s_chunk[0].take = 0;
+                if (edge == 0) s_chunk[0].take = 0;
                 mbar_arrive(&q_full[0]);
             }
             return;
@@ -572,20 +581,17 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
         // q: column c of the slice is query token c / group, head c % group. Lane (g, t)
         // holds dims t * hd/4 .. of column g, as the products need them. A chunk's rows
         // are read while the chunk before it is prepared and the one before that joined.
-        uint4 raw[NT][HD / 32];
+        uint4 raw[HD / 32];
         auto read_q = [&]() {
-            const int kvh = cw.seg / p.slices, col0 = (cw.seg - kvh * p.slices) * kCols;
+            const int kvh = cw.seg / p.slices;
+            const int col = (cw.seg - kvh * p.slices) * kCols + edge * 8 + g;
+            const int i = col / p.group, h = col - i * p.group;
+            const bf16 *src = p.q + ((int64_t)cw.b * p.tokens + i) * p.q_stride +
+                              (int64_t)(kvh * p.group + h) * HD + t * (HD / 4);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const int col = col0 + nt * 8 + g;
-                const int i = col / p.group, h = col - i * p.group;
-                const bf16 *src = p.q + ((int64_t)cw.b * p.tokens + i) * p.q_stride +
-                                  (int64_t)(kvh * p.group + h) * HD + t * (HD / 4);
-#pragma unroll
-                for (int k = 0; k < HD / 32; ++k)
-                    raw[nt][k] = col < p.cols ? __ldg(reinterpret_cast<const uint4 *>(src) + k)
-                                              : make_uint4(0, 0, 0, 0);
-            }
+            for (int k = 0; k < HD / 32; ++k)
+                raw[k] = col < p.cols ? __ldg(reinterpret_cast<const uint4 *>(src) + k)
+                                      : make_uint4(0, 0, 0, 0);
         };
         read_q();
         ChunkInfo prev{};
@@ -595,37 +601,34 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
             ChunkInfo ch{cw.b, cw.seg, cw.p0, cw.take, cw.n, cw.seg_at, 0};
             more = cw.next(p, end);
             ch.last = !more;
+            const uint32_t *r = reinterpret_cast<const uint32_t *>(raw);
+            uint32_t top = 0;  // largest magnitude, as bf16 bits
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const uint32_t *r = reinterpret_cast<const uint32_t *>(raw[nt]);
-                uint32_t top = 0;  // largest magnitude, as bf16 bits
+            for (int k = 0; k < HD / 8; ++k)
+                top = max(top, max(r[k] & 0x7fffu, (r[k] >> 16) & 0x7fffu));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // 2^-e and 2^e, kept within the normal numbers
+            const int e = min(max((int)(top >> 7) - 127, -126), 126);
+            const float down = __int_as_float((127 - e) << 23);
+            // never zero, so that a masked score stays -inf
+            if (t == 0)
+                s_f[buf][edge * 8 + g] =
+                    fmaxf(p.scale_log2 * __int_as_float((127 + e) << 23), FLT_MIN);
+            uint2 *dst = reinterpret_cast<uint2 *>(q_ops + buf * C::kQ) + edge * kSteps * 32 + lane;
 #pragma unroll
-                for (int k = 0; k < HD / 8; ++k)
-                    top = max(top, max(r[k] & 0x7fffu, (r[k] >> 16) & 0x7fffu));
-                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                // 2^-e and 2^e, kept within the normal numbers
-                const int e = min(max((int)(top >> 7) - 127, -126), 126);
-                const float down = __int_as_float((127 - e) << 23);
-                // never zero, so that a masked score stays -inf
-                if (t == 0)
-                    s_f[buf][nt * 8 + g] =
-                        fmaxf(p.scale_log2 * __int_as_float((127 + e) << 23), FLT_MIN);
-                uint2 *dst = reinterpret_cast<uint2 *>(q_ops + buf * C::kQ) + nt * kSteps * 32 + lane;
+            for (int k = 0; k < HD / 16; ++k) {
+                uint32_t v[2];
 #pragma unroll
-                for (int k = 0; k < HD / 16; ++k) {
-                    uint32_t v[2];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint32_t x = r[2 * k + i];
-                        const __half2 y = __floats2half2_rn(__uint_as_float(x << 16) * down,
-                                                            __uint_as_float(x & 0xffff0000u) * down);
-                        v[i] = *reinterpret_cast<const uint32_t *>(&y) ^ p.q_sign;
-                    }
-                    dst[k * 32] = make_uint2(v[0], v[1]);
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t x = r[2 * k + i];
+                    const __half2 y = __floats2half2_rn(__uint_as_float(x << 16) * down,
+                                                        __uint_as_float(x & 0xffff0000u) * down);
+                    v[i] = *reinterpret_cast<const uint32_t *>(&y) ^ p.q_sign;
                 }
+                dst[k * 32] = make_uint2(v[0], v[1]);
             }
-            if (lane == 0) s_chunk[buf] = ch;
+            if (edge == 0 && lane == 0) s_chunk[buf] = ch;
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_full[buf]);
             if (more) read_q();
@@ -634,8 +637,8 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
                 if (!mbar_wait_bounded(&states_full, (chunk - 1) & 1, &s_abort, p.status)) return;
                 const bool whole = prev.take == pages_of(prev.n);
                 const int64_t seg = (int64_t)prev.b * p.seg_per_seq + prev.seg;
-#pragma unroll 2
-                for (int c = 0; c < kCols; ++c) {
+#pragma unroll(kEdges == 1 ? 2 : 1)
+                for (int c = edge; c < kCols; c += kEdges) {
                     Joined<HD, NT> j;
                     join_states<HD, NT>(s_ml, states, c, lane, j);
                     if (whole)
@@ -648,11 +651,12 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
                 if (!whole) {  // the CTA's first chunk, the end of a segment
                     int c0;
                     const int pieces = pieces_of(p, cut, prev, c0);
-                    const bool mine = lane < kCols && last_piece<kCols>(p, seg, lane, pieces);
+                    const bool mine = lane < kCols && lane % kEdges == edge &&
+                                      last_piece<kCols>(p, seg, lane, pieces);
                     const uint32_t cols = __ballot_sync(0xffffffffu, mine);
-                    if (lane == 0 && cols) {
-                        s_left = prev;
-                        s_left_cols = cols;
+                    if (lane == 0) {
+                        if (edge == 0) s_left = prev;
+                        if (cols) atomicOr(&s_left_cols, cols);
                     }
                 }
             }
@@ -664,6 +668,9 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
     }
 
     // ---- computing warps
+    if constexpr (C::kRegs != 0)
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegs ? C::kRegs : 24));
+    if (p.pdl_mode == 2) griddep_wait();
     const int pi0 = g & 1 ? 7 - (g >> 1) : g >> 1;  // token of tile row g
     const uint8_t *ring = smem + warp * C::kStages * C::kStage;
     int stage = 0;
@@ -983,8 +990,8 @@ struct WsLayout {
 
 // Tiles of 8 columns that a segment takes at once: K and V unpack once for all of
 // them, so as few slices as three tiles allow, and then no more tiles than needed.
-// (24 columns, 8 sequences of 1024 .. 32768 tokens of 64/8 heads of 128: 86 us with
-// three tiles, 104 us as two slices of two.)
+// (24 columns, 8 sequences of 1024 .. 32768 tokens of 64/8 heads of 128: 69 us with
+// three tiles, 101 us as two slices of two.)
 int tiles(int64_t cols) {
     if (cols <= 8) return 1;
     return (cols + 23) / 24 < (cols + 15) / 16 ? 3 : 2;
@@ -1004,6 +1011,15 @@ int launch(DecodeKv4Params p, int max_context_len, cudaStream_t stream) {
     auto kern = decode_kv4_kernel<HD, NT>;
     const int rc = ensure_smem_attr((const void *)kern, C::kSmem);
     if (rc) return rc;
+    if constexpr (C::kRegs != 0) {  // the registers handed over are those of the launch, no more
+        static const bool fits = [&] {
+            cudaFuncAttributes a = {};
+            return cudaFuncGetAttributes(&a, kern) == cudaSuccess &&
+                   C::kWarps * C::kRegs + (1 + C::kEdges) * C::kSideRegs <=
+                       C::kThreads / 32 * a.numRegs;
+        }();
+        if (!fits) return LC_ERR_NOT_SUPPORTED;
+    }
     p.slices = (p.cols + C::kCols - 1) / C::kCols;
     p.seg_per_seq = p.num_kv_heads * p.slices;
     // the stream's indexes are int32
