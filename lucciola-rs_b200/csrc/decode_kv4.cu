@@ -13,6 +13,14 @@
 // (arrival counter) joins them in the order of the stream, so the result does
 // not depend on timing.
 //
+// Bounds. 64 sequences of 1024 .. 16384 tokens, 64/8 heads of 128: 125 us, 4.9 TB/s
+// of pages (75 % of a device copy's rate); 32 of 8192, 28/4 heads: 39 us, 3.8 TB/s. A
+// page of 128 dims costs 263 instructions of a warp, about half of them at half
+// rate, nearly the issue slots of the time that it takes from memory: unpacking
+// binds before the bytes do. Short work is bound by its ends, length -> table ->
+// page before the first product and the join after the last: one sequence of 1024
+// tokens 6.9 us.
+//
 // Inside a CTA eight warps compute, taking groups of kGroup pages in turn, each
 // from a ring of its own. A loading warp fills the rings, one lane per page of a
 // group: one bulk copy brings K and V of the kv head (18 hd bytes, contiguous),
@@ -52,8 +60,8 @@ namespace lc {
 namespace {
 
 constexpr int kGroup = 2;             // pages of one warp at a time
-constexpr int kMinPages = 16;         // pages per CTA at least
-constexpr int kEdgeUnits = 24;
+constexpr int kMinPages = 16;         // pages per CTA at least: a group for each of its warps
+constexpr int kEdgeUnits = 32;        // see edge_units
 constexpr float kLazy = 8.f;  // p may reach 2^8 before O and l are rescaled
 
 struct DecodeKv4Params {
@@ -76,6 +84,7 @@ struct DecodeKv4Params {
     uint32_t q_sign;   // sign of sm_scale, on both halves of an fp16 pair
     float v_scale;
     int pdl_mode;
+    int seg_ctas;   // CTAs of the grid per segment, when there is one sequence
     int *ws_cnt;    // [batch * seg_per_seq][kCols] arrivals
     float2 *ws_ml;  // [pieces][kCols] m, l
     float *ws_o;    // [pieces][kCols][hd]
@@ -184,8 +193,11 @@ __device__ __forceinline__ int pages_of(int tokens) {
 
 // Units of one segment in the stream: its pages and, before them, kEdgeUnits
 // without a page, about what a chunk's two ends cost in page times; without them
-// a CTA whose pages lie in many short segments takes longer than the others. A
-// single sequence fills no CTA with several segments and has none.
+// a CTA whose pages lie in many short segments takes longer than the others. (64
+// sequences of 256 .. 4096 tokens, 14/2 heads of 64: 15.0 us with 32 units, 15.7
+// with 24, 19.1 with none; 256 of 100 .. 300: 16.1, 16.1, 20.6; 32 of 8192, 28/4
+// heads of 128: 39.0, 38.9, 40.0, and 40.0 with 36.) A single sequence fills no
+// CTA with several segments and has none.
 __device__ __forceinline__ int edge_units(const DecodeKv4Params &p) {
     return p.batch > 1 ? kEdgeUnits : 0;
 }
@@ -193,16 +205,30 @@ __device__ __forceinline__ int units_of(const DecodeKv4Params &p, int tokens) {
     return tokens > 0 ? pages_of(tokens) + edge_units(p) : 0;
 }
 
+// CTAs that share the stream, of the grid's. `pages`: those of a segment when there is
+// one sequence.
+__device__ __forceinline__ int ctas_of(const DecodeKv4Params &p, int total, int pages) {
+    // One sequence: as many CTAs for each segment, so that none of them joins two in
+    // turn, and no more than the rounds of groups ask for that the fullest one works
+    // through. (28/4 heads of 128, 12345 tokens: 256 CTAs of 13 pages 18.8 us, 196 of 16
+    // 14.1 us; 32768 tokens: 296 of 28 19.1 us, 256 of 32 17.8 us.) From the fifth round
+    // on a full grid does as well (100000 tokens, 64/8 heads: 34.8 us, 36.0 us in rounds).
+    if (p.batch == 1 && p.seg_ctas > 0) {
+        int each = p.seg_ctas;
+        for (int r = 1; r <= 4; ++r) {
+            if (pages > kMinPages * r * p.seg_ctas) continue;
+            each = r == 1 ? (pages + kMinPages - 1) / kMinPages
+                          : (int)((unsigned)(pages + kMinPages * r - 1) / (unsigned)(kMinPages * r));
+            break;
+        }
+        return max(1, each * p.seg_per_seq);
+    }
+    return max(1, min((int)gridDim.x, (total + kMinPages - 1) / kMinPages));
+}
+
 // The stream over `ctas` CTAs: CTA c takes the units from total * c / ctas on.
 struct Cut {
     int total, ctas;
-    __device__ __forceinline__ Cut(const DecodeKv4Params &p, int units, int max_ctas) {
-        total = units;
-        ctas = max(1, min(max_ctas, (total + kMinPages - 1) / kMinPages));
-        // One sequence on part of the GPU: whole CTAs per segment, so that none of them
-        // joins two segments in turn.
-        if (p.batch == 1 && ctas < max_ctas && ctas > p.seg_per_seq) ctas -= ctas % p.seg_per_seq;
-    }
     // In 32 bits where the products fit: a 64-bit division costs a good part of a
     // microsecond before the first load.
     __device__ __forceinline__ int start(int cta) const {
@@ -210,7 +236,8 @@ struct Cut {
         return (int)((long long)total * cta / ctas);
     }
     __device__ __forceinline__ int owner(int unit) const {
-        if (total < (1 << 22)) return (int)((((unsigned)unit + 1u) * (unsigned)ctas - 1u) / (unsigned)total);
+        if (total < (1 << 22))
+            return (int)((((unsigned)unit + 1u) * (unsigned)ctas - 1u) / (unsigned)total);
         return (int)((((long long)unit + 1) * ctas - 1) / total);
     }
 };
@@ -387,7 +414,8 @@ __device__ __forceinline__ void join_pieces(const DecodeKv4Params &p, int64_t pl
 }
 
 // The pieces of a chunk's segment: the CTA of the first one, and how many.
-__device__ __forceinline__ int pieces_of(const DecodeKv4Params &p, const Cut &cut, const ChunkInfo &ch, int &c0) {
+__device__ __forceinline__ int pieces_of(const DecodeKv4Params &p, const Cut &cut,
+                                         const ChunkInfo &ch, int &c0) {
     const int first = ch.seg_at + edge_units(p);
     c0 = cut.owner(first);
     return cut.owner(first + pages_of(ch.n) - 1) - c0 + 1;
@@ -410,7 +438,8 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
     __shared__ uint32_t s_left_cols;
     __shared__ float s_f[2][kCols];
     __shared__ float2 s_ml[kWarps][kCols];
-    __shared__ int s_abort, s_total;
+    __shared__ int s_abort;
+    __shared__ Cut s_cut;
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3;
@@ -448,6 +477,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
         int mine = 0;
         for (int b = q0; b < q1; ++b)
             mine += units_of(p, tokens_of(p, b, cta == 0 && warp == kEdgeWarp));
+        const int pages = __shfl_sync(0xffffffffu, mine, 0);
         mine *= p.seg_per_seq;
         int upto = mine;
 #pragma unroll
@@ -456,7 +486,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
             if (lane >= d) upto += u;
         }
         const int total = __shfl_sync(0xffffffffu, upto, 31);
-        const Cut cut(p, total, gridDim.x);
+        const Cut cut{total, ctas_of(p, total, pages)};
         if (cta < cut.ctas) {
             first = cut.start(cta);
             end = cut.start(cta + 1);
@@ -564,7 +594,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
                 p.out[((int64_t)b * p.tokens + i / width) * p.out_stride + i % width] =
                     __float2bfloat16(0.f);
         }
-        if (edge == 0 && lane == 0) s_total = total;  // seen with the first chunk's barrier
+        if (edge == 0 && lane == 0) s_cut = cut;  // seen with the first chunk's barrier
         Walk cw;
         bool more = first < end;
         if (more) {
@@ -943,7 +973,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
         if (!last) continue;
         if (!mbar_wait_bounded(&states_full, chunk & 1, &s_abort, p.status)) return;
         const ChunkInfo ch = s_chunk[buf];
-        const Cut cut(p, s_total, gridDim.x);
+        const Cut cut = s_cut;
         const bool whole = ch.take == pages_of(ch.n);
         const int64_t seg = (int64_t)ch.b * p.seg_per_seq + ch.seg;
         int c0 = 0, pieces = 0;
@@ -1023,15 +1053,18 @@ int launch(DecodeKv4Params p, int max_context_len, cudaStream_t stream) {
     p.slices = (p.cols + C::kCols - 1) / C::kCols;
     p.seg_per_seq = p.num_kv_heads * p.slices;
     // the stream's indexes are int32
-    if ((int64_t)p.batch * (p.table_stride + kEdgeUnits) > INT_MAX / p.seg_per_seq) return LC_ERR_UNSUPPORTED_SHAPE;
+    if ((int64_t)p.batch * (p.table_stride + kEdgeUnits) > INT_MAX / p.seg_per_seq)
+        return LC_ERR_UNSUPPORTED_SHAPE;
     int64_t grid = (int64_t)sm_count() * C::kCtasPerSm;
     if (max_context_len > 0) {  // less work than kMinPages pages per CTA
-        const int64_t pages = (int64_t)p.batch * p.seg_per_seq *
-                              (((int64_t)max_context_len + kBlockSize - 1) / kBlockSize);
-        grid = std::min<int64_t>(grid, (pages + kMinPages - 1) / kMinPages);
+        const int64_t pages = ((int64_t)max_context_len + kBlockSize - 1) / kBlockSize;
+        grid = std::min<int64_t>(grid, (pages + kMinPages - 1) / kMinPages *
+                                           ((int64_t)p.batch * p.seg_per_seq));
     }
+    grid = std::max<int64_t>(grid, 1);
+    p.seg_ctas = (int)(grid / p.seg_per_seq);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)std::max<int64_t>(grid, 1));
+    cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(C::kThreads);
     cfg.dynamicSmemBytes = C::kSmem;
     cfg.stream = stream;

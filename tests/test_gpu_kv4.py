@@ -419,6 +419,16 @@ def test_decode_many_short_sequences():
     check_decode(8, 1, 128, rng.integers(1, 20, 900), seed=23, hint=19)
 
 
+@pytest.mark.parametrize("n", [2304, 2305, 4608, 4609, 7003, 9216, 9217])
+def test_decode_one_sequence_in_several_rounds(n):
+    """Around the lengths from which each CTA works through one more round of pages."""
+    check_decode(32, 32, 64, [n], seed=n)
+
+
+def test_decode_one_sequence_of_more_heads_than_ctas():
+    check_decode(300, 300, 64, [41], seed=5)
+
+
 @pytest.mark.parametrize("mode", [1, 2])
 def test_decode_with_dependent_launch(mode):
     """An append and the decode over it, back to back: the same bits in every launch mode."""
