@@ -450,6 +450,13 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
         griddep_launch_dependents();
         if (p.pdl_mode == 1) griddep_wait();
     }
+    // The side warps need the lengths first: their reads go out before the barriers are set up.
+    int mine = 0;  // units of this lane's sequences
+    const int per = (p.batch + 31) / 32;
+    const int q0 = min(p.batch, lane * per), q1 = min(p.batch, q0 + per);
+    if (warp >= kWarps)
+        for (int b = q0; b < q1; ++b)
+            mine += units_of(p, tokens_of(p, b, cta == 0 && warp == kEdgeWarp));
     if (warp < kWarps && lane < C::kStages) {
         mbar_init(&full[warp][lane], kGroup);
         mbar_init(&empty[warp][lane], 1);
@@ -472,11 +479,6 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
         if constexpr (C::kRegs != 0)
             asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kSideRegs));
         int first = 0, end = 0, b0 = 0, before = 0;
-        const int per = (p.batch + 31) / 32;
-        const int q0 = min(p.batch, lane * per), q1 = min(p.batch, q0 + per);
-        int mine = 0;
-        for (int b = q0; b < q1; ++b)
-            mine += units_of(p, tokens_of(p, b, cta == 0 && warp == kEdgeWarp));
         const int pages = __shfl_sync(0xffffffffu, mine, 0);
         mine *= p.seg_per_seq;
         int upto = mine;
