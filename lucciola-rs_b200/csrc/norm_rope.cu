@@ -16,10 +16,18 @@
 //
 // hd/16 lanes share a head, each with 8 dims of the first half and their 8
 // rotation partners: two 16-byte loads, both halves of a rotation in one
-// thread, a reduction of 2 or 3 shuffles. A warp takes 32 / (hd/16) heads of one
-// row at a time and loads the next ones before it works on these, so that a
-// read's latency (the row, and the position before the cos and sin) is not paid
-// once per set of warps that fits the GPU.
+// thread, a reduction of 2 or 3 shuffles. A warp takes 32 / (hd/16) heads at a time,
+// in the order of the rows and across their ends (18 heads of 64 in turns of 8: 2.25
+// per row, not 3; 16384 such rows 18.3 us, 20.8 us with turns that end with the row).
+// The grid stays, and a warp loads its next heads before it works on these, so that a
+// read's latency (the row, and the position before the cos and sin) is not paid once
+// per set of warps that fits the GPU (16384 rows of 12/2 heads of 128: 29.6 us, 32.5 us
+// with a warp per turn).
+//
+// Bounds. Those 16384 rows move 143 MB at 4.8 TB/s, 74 % of a device copy's rate; what
+// is missing are issue slots, the products and sums not being contracted. Into the
+// 4-bit pool (8192 rows of 28/4 heads, 34 us, 64 %) the quotients of K and V come on
+// top. 32 rows are launch and latency: 2.4 us.
 #include <algorithm>
 #include <cfloat>
 #include <climits>
@@ -51,7 +59,6 @@ struct NormRopeParams {
     float k_scale, v_scale;
     int64_t num_blocks;
     int num_layers, layer, num_q_heads, num_kv_heads;
-    int groups;  // warp tasks per row
     int *status;
 };
 
@@ -118,25 +125,26 @@ __global__ void __launch_bounds__(kNormRopeThreads, kNormRopeCtas) norm_rope_app
     const int hq = p.num_q_heads, hk = hq + p.num_kv_heads, heads = hk + p.num_kv_heads;
     const int c8 = (lane % kLanes) * 8;
     const uint64_t one = pair2(p.one, p.one), minus_one = pair2(-p.one, -p.one);
-    const uint32_t tasks = (uint32_t)p.rows * p.groups;  // kHeads heads of one row each
+    // a task: kHeads heads in turn, of one row or of several
+    const uint32_t total = (uint32_t)p.rows * heads, tasks = (total + kHeads - 1) / kHeads;
     const uint32_t step = gridDim.x * (kNormRopeThreads / 32);
 
     struct Task {
         uint4 a, b;  // this lane's dims of both halves
-        int row, first, pos, slot;
+        int row, h, pos, slot;
     };
     auto fetch = [&](uint32_t task, Task &k) {
-        const uint32_t row = task / (uint32_t)p.groups;
+        const uint32_t i = task * kHeads + lane / kLanes;
+        const uint32_t row = i / (uint32_t)heads;
         k.row = (int)row;
-        k.first = (int)(task - row * p.groups) * kHeads;
-        const int h = k.first + lane / kLanes;
+        k.h = (int)(i - row * heads);
         k.a = k.b = make_uint4(0, 0, 0, 0);
-        if (h < heads) {
-            // plain loads: q_out may be these rows
-            const bf16 *src = p.qkv + (int64_t)k.row * p.row_stride + (int64_t)h * HD + c8;
-            k.a = *reinterpret_cast<const uint4 *>(src);
-            k.b = *reinterpret_cast<const uint4 *>(src + kHalf);
-        }
+        k.pos = k.slot = -1;
+        if (i >= total) return;
+        // plain loads: q_out may be these rows
+        const bf16 *src = p.qkv + (int64_t)k.row * p.row_stride + (int64_t)k.h * HD + c8;
+        k.a = *reinterpret_cast<const uint4 *>(src);
+        k.b = *reinterpret_cast<const uint4 *>(src + kHalf);
         k.pos = __ldg(p.positions + k.row);
         k.slot = __ldg(p.slot_map + k.row);
     };
@@ -147,30 +155,28 @@ __global__ void __launch_bounds__(kNormRopeThreads, kNormRopeCtas) norm_rope_app
     fetch(task, next);
     for (; task < tasks; task += step) {
         const Task cur = next;
+        const int h = cur.h;
+        const bool is_q = h < hq, is_v = h >= hk;
+        const int hl = is_q ? h : is_v ? h - hk : h - hq;  // head within its part
+        const bool live = cur.pos >= 0 && cur.pos < p.rope_rows;  // not: a padding row, or none
         uint64_t cs[4] = {}, sn[4] = {};
-        const bool pos_ok = cur.pos >= 0 && cur.pos < p.rope_rows;
-        if (pos_ok && cur.first < hk) {
+        if (live && !is_v) {
             load8f(p.cos_t + (int64_t)cur.pos * kHalf + c8, cs);
             load8f(p.sin_t + (int64_t)cur.pos * kHalf + c8, sn);
         }
         if (task + step < tasks) fetch(task + step, next);
-        if (!pos_ok) {  // -1: a padding row
-            if (cur.pos != -1 && cur.first == 0 && lane == 0) set_status(p.status, LC_DEV_BAD_POS);
-            continue;
-        }
         const bool stored = cur.slot >= 0 && cur.slot < p.num_blocks * kBlockSize;
-        if (!stored && cur.slot != -1 && cur.first == 0 && lane == 0)
-            set_status(p.status, LC_DEV_BAD_BLOCK);
+        if (h == 0 && c8 == 0) {  // one lane per row
+            if (!live && cur.pos != -1) set_status(p.status, LC_DEV_BAD_POS);
+            if (live && !stored && cur.slot != -1) set_status(p.status, LC_DEV_BAD_BLOCK);
+        }
+        if (!__any_sync(0xffffffffu, live)) continue;
         const int phys = cur.slot / kBlockSize, off = cur.slot % kBlockSize;
-
-        const int h = cur.first + lane / kLanes;
-        const bool is_q = h < hq, is_v = h >= hk;
-        const int hl = is_q ? h : is_v ? h - hk : h - hq;  // head within its part
         uint64_t x1[4], x2[4];
         unpack8(cur.a, x1);
         unpack8(cur.b, x2);
         const bf16 *bias = is_q ? p.q_bias : is_v ? p.v_bias : p.k_bias;
-        if (bias && h < heads) {
+        if (bias && live) {
             uint64_t t1[4], t2[4];
             unpack8(ldg16(bias + (int64_t)hl * HD + c8), t1);
             unpack8(ldg16(bias + (int64_t)hl * HD + c8 + kHalf), t2);
@@ -180,7 +186,7 @@ __global__ void __launch_bounds__(kNormRopeThreads, kNormRopeCtas) norm_rope_app
                 x2[e] = add2(x2[e], t2[e]);
             }
         }
-        if (cur.first < hk) {  // warp-uniform: some head of this turn is q or k
+        if (__any_sync(0xffffffffu, !is_v)) {  // some head of this turn is q or k
             const bf16 *w = is_q ? p.q_norm : p.k_norm;
             if (p.q_norm || p.k_norm) {  // for the whole warp: the sum goes across lanes
                 const float r = rms_factor<HD>(x1, x2, p.eps, one);
@@ -205,17 +211,17 @@ __global__ void __launch_bounds__(kNormRopeThreads, kNormRopeCtas) norm_rope_app
                 }
             }
         }
-        if (is_q) {
+        if (is_q && live) {
             bf16 *dst = p.q_out + (int64_t)cur.row * p.q_out_stride + (int64_t)h * HD + c8;
             *reinterpret_cast<uint4 *>(dst) = pack8(x1);
             *reinterpret_cast<uint4 *>(dst + kHalf) = pack8(x2);
         }
-        if (cur.first + kHeads <= hq) continue;  // warp-uniform: only queries in this turn
+        if (__all_sync(0xffffffffu, is_q)) continue;  // only queries in this turn
         if constexpr (KV4) {
             const float g = is_v ? p.v_scale : p.k_scale;
             const uint32_t m1 = group_amax(x1), m2 = group_amax(x2);
             const uint32_t s1 = kv4_scale_byte(m1, 6.f * g), s2 = kv4_scale_byte(m2, 6.f * g);
-            if (is_q || h >= heads || !stored) continue;
+            if (is_q || !live || !stored) continue;
             uint8_t *page = p.kv_pool + kv4_offset(phys, p.layer, hl, p.num_layers,
                                                    p.num_kv_heads, HD) +
                             (is_v ? kv4_half_bytes(HD) : 0);
@@ -228,7 +234,7 @@ __global__ void __launch_bounds__(kNormRopeThreads, kNormRopeCtas) norm_rope_app
                 sc[kHalf / kKv4Group] = (uint8_t)s2;
             }
         } else {
-            if (is_q || h >= heads || !stored) continue;
+            if (is_q || !live || !stored) continue;
             bf16 *dst = (is_v ? p.v_pool : p.k_pool) +
                         (page_row(phys, p.layer, hl, p.num_layers, p.num_kv_heads) + off) * HD + c8;
             *reinterpret_cast<uint4 *>(dst) = pack8(x1);
@@ -240,9 +246,10 @@ __global__ void __launch_bounds__(kNormRopeThreads, kNormRopeCtas) norm_rope_app
 template <int HD, bool KV4>
 int launch_dim(NormRopeParams p, cudaStream_t stream) {
     constexpr int kHeads = 32 / (HD / 16), kWarps = kNormRopeThreads / 32;
-    p.groups = (p.num_q_heads + 2 * p.num_kv_heads + kHeads - 1) / kHeads;
-    const int64_t tasks = (int64_t)p.rows * p.groups;
-    if (tasks > INT_MAX) return LC_ERR_UNSUPPORTED_SHAPE;
+    // 32-bit head numbers; more heads than that do not fit the memory
+    const int64_t total = (int64_t)p.rows * (p.num_q_heads + 2 * p.num_kv_heads);
+    if (total > INT_MAX) return LC_ERR_UNSUPPORTED_SHAPE;
+    const int64_t tasks = (total + kHeads - 1) / kHeads;
     const int64_t blocks = std::min<int64_t>((tasks + kWarps - 1) / kWarps,
                                              (int64_t)sm_count() * kNormRopeCtas);
     norm_rope_append_kernel<HD, KV4><<<(unsigned)blocks, kNormRopeThreads, 0, stream>>>(p);
