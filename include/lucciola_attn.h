@@ -79,6 +79,8 @@ const char *lc_version(void);
  *     then not write the context lengths/positions, the block tables, the
  *     biases, the RoPE tables, or this layer's cached K/V (a decode step's QKV
  *     projection or another layer's attention qualifies).
+ * lc_paged_decode_kv4 follows the mode too; in mode 2 it reads nothing but the
+ * context lengths before the wait.
  * Returns the previous mode, or -1 for an invalid mode. */
 int lc_set_dependent_launch(int mode);
 

@@ -117,7 +117,8 @@ __device__ __forceinline__ uint32_t group_amax(const uint64_t (&x)[4]) {
 }
 
 template <int HD, bool KV4>
-__global__ void __launch_bounds__(kNormRopeThreads, kNormRopeCtas) norm_rope_append_kernel(NormRopeParams p) {
+__global__ void __launch_bounds__(kNormRopeThreads, kNormRopeCtas)
+    norm_rope_append_kernel(NormRopeParams p) {
     constexpr int kLanes = HD / 16;      // lanes per head
     constexpr int kHeads = 32 / kLanes;  // heads per warp at a time
     constexpr int kHalf = HD / 2;
