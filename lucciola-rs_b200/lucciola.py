@@ -346,8 +346,10 @@ def gather_kv(k_out, v_out, k_pool, v_pool, num_blocks, num_layers, layer, num_k
 
 # ------------------------------------------------ device-side step, 4-bit cache --
 
+# t.stride()[0] below takes 0.15 us, t.stride(0) 0.26, of calls of about 9 us.
+
 def _nbytes(t):
-    return 0 if t is None else t.numel() * t.element_size()
+    return 0 if t is None else t.nbytes
 
 
 def alloc_step_workspace(device="cuda"):
@@ -361,10 +363,10 @@ def step_tables(block_tables, context_lens, new_lens, free_pages, free_count, po
                 dev_status=None, stream=None):
     """A step's pages, table rows, positions and slot map from the requests' lengths.
     All int32 device tensors; context_out may be context_lens, free_count_out free_count."""
-    check(lib.lc_step_tables(_p(block_tables), block_tables.stride(0), block_tables.shape[0],
+    check(lib.lc_step_tables(_p(block_tables), block_tables.stride()[0], block_tables.shape[0],
                              _p(slots), _p(context_lens), _p(new_lens), context_lens.shape[0],
                              _p(free_pages), _p(free_count), free_pages.shape[0], _p(step_tables),
-                             0 if step_tables is None else step_tables.stride(0), _p(positions),
+                             0 if step_tables is None else step_tables.stride()[0], _p(positions),
                              _p(slot_map), positions.shape[0], _p(row_starts), _p(context_out),
                              _p(free_count_out), _p(workspace), _nbytes(workspace),
                              _p(dev_status), _stream(stream)), "lc_step_tables")
@@ -374,7 +376,7 @@ def step_release(free_pages, free_count, block_tables, context_lens, free_count_
                  slots=None, dev_status=None, stream=None):
     """Returns the pages of finished requests to the free stack."""
     check(lib.lc_step_release(_p(free_pages), _p(free_count), free_pages.shape[0],
-                              _p(block_tables), block_tables.stride(0), block_tables.shape[0],
+                              _p(block_tables), block_tables.stride()[0], block_tables.shape[0],
                               _p(slots), _p(context_lens), context_lens.shape[0],
                               _p(free_count_out), _p(workspace), _nbytes(workspace),
                               _p(dev_status), _stream(stream)), "lc_step_release")
@@ -386,7 +388,7 @@ def qk_norm_rope_append(q_out, qkv, positions, slot_map, cos, sin, k_pool, v_poo
                         dev_status=None, stream=None):
     """Bias, RMS norm per q / k head, RoPE and append by slot, into bf16 pools."""
     check(lib.lc_qk_norm_rope_append(
-        _p(q_out), q_out.stride(0), _p(qkv), qkv.stride(0), positions.shape[0], _p(positions),
+        _p(q_out), q_out.stride()[0], _p(qkv), qkv.stride()[0], positions.shape[0], _p(positions),
         _p(slot_map), _p(q_bias), _p(k_bias), _p(v_bias), _p(q_norm), _p(k_norm), eps, _p(cos),
         _p(sin), cos.shape[0], _p(k_pool), _p(v_pool), num_blocks, num_layers, layer, num_q_heads,
         num_kv_heads, head_dim, _p(dev_status), _stream(stream)), "lc_qk_norm_rope_append")
@@ -412,7 +414,7 @@ def qk_norm_rope_append_kv4(q_out, qkv, positions, slot_map, cos, sin, kv_pool, 
                             k_bias=None, v_bias=None, dev_status=None, stream=None):
     """qk_norm_rope_append into a 4-bit pool."""
     check(lib.lc_qk_norm_rope_append_kv4(
-        _p(q_out), q_out.stride(0), _p(qkv), qkv.stride(0), positions.shape[0], _p(positions),
+        _p(q_out), q_out.stride()[0], _p(qkv), qkv.stride()[0], positions.shape[0], _p(positions),
         _p(slot_map), _p(q_bias), _p(k_bias), _p(v_bias), _p(q_norm), _p(k_norm), eps, _p(cos),
         _p(sin), cos.shape[0], _p(kv_pool), k_scale, v_scale, num_blocks, num_layers, layer,
         num_q_heads, num_kv_heads, head_dim, _p(dev_status), _stream(stream)),
@@ -424,7 +426,7 @@ def unpack_kv4(k_out, v_out, kv_pool, num_blocks, num_layers, layer, num_kv_head
                len_offset=0, dev_status=None, stream=None):
     """The sequences' 4-bit pages as bf16 pages [batch * P][1][Hkv][16][hd]."""
     check(lib.lc_unpack_kv4(_p(k_out), _p(v_out), _p(kv_pool), num_blocks, num_layers, layer,
-                            num_kv_heads, head_dim, _p(block_tables), block_tables.stride(0),
+                            num_kv_heads, head_dim, _p(block_tables), block_tables.stride()[0],
                             _p(context_lens), len_offset, context_lens.shape[0], max_context_len,
                             k_scale, v_scale, _p(dev_status), _stream(stream)), "lc_unpack_kv4")
 
@@ -445,9 +447,9 @@ def paged_decode_kv4(out, q, kv_pool, num_blocks, num_layers, layer, num_q_heads
     """Attention of each sequence's newest tokens_per_seq tokens over a 4-bit pool."""
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(head_dim)
-    check(lib.lc_paged_decode_kv4(_p(out), out.stride(0), _p(q), q.stride(0), _p(kv_pool),
+    check(lib.lc_paged_decode_kv4(_p(out), out.stride()[0], _p(q), q.stride()[0], _p(kv_pool),
                                   num_blocks, num_layers, layer, num_q_heads, num_kv_heads,
-                                  head_dim, _p(block_tables), block_tables.stride(0),
+                                  head_dim, _p(block_tables), block_tables.stride()[0],
                                   _p(context_lens), len_offset, context_lens.shape[0],
                                   tokens_per_seq, max_context_len, k_scale, v_scale, sm_scale,
                                   _p(workspace), _nbytes(workspace), _p(dev_status),
