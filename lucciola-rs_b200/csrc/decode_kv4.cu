@@ -254,8 +254,14 @@ struct Walk {
         b = b0;
         n = tokens_of(p, b, false);
         const int units = units_of(p, n);  // not zero
-        seg = (first - before_b0) / units;
-        seg_at = before_b0 + seg * units;
+        // by steps: there are few segments, and the first load waits for this
+        seg = 0, seg_at = before_b0;
+        if (p.seg_per_seq <= 8) {
+            for (; first >= seg_at + units; ++seg) seg_at += units;
+        } else {
+            seg = (first - before_b0) / units;
+            seg_at += seg * units;
+        }
         unit = first;
         p0 = take = 0;
     }
@@ -280,6 +286,11 @@ struct Walk {
         return false;
     }
 };
+
+// The kv head of a segment, without the division in the ordinary case.
+__device__ __forceinline__ int kv_head(const DecodeKv4Params &p, int seg) {
+    return p.slices == 1 ? seg : seg / p.slices;
+}
 
 // What the edge warp tells the computing warps about a chunk.
 struct ChunkInfo {
@@ -324,7 +335,7 @@ template <int HD, int NT>
 __device__ __forceinline__ void write_row(const DecodeKv4Params &p, const ChunkInfo &ch, int c,
                                           int lane, const Joined<HD, NT> &j) {
     constexpr int kPer = HD / 32;
-    const int kvh = ch.seg / p.slices, col = (ch.seg - kvh * p.slices) * Cfg<HD, NT>::kCols + c;
+    const int kvh = kv_head(p, ch.seg), col = (ch.seg - kvh * p.slices) * Cfg<HD, NT>::kCols + c;
     if (col >= p.cols) return;
     const int qi = col / p.group, h = col - qi * p.group;
     // a row without tokens gets zeros
@@ -377,14 +388,16 @@ __device__ __forceinline__ void join_pieces(const DecodeKv4Params &p, int64_t pl
     constexpr int kCols = Cfg<HD, NT>::kCols, kPer = HD / 32;
     const float2 *bml = p.ws_ml + place * kCols + c;
     const float *bo = p.ws_o + (place * kCols + c) * HD + lane * kPer;
+    constexpr int kBatch = 8;  // pieces read at once
     j.m = -INFINITY;
-    for (int k = lane; k < pieces; k += 32) j.m = fmaxf(j.m, __ldcg(&bml[k * kCols].x));
+    if (pieces > kBatch) {
+        for (int k = lane; k < pieces; k += 32) j.m = fmaxf(j.m, __ldcg(&bml[k * kCols].x));
 #pragma unroll
-    for (int d = 16; d; d >>= 1) j.m = fmaxf(j.m, __shfl_xor_sync(0xffffffffu, j.m, d));
+        for (int d = 16; d; d >>= 1) j.m = fmaxf(j.m, __shfl_xor_sync(0xffffffffu, j.m, d));
+    }
     j.l = 0.f;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) j.o[i] = 0.f;
-    constexpr int kBatch = 8;  // pieces read at once
     for (int k0 = 0; k0 < pieces; k0 += kBatch) {
         float2 ml[kBatch];
         float x[kBatch][kPer];
@@ -401,6 +414,10 @@ __device__ __forceinline__ void join_pieces(const DecodeKv4Params &p, int64_t pl
                 const float2 v = __ldcg(reinterpret_cast<const float2 *>(src));
                 x[i][0] = v.x, x[i][1] = v.y;
             }
+        }
+        if (pieces <= kBatch) {  // the only turn: the maximum comes with it
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) j.m = fmaxf(j.m, ml[i].x);
         }
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
@@ -527,7 +544,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
                     phys = __ldg(p.tables + (int64_t)lw.b * p.table_stride + lw.p0 + base + k);
                     if (phys < 0) phys = INT_MAX;  // a bad entry, reported when it is loaded
                 }
-                head = p.kv_pool + kv4_offset(0, p.layer, lw.seg / p.slices, p.num_layers,
+                head = p.kv_pool + kv4_offset(0, p.layer, kv_head(p, lw.seg), p.num_layers,
                                               p.num_kv_heads, HD);
             };
             advance();
@@ -615,7 +632,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
         // are read while the chunk before it is prepared and the one before that joined.
         uint4 raw[HD / 32];
         auto read_q = [&]() {
-            const int kvh = cw.seg / p.slices;
+            const int kvh = kv_head(p, cw.seg);
             const int col = (cw.seg - kvh * p.slices) * kCols + edge * 8 + g;
             const int i = col / p.group, h = col - i * p.group;
             const bf16 *src = p.q + ((int64_t)cw.b * p.tokens + i) * p.q_stride +
