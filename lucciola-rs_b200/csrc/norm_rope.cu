@@ -24,10 +24,12 @@
 // per set of warps that fits the GPU (16384 rows of 12/2 heads of 128: 29.6 us, 32.5 us
 // with a warp per turn).
 //
-// Bounds. Those 16384 rows move 143 MB at 4.8 TB/s, 74 % of a device copy's rate; what
-// is missing are issue slots, the products and sums not being contracted. Into the
-// 4-bit pool (8192 rows of 28/4 heads, 34 us, 64 %) the quotients of K and V come on
-// top. 32 rows are launch and latency: 2.4 us.
+// Bounds. Those 16384 rows of 128-dim heads now take 27.9 us: 143 MB at 5.1 TB/s, 78 %
+// of a device copy's rate. What is missing are issue slots, the products and sums not
+// being contracted (counting rows and heads on without a division: 29.6 us before).
+// Into the 4-bit pool (8192 rows of 28/4 heads, 33 us, 66 %) the quotients of K and V
+// come on top: 69 % of the issue slots, with the packed operations at half rate. 32
+// rows are launch and latency: 2.4 us.
 #include <algorithm>
 #include <cfloat>
 #include <climits>
@@ -127,21 +129,30 @@ __global__ void __launch_bounds__(kNormRopeThreads, kNormRopeCtas)
     const int c8 = (lane % kLanes) * 8;
     const uint64_t one = pair2(p.one, p.one), minus_one = pair2(-p.one, -p.one);
     // a task: kHeads heads in turn, of one row or of several
-    const uint32_t total = (uint32_t)p.rows * heads, tasks = (total + kHeads - 1) / kHeads;
+    const uint32_t tasks = ((uint32_t)p.rows * heads + kHeads - 1) / kHeads;
     const uint32_t step = gridDim.x * (kNormRopeThreads / 32);
 
     struct Task {
         uint4 a, b;  // this lane's dims of both halves
         int row, h, pos, slot;
     };
-    auto fetch = [&](uint32_t task, Task &k) {
-        const uint32_t i = task * kHeads + lane / kLanes;
-        const uint32_t row = i / (uint32_t)heads;
-        k.row = (int)row;
-        k.h = (int)(i - row * heads);
+    // Row and head that this lane loads next; a step of the grid moves them on without
+    // a division.
+    uint32_t task = blockIdx.x * (kNormRopeThreads / 32) + (threadIdx.x >> 5);
+    if (task >= tasks) return;
+    int row = (int)((task * kHeads + lane / kLanes) / (uint32_t)heads);
+    int head = (int)(task * kHeads + lane / kLanes - (uint32_t)row * heads);
+    const int step_rows = (int)(step * kHeads / (uint32_t)heads);
+    const int step_heads = (int)(step * kHeads - (uint32_t)step_rows * heads);
+    auto fetch = [&](Task &k) {
+        k.row = row;
+        k.h = head;
+        row += step_rows;
+        head += step_heads;
+        if (head >= heads) head -= heads, ++row;
         k.a = k.b = make_uint4(0, 0, 0, 0);
         k.pos = k.slot = -1;
-        if (i >= total) return;
+        if (k.row >= p.rows) return;
         // plain loads: q_out may be these rows
         const bf16 *src = p.qkv + (int64_t)k.row * p.row_stride + (int64_t)k.h * HD + c8;
         k.a = *reinterpret_cast<const uint4 *>(src);
@@ -150,10 +161,8 @@ __global__ void __launch_bounds__(kNormRopeThreads, kNormRopeCtas)
         k.slot = __ldg(p.slot_map + k.row);
     };
 
-    uint32_t task = blockIdx.x * (kNormRopeThreads / 32) + (threadIdx.x >> 5);
-    if (task >= tasks) return;
     Task next;
-    fetch(task, next);
+    fetch(next);
     for (; task < tasks; task += step) {
         const Task cur = next;
         const int h = cur.h;
@@ -165,14 +174,13 @@ __global__ void __launch_bounds__(kNormRopeThreads, kNormRopeCtas)
             load8f(p.cos_t + (int64_t)cur.pos * kHalf + c8, cs);
             load8f(p.sin_t + (int64_t)cur.pos * kHalf + c8, sn);
         }
-        if (task + step < tasks) fetch(task + step, next);
+        if (task + step < tasks) fetch(next);
         const bool stored = cur.slot >= 0 && cur.slot < p.num_blocks * kBlockSize;
         if (h == 0 && c8 == 0) {  // one lane per row
             if (!live && cur.pos != -1) set_status(p.status, LC_DEV_BAD_POS);
             if (live && !stored && cur.slot != -1) set_status(p.status, LC_DEV_BAD_BLOCK);
         }
         if (!__any_sync(0xffffffffu, live)) continue;
-        const int phys = cur.slot / kBlockSize, off = cur.slot % kBlockSize;
         uint64_t x1[4], x2[4];
         unpack8(cur.a, x1);
         unpack8(cur.b, x2);
@@ -218,6 +226,7 @@ __global__ void __launch_bounds__(kNormRopeThreads, kNormRopeCtas)
             *reinterpret_cast<uint4 *>(dst + kHalf) = pack8(x2);
         }
         if (__all_sync(0xffffffffu, is_q)) continue;  // only queries in this turn
+        const int phys = cur.slot / kBlockSize, off = cur.slot % kBlockSize;
         if constexpr (KV4) {
             const float g = is_v ? p.v_scale : p.k_scale;
             const uint32_t m1 = group_amax(x1), m2 = group_amax(x2);
