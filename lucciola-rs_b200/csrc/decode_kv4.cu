@@ -381,32 +381,37 @@ __device__ __forceinline__ bool last_piece(const DecodeKv4Params &p, int64_t seg
     return true;
 }
 
-// Joins the pieces of column c, the first of which lies at `place`, in order.
+__device__ __forceinline__ void cp_async16(void *dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src)
+                 : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// Joins the pieces of column c, the first of which lies at `place`, in order. Up to
+// eight come in one round of reads to registers, more through `buf`, 8 KB of this
+// warp's own, 16 (32 at hd 64) at a time: one sequence of 32768 tokens, 28/4 heads of
+// 128, has 64 per column.
 template <int HD, int NT>
 __device__ __forceinline__ void join_pieces(const DecodeKv4Params &p, int64_t place, int pieces, int c,
-                                            int lane, Joined<HD, NT> &j) {
+                                            int lane, float *buf, Joined<HD, NT> &j) {
     constexpr int kCols = Cfg<HD, NT>::kCols, kPer = HD / 32;
     const float2 *bml = p.ws_ml + place * kCols + c;
-    const float *bo = p.ws_o + (place * kCols + c) * HD + lane * kPer;
-    constexpr int kBatch = 8;  // pieces read at once
-    j.m = -INFINITY;
-    if (pieces > kBatch) {
-        for (int k = lane; k < pieces; k += 32) j.m = fmaxf(j.m, __ldcg(&bml[k * kCols].x));
-#pragma unroll
-        for (int d = 16; d; d >>= 1) j.m = fmaxf(j.m, __shfl_xor_sync(0xffffffffu, j.m, d));
-    }
-    j.l = 0.f;
+    const float *bo = p.ws_o + (place * kCols + c) * HD;
+    j.m = -INFINITY, j.l = 0.f;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) j.o[i] = 0.f;
-    for (int k0 = 0; k0 < pieces; k0 += kBatch) {
-        float2 ml[kBatch];
-        float x[kBatch][kPer];
+    constexpr int kFew = 8;
+    if (pieces <= kFew) {
+        float2 ml[kFew];
+        float x[kFew][kPer];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
+        for (int i = 0; i < kFew; ++i) {
             ml[i] = make_float2(-INFINITY, 0.f);
-            if (k0 + i >= pieces) continue;
-            const float *src = bo + (int64_t)(k0 + i) * kCols * HD;
-            ml[i] = __ldcg(&bml[(k0 + i) * kCols]);
+            if (i >= pieces) continue;
+            const float *src = bo + (int64_t)i * kCols * HD + lane * kPer;
+            ml[i] = __ldcg(&bml[i * kCols]);
             if constexpr (kPer == 4) {
                 const float4 v = __ldcg(reinterpret_cast<const float4 *>(src));
                 x[i][0] = v.x, x[i][1] = v.y, x[i][2] = v.z, x[i][3] = v.w;
@@ -415,18 +420,57 @@ __device__ __forceinline__ void join_pieces(const DecodeKv4Params &p, int64_t pl
                 x[i][0] = v.x, x[i][1] = v.y;
             }
         }
-        if (pieces <= kBatch) {  // the only turn: the maximum comes with it
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) j.m = fmaxf(j.m, ml[i].x);
-        }
+        for (int i = 0; i < kFew; ++i) j.m = fmaxf(j.m, ml[i].x);
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
+        for (int i = 0; i < kFew; ++i) {
             if (ml[i].x == -INFINITY) continue;
             const float r = ex2(ml[i].x - j.m);
             j.l = fmaf(ml[i].y, r, j.l);
 #pragma unroll
             for (int d = 0; d < kPer; ++d) j.o[d] = fmaf(x[i][d], r, j.o[d]);
         }
+        return;
+    }
+    constexpr int kRows = 2048 / HD, kLanes = HD / 4;  // pieces at a time, lanes per piece
+    auto read = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < kRows; i += 32 / kLanes) {
+            const int row = i + lane / kLanes, at = lane % kLanes * 4;
+            if (k0 + row < pieces)
+                cp_async16(buf + row * HD + at, bo + (int64_t)(k0 + row) * kCols * HD + at);
+        }
+    };
+    read(0);
+    float2 ml = make_float2(-INFINITY, 0.f);  // of piece lane, then lane + 32, ..
+    if (lane < pieces) ml = __ldcg(&bml[lane * kCols]);
+    j.m = ml.x;
+    for (int k = lane + 32; k < pieces; k += 32) j.m = fmaxf(j.m, __ldcg(&bml[k * kCols].x));
+#pragma unroll
+    for (int d = 16; d; d >>= 1) j.m = fmaxf(j.m, __shfl_xor_sync(0xffffffffu, j.m, d));
+    for (int k0 = 0; k0 < pieces; k0 += kRows) {
+        if (k0 > 0 && k0 % 32 == 0) {
+            ml = make_float2(-INFINITY, 0.f);
+            if (k0 + lane < pieces) ml = __ldcg(&bml[(k0 + lane) * kCols]);
+        }
+        const float r = ml.x == -INFINITY ? 0.f : ex2(ml.x - j.m);
+        const uint32_t seen = __ballot_sync(0xffffffffu, ml.x != -INFINITY);
+        cp_async_wait_all();
+        __syncwarp();
+        const int rows = min(kRows, pieces - k0);
+#pragma unroll 4
+        for (int i = 0; i < rows; ++i) {
+            const int from = (k0 + i) % 32;
+            const float ri = __shfl_sync(0xffffffffu, r, from);
+            const float li = __shfl_sync(0xffffffffu, ml.y, from);
+            if (!(seen >> from & 1)) continue;
+            j.l = fmaf(li, ri, j.l);
+            const float *x = buf + i * HD + lane * kPer;
+#pragma unroll
+            for (int d = 0; d < kPer; ++d) j.o[d] = fmaf(x[d], ri, j.o[d]);
+        }
+        __syncwarp();
+        if (k0 + kRows < pieces) read(k0 + kRows);
     }
 }
 
@@ -990,6 +1034,9 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
         __syncwarp();
         if (lane == 0) mbar_arrive(&states_full);
         if (!last) continue;
+        // Every page of this warp has been read: its ring takes the pieces.
+        float *join_buf = reinterpret_cast<float *>(smem + warp * C::kStages * C::kStage);
+        static_assert(C::kStages * C::kStage >= 8192 && C::kStages * C::kStage % 16 == 0);
         if (!mbar_wait_bounded(&states_full, chunk & 1, &s_abort, p.status)) return;
         const ChunkInfo ch = s_chunk[buf];
         const Cut cut = s_cut;
@@ -1006,7 +1053,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
                 __syncwarp();
                 const int mine = lane == 0 && last_piece<kCols>(p, seg, c, pieces);
                 if (!__shfl_sync(0xffffffffu, mine, 0)) continue;
-                join_pieces<HD, NT>(p, seg + c0, pieces, c, lane, j);
+                join_pieces<HD, NT>(p, seg + c0, pieces, c, lane, join_buf, j);
             }
             write_row<HD, NT>(p, ch, c, lane, j);
         }
@@ -1021,7 +1068,8 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
         for (int c = warp; c < kCols; c += kWarps) {
             if (!(left >> c & 1)) continue;
             Joined<HD, NT> j;
-            join_pieces<HD, NT>(p, (int64_t)lc.b * p.seg_per_seq + lc.seg + c0, pieces, c, lane, j);
+            join_pieces<HD, NT>(p, (int64_t)lc.b * p.seg_per_seq + lc.seg + c0, pieces, c, lane,
+                                join_buf, j);
             write_row<HD, NT>(p, lc, c, lane, j);
         }
         return;

@@ -425,6 +425,13 @@ def test_decode_one_sequence_in_several_rounds(n):
     check_decode(32, 32, 64, [n], seed=n)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n", [2300, 4100, 4352, 8300, 8704, 20000])
+def test_decode_one_sequence_of_many_pieces(n, hd):
+    """9 to 79 pieces per head, around the 16 and 32 that are joined at a time."""
+    check_decode(4, 2, hd, [n], seed=n)
+
+
 def test_decode_one_sequence_of_more_heads_than_ctas():
     check_decode(300, 300, 64, [41], seed=5)
 
