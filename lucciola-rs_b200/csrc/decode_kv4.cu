@@ -86,6 +86,7 @@ struct DecodeKv4Params {
     int pdl_mode;
     int seg_ctas;   // CTAs of the grid per segment, when there is one sequence
     int *ws_cnt;    // [batch * seg_per_seq][kCols] arrivals
+    int *ws_group;  // [pieces][kCols] arrivals of a group, at its first piece
     float2 *ws_ml;  // [pieces][kCols] m, l
     float *ws_o;    // [pieces][kCols][hd]
     int *status;
@@ -371,12 +372,27 @@ __device__ __forceinline__ void store_piece(const DecodeKv4Params &p, int64_t pl
     if (lane == 0) p.ws_ml[place * kCols + c] = make_float2(j.m, j.l);
 }
 
-// Counts a piece of column c; true for the segment's last one. One lane, after
-// the warp's stores and a __syncwarp.
+// Pieces are joined by the warp that leaves the last one: up to kTreePieces at once,
+// more in groups of kTreeGroup, whose results take the place of their first piece and
+// are joined by the group that ends last, so that one CTA does not read them all.
+// Groups and orders are those of the stream. (One sequence of 32768 tokens, 28/4 heads
+// of 128, 64 pieces per column: 14.1 us, 16.8 us joined by one; 12345 tokens, 49: 11.3,
+// 13.6.)
+constexpr int kTreePieces = 32, kTreeGroup = 8;
+
+// Counts piece `mine` (or, `top`, a joined group) of column c; true for the last one of
+// its group or segment. One lane, after the warp's stores and a __syncwarp.
 template <int kCols>
-__device__ __forceinline__ bool last_piece(const DecodeKv4Params &p, int64_t seg, int c, int pieces) {
+__device__ __forceinline__ bool last_piece(const DecodeKv4Params &p, int64_t seg, int c0, int pieces,
+                                           int mine, int c, bool top) {
     int *cnt = p.ws_cnt + seg * kCols + c;
-    if (atom_add_acq_rel_gpu(cnt, 1) != pieces - 1) return false;
+    int count = pieces;
+    if (pieces > kTreePieces) {
+        const int first = mine / kTreeGroup * kTreeGroup;
+        count = top ? (pieces + kTreeGroup - 1) / kTreeGroup : min(kTreeGroup, pieces - first);
+        if (!top) cnt = p.ws_group + (seg + c0 + first) * kCols + c;
+    }
+    if (atom_add_acq_rel_gpu(cnt, 1) != count - 1) return false;
     *cnt = 0;  // ready for the next call
     return true;
 }
@@ -389,16 +405,17 @@ __device__ __forceinline__ void cp_async_wait_all() {
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// Joins the pieces of column c, the first of which lies at `place`, in order. Up to
+// Joins `pieces` pieces of column c, at `place` and `stride` apart, in order. Up to
 // eight come in one round of reads to registers, more through `buf`, 8 KB of this
-// warp's own, 16 (32 at hd 64) at a time: one sequence of 32768 tokens, 28/4 heads of
-// 128, has 64 per column.
+// warp's own, 16 (32 at hd 64) at a time.
 template <int HD, int NT>
-__device__ __forceinline__ void join_pieces(const DecodeKv4Params &p, int64_t place, int pieces, int c,
-                                            int lane, float *buf, Joined<HD, NT> &j) {
+__device__ __forceinline__ void join_pieces(const DecodeKv4Params &p, int64_t place, int pieces,
+                                            int stride, int c, int lane, float *buf,
+                                            Joined<HD, NT> &j) {
     constexpr int kCols = Cfg<HD, NT>::kCols, kPer = HD / 32;
     const float2 *bml = p.ws_ml + place * kCols + c;
     const float *bo = p.ws_o + (place * kCols + c) * HD;
+    const int apart = stride * kCols;
     j.m = -INFINITY, j.l = 0.f;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) j.o[i] = 0.f;
@@ -410,8 +427,8 @@ __device__ __forceinline__ void join_pieces(const DecodeKv4Params &p, int64_t pl
         for (int i = 0; i < kFew; ++i) {
             ml[i] = make_float2(-INFINITY, 0.f);
             if (i >= pieces) continue;
-            const float *src = bo + (int64_t)i * kCols * HD + lane * kPer;
-            ml[i] = __ldcg(&bml[i * kCols]);
+            const float *src = bo + (int64_t)i * apart * HD + lane * kPer;
+            ml[i] = __ldcg(&bml[i * apart]);
             if constexpr (kPer == 4) {
                 const float4 v = __ldcg(reinterpret_cast<const float4 *>(src));
                 x[i][0] = v.x, x[i][1] = v.y, x[i][2] = v.z, x[i][3] = v.w;
@@ -438,20 +455,20 @@ __device__ __forceinline__ void join_pieces(const DecodeKv4Params &p, int64_t pl
         for (int i = 0; i < kRows; i += 32 / kLanes) {
             const int row = i + lane / kLanes, at = lane % kLanes * 4;
             if (k0 + row < pieces)
-                cp_async16(buf + row * HD + at, bo + (int64_t)(k0 + row) * kCols * HD + at);
+                cp_async16(buf + row * HD + at, bo + (int64_t)(k0 + row) * apart * HD + at);
         }
     };
     read(0);
     float2 ml = make_float2(-INFINITY, 0.f);  // of piece lane, then lane + 32, ..
-    if (lane < pieces) ml = __ldcg(&bml[lane * kCols]);
+    if (lane < pieces) ml = __ldcg(&bml[lane * apart]);
     j.m = ml.x;
-    for (int k = lane + 32; k < pieces; k += 32) j.m = fmaxf(j.m, __ldcg(&bml[k * kCols].x));
+    for (int k = lane + 32; k < pieces; k += 32) j.m = fmaxf(j.m, __ldcg(&bml[k * apart].x));
 #pragma unroll
     for (int d = 16; d; d >>= 1) j.m = fmaxf(j.m, __shfl_xor_sync(0xffffffffu, j.m, d));
     for (int k0 = 0; k0 < pieces; k0 += kRows) {
         if (k0 > 0 && k0 % 32 == 0) {
             ml = make_float2(-INFINITY, 0.f);
-            if (k0 + lane < pieces) ml = __ldcg(&bml[(k0 + lane) * kCols]);
+            if (k0 + lane < pieces) ml = __ldcg(&bml[(k0 + lane) * apart]);
         }
         const float r = ml.x == -INFINITY ? 0.f : ex2(ml.x - j.m);
         const uint32_t seen = __ballot_sync(0xffffffffu, ml.x != -INFINITY);
@@ -472,6 +489,26 @@ __device__ __forceinline__ void join_pieces(const DecodeKv4Params &p, int64_t pl
         __syncwarp();
         if (k0 + kRows < pieces) read(k0 + kRows);
     }
+}
+
+// After the last piece of this warp's column (or of its group): true when j holds all of it.
+template <int HD, int NT>
+__device__ __forceinline__ bool finish_column(const DecodeKv4Params &p, int64_t seg, int c0,
+                                              int pieces, int mine, int c, int lane, float *buf,
+                                              Joined<HD, NT> &j) {
+    if (pieces <= kTreePieces) {
+        join_pieces<HD, NT>(p, seg + c0, pieces, 1, c, lane, buf, j);
+        return true;
+    }
+    const int first = mine / kTreeGroup * kTreeGroup;
+    join_pieces<HD, NT>(p, seg + c0 + first, min(kTreeGroup, pieces - first), 1, c, lane, buf, j);
+    store_piece<HD, NT>(p, seg + c0 + first, c, lane, j);
+    __syncwarp();
+    const int last = lane == 0 && last_piece<Cfg<HD, NT>::kCols>(p, seg, c0, pieces, mine, c, true);
+    if (!__shfl_sync(0xffffffffu, last, 0)) return false;
+    join_pieces<HD, NT>(p, seg + c0, (pieces + kTreeGroup - 1) / kTreeGroup, kTreeGroup, c, lane, buf,
+                        j);
+    return true;
 }
 
 // The pieces of a chunk's segment: the CTA of the first one, and how many.
@@ -745,7 +782,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
                     int c0;
                     const int pieces = pieces_of(p, cut, prev, c0);
                     const bool mine = lane < kCols && lane % kEdges == edge &&
-                                      last_piece<kCols>(p, seg, lane, pieces);
+                                      last_piece<kCols>(p, seg, c0, pieces, cta - c0, lane, false);
                     const uint32_t cols = __ballot_sync(0xffffffffu, mine);
                     if (lane == 0) {
                         if (edge == 0) s_left = prev;
@@ -1051,9 +1088,10 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
             if (!whole) {
                 store_piece<HD, NT>(p, seg + cta, c, lane, j);
                 __syncwarp();
-                const int mine = lane == 0 && last_piece<kCols>(p, seg, c, pieces);
+                const int mine = lane == 0 && last_piece<kCols>(p, seg, c0, pieces, cta - c0, c, false);
                 if (!__shfl_sync(0xffffffffu, mine, 0)) continue;
-                join_pieces<HD, NT>(p, seg + c0, pieces, c, lane, join_buf, j);
+                if (!finish_column<HD, NT>(p, seg, c0, pieces, cta - c0, c, lane, join_buf, j))
+                    continue;
             }
             write_row<HD, NT>(p, ch, c, lane, j);
         }
@@ -1068,9 +1106,9 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
         for (int c = warp; c < kCols; c += kWarps) {
             if (!(left >> c & 1)) continue;
             Joined<HD, NT> j;
-            join_pieces<HD, NT>(p, (int64_t)lc.b * p.seg_per_seq + lc.seg + c0, pieces, c, lane,
-                                join_buf, j);
-            write_row<HD, NT>(p, lc, c, lane, j);
+            if (finish_column<HD, NT>(p, (int64_t)lc.b * p.seg_per_seq + lc.seg, c0, pieces, cta - c0,
+                                      c, lane, join_buf, j))
+                write_row<HD, NT>(p, lc, c, lane, j);
         }
         return;
     }
@@ -1078,10 +1116,10 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
-// counters [segments][cols] int32 | m, l [pieces][cols] | o [pieces][cols][hd], with
-// pieces = segments + CTAs (a piece's place is its segment + its CTA).
+// counters [segments][cols], [pieces][cols] int32 | m, l [pieces][cols] | o [pieces][cols][hd],
+// with pieces = segments + CTAs (a piece's place is its segment + its CTA).
 struct WsLayout {
-    size_t cnt, ml, o;
+    size_t seg, cnt, ml, o;  // cnt: of both, seg: of the segments alone
     size_t total() const { return cnt + ml + o; }
 };
 
@@ -1099,7 +1137,8 @@ WsLayout ws_layout(int64_t batch, int hq, int hkv, int hd, int tokens) {
     const int nc = 8 * tiles(cols);
     const int64_t segs = batch * hkv * ((cols + nc - 1) / nc);
     const int64_t pieces = segs + (int64_t)sm_count() * (nc == 8 ? 2 : 1);
-    return {align256(segs * nc * 4), align256(pieces * nc * 8), (size_t)pieces * nc * hd * 4};
+    return {(size_t)segs * nc * 4, align256((segs + pieces) * nc * 4),
+            align256(pieces * nc * 8), (size_t)pieces * nc * hd * 4};
 }
 
 template <int HD, int NT>
@@ -1213,6 +1252,7 @@ extern "C" int lc_paged_decode_kv4(void *out, int64_t out_stride, const void *q,
     p.v_scale = v_scale;
     uint8_t *ws = (uint8_t *)workspace;
     p.ws_cnt = (int *)ws;
+    p.ws_group = (int *)(ws + wl.seg);
     p.ws_ml = (float2 *)(ws + wl.cnt);
     p.ws_o = (float *)(ws + wl.cnt + wl.ml);
     p.status = dev_status;
