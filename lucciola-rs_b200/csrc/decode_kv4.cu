@@ -13,13 +13,13 @@
 // (arrival counter) joins them in the order of the stream, so the result does
 // not depend on timing.
 //
-// Bounds. 64 sequences of 1024 .. 16384 tokens, 64/8 heads of 128: 125 us, 4.9 TB/s
-// of pages (75 % of a device copy's rate); 32 of 8192, 28/4 heads: 39 us, 3.8 TB/s. A
-// page of 128 dims costs 263 instructions of a warp, about half of them at half
+// Bounds. 64 sequences of 1024 .. 16384 tokens, 64/8 heads of 128: 122 us, 5.0 TB/s
+// of pages (77 % of a device copy's rate); 32 of 8192, 28/4 heads: 37.5 us, 3.9 TB/s. A
+// page of 128 dims costs 300 instructions of a warp, about half of them at half
 // rate, nearly the issue slots of the time that it takes from memory: unpacking
 // binds before the bytes do. Short work is bound by its ends, length -> table ->
-// page before the first product and the join after the last: one sequence of 1024
-// tokens 6.7 us.
+// page before the first product (3.6 us) and the join after the last (2 to 4 us): one
+// sequence of 1024 tokens 6.4 us.
 //
 // Inside a CTA eight warps compute, taking groups of kGroup pages in turn, each
 // from a ring of its own. A loading warp fills the rings, one lane per page of a
@@ -195,9 +195,9 @@ __device__ __forceinline__ int pages_of(int tokens) {
 // Units of one segment in the stream: its pages and, before them, kEdgeUnits
 // without a page, about what a chunk's two ends cost in page times; without them
 // a CTA whose pages lie in many short segments takes longer than the others. (64
-// sequences of 256 .. 4096 tokens, 14/2 heads of 64: 15.0 us with 32 units, 15.7
-// with 24, 19.1 with none; 256 of 100 .. 300: 16.1, 16.1, 20.6; 32 of 8192, 28/4
-// heads of 128: 39.0, 38.9, 40.0, and 40.0 with 36.) A single sequence fills no
+// sequences of 256 .. 4096 tokens, 14/2 heads of 64: 14.6 us with 32 units, 15.1
+// with 24, 18.3 with none; 256 of 100 .. 300: 15.2, 15.3, 19.5; 32 of 8192, 28/4
+// heads of 128: 37.5, 37.4, 38.9, and 38.1 with 36.) A single sequence fills no
 // CTA with several segments and has none.
 __device__ __forceinline__ int edge_units(const DecodeKv4Params &p) {
     return p.batch > 1 ? kEdgeUnits : 0;
@@ -211,9 +211,10 @@ __device__ __forceinline__ int units_of(const DecodeKv4Params &p, int tokens) {
 __device__ __forceinline__ int ctas_of(const DecodeKv4Params &p, int total, int pages) {
     // One sequence: as many CTAs for each segment, so that none of them joins two in
     // turn, and no more than the rounds of groups ask for that the fullest one works
-    // through. (28/4 heads of 128, 12345 tokens: 256 CTAs of 13 pages 18.8 us, 196 of 16
-    // 14.1 us; 32768 tokens: 296 of 28 19.1 us, 256 of 32 17.8 us.) From the fifth round
-    // on a full grid does as well (100000 tokens, 64/8 heads: 34.8 us, 36.0 us in rounds).
+    // through. (28/4 heads of 128, 12345 tokens: 196 CTAs of 16 pages 11.3 us, 296 of 10
+    // or 11 14.3 us; 32768 tokens: 256 of 32 14.3 us, 296 of 28 14.7 us.) From the fifth
+    // round on a full grid does as well or better (100000 tokens, 64/8 heads: 32.4 us, 33.3
+    // us in rounds).
     if (p.batch == 1 && p.seg_ctas > 0) {
         int each = p.seg_ctas;
         for (int r = 1; r <= 4; ++r) {
@@ -376,7 +377,7 @@ __device__ __forceinline__ void store_piece(const DecodeKv4Params &p, int64_t pl
 // more in groups of kTreeGroup, whose results take the place of their first piece and
 // are joined by the group that ends last, so that one CTA does not read them all.
 // Groups and orders are those of the stream. (One sequence of 32768 tokens, 28/4 heads
-// of 128, 64 pieces per column: 14.1 us, 16.8 us joined by one; 12345 tokens, 49: 11.3,
+// of 128, 64 pieces per column: 14.3 us, 16.8 us joined by one; 12345 tokens, 49: 11.3,
 // 13.6.)
 constexpr int kTreePieces = 32, kTreeGroup = 8;
 
@@ -1125,8 +1126,8 @@ struct WsLayout {
 
 // Tiles of 8 columns that a segment takes at once: K and V unpack once for all of
 // them, so as few slices as three tiles allow, and then no more tiles than needed.
-// (24 columns, 8 sequences of 1024 .. 32768 tokens of 64/8 heads of 128: 69 us with
-// three tiles, 101 us as two slices of two.)
+// (24 columns, 8 sequences of 1024 .. 32768 tokens of 64/8 heads of 128: 66 us with
+// three tiles, 100 us as two slices of two.)
 int tiles(int64_t cols) {
     if (cols <= 8) return 1;
     return (cols + 23) / 24 < (cols + 15) / 16 ? 3 : 2;
