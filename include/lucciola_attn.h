@@ -418,9 +418,13 @@ int lc_unpack_kv4(void *k_out, void *v_out, const void *kv_pool, int64_t num_blo
                   int len_offset, int batch, int max_context_len, float k_scale,
                   float v_scale, int *dev_status, lc_stream_t stream);
 
-/* Workspace of lc_paged_decode_kv4 on the current device, as
- * lc_paged_decode_workspace_size: zero it once (lc_paged_decode_workspace_init),
- * and again after a status word with LC_DEV_TIMEOUT. */
+/* Workspace of lc_paged_decode_kv4 on the current device: zero it once
+ * (lc_paged_decode_workspace_init), and again after a status word with
+ * LC_DEV_TIMEOUT. Its counters come first, in the same bytes (288 per SM, rounded
+ * up) whatever the call's shape, and are left zero; the rest is left as it is. So
+ * one workspace, as large as the largest call needs, serves calls of any shapes
+ * that are ordered on one stream; lc_paged_decode needs one of its own, all of
+ * whose words it expects to be zero. */
 size_t lc_paged_decode_kv4_workspace_size(int batch, int num_q_heads, int num_kv_heads,
                                           int head_dim, int tokens_per_seq);
 

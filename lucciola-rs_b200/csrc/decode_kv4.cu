@@ -85,8 +85,8 @@ struct DecodeKv4Params {
     float v_scale;
     int pdl_mode;
     int seg_ctas;   // CTAs of the grid per segment, when there is one sequence
-    int *ws_cnt;    // [batch * seg_per_seq][kCols] arrivals
-    int *ws_group;  // [pieces][kCols] arrivals of a group, at its first piece
+    int *ws_cnt;    // [CTAs][kCols] arrivals, at the CTA of a segment's first piece
+    int *ws_group;  // [2][CTAs][kCols] arrivals of a group, at the CTA of its first piece
     float2 *ws_ml;  // [pieces][kCols] m, l
     float *ws_o;    // [pieces][kCols][hd]
     int *status;
@@ -381,17 +381,24 @@ __device__ __forceinline__ void store_piece(const DecodeKv4Params &p, int64_t pl
 // 13.6.)
 constexpr int kTreePieces = 32, kTreeGroup = 8;
 
-// Counts piece `mine` (or, `top`, a joined group) of column c; true for the last one of
-// its group or segment. One lane, after the warp's stores and a __syncwarp.
+// Counts piece `mine` (or, `top`, a joined group) of column c of the segment whose first
+// piece is CTA c0's; true for the last one of its group or segment. One lane, after the
+// warp's stores and a __syncwarp.
+//
+// A counter's place is that of a CTA, not of a segment, so that the counters take the same
+// room in a call of any shape and no call's pieces lie on another's counters. One place
+// per CTA is enough: a CTA holds at most one piece that begins a segment (its last chunk)
+// and one that does not (its first chunk), and so the first piece of at most one group
+// that begins a segment and of one that does not.
 template <int kCols>
-__device__ __forceinline__ bool last_piece(const DecodeKv4Params &p, int64_t seg, int c0, int pieces,
-                                           int mine, int c, bool top) {
-    int *cnt = p.ws_cnt + seg * kCols + c;
+__device__ __forceinline__ bool last_piece(const DecodeKv4Params &p, int c0, int pieces, int mine,
+                                           int c, bool top) {
+    int *cnt = p.ws_cnt + c0 * kCols + c;
     int count = pieces;
     if (pieces > kTreePieces) {
         const int first = mine / kTreeGroup * kTreeGroup;
         count = top ? (pieces + kTreeGroup - 1) / kTreeGroup : min(kTreeGroup, pieces - first);
-        if (!top) cnt = p.ws_group + (seg + c0 + first) * kCols + c;
+        if (!top) cnt = p.ws_group + ((first ? 0 : (int)gridDim.x) + c0 + first) * kCols + c;
     }
     if (atom_add_acq_rel_gpu(cnt, 1) != count - 1) return false;
     *cnt = 0;  // ready for the next call
@@ -505,7 +512,7 @@ __device__ __forceinline__ bool finish_column(const DecodeKv4Params &p, int64_t 
     join_pieces<HD, NT>(p, seg + c0 + first, min(kTreeGroup, pieces - first), 1, c, lane, buf, j);
     store_piece<HD, NT>(p, seg + c0 + first, c, lane, j);
     __syncwarp();
-    const int last = lane == 0 && last_piece<Cfg<HD, NT>::kCols>(p, seg, c0, pieces, mine, c, true);
+    const int last = lane == 0 && last_piece<Cfg<HD, NT>::kCols>(p, c0, pieces, mine, c, true);
     if (!__shfl_sync(0xffffffffu, last, 0)) return false;
     join_pieces<HD, NT>(p, seg + c0, (pieces + kTreeGroup - 1) / kTreeGroup, kTreeGroup, c, lane, buf,
                         j);
@@ -783,7 +790,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
                     int c0;
                     const int pieces = pieces_of(p, cut, prev, c0);
                     const bool mine = lane < kCols && lane % kEdges == edge &&
-                                      last_piece<kCols>(p, seg, c0, pieces, cta - c0, lane, false);
+                                      last_piece<kCols>(p, c0, pieces, cta - c0, lane, false);
                     const uint32_t cols = __ballot_sync(0xffffffffu, mine);
                     if (lane == 0) {
                         if (edge == 0) s_left = prev;
@@ -1089,7 +1096,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
             if (!whole) {
                 store_piece<HD, NT>(p, seg + cta, c, lane, j);
                 __syncwarp();
-                const int mine = lane == 0 && last_piece<kCols>(p, seg, c0, pieces, cta - c0, c, false);
+                const int mine = lane == 0 && last_piece<kCols>(p, c0, pieces, cta - c0, c, false);
                 if (!__shfl_sync(0xffffffffu, mine, 0)) continue;
                 if (!finish_column<HD, NT>(p, seg, c0, pieces, cta - c0, c, lane, join_buf, j))
                     continue;
@@ -1117,8 +1124,10 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
-// counters [segments][cols], [pieces][cols] int32 | m, l [pieces][cols] | o [pieces][cols][hd],
-// with pieces = segments + CTAs (a piece's place is its segment + its CTA).
+// Counters of segments, of groups, int32 | m, l [pieces][cols] | o [pieces][cols][hd], with
+// pieces = segments + CTAs (a piece's place is its segment + its CTA). The counters, which
+// a call leaves zero, take the same room whatever the call's shape, that of the most
+// columns; what lies behind them is written before it is read.
 struct WsLayout {
     size_t seg, cnt, ml, o;  // cnt: of both, seg: of the segments alone
     size_t total() const { return cnt + ml + o; }
@@ -1138,8 +1147,9 @@ WsLayout ws_layout(int64_t batch, int hq, int hkv, int hd, int tokens) {
     const int nc = 8 * tiles(cols);
     const int64_t segs = batch * hkv * ((cols + nc - 1) / nc);
     const int64_t pieces = segs + (int64_t)sm_count() * (nc == 8 ? 2 : 1);
-    return {(size_t)segs * nc * 4, align256((segs + pieces) * nc * 4),
-            align256(pieces * nc * 8), (size_t)pieces * nc * hd * 4};
+    constexpr size_t kCounters = std::max({2 * 8, 16, 24});  // per SM: CTAs * columns
+    const size_t seg = align256(sm_count() * kCounters * 4);
+    return {seg, 3 * seg, align256(pieces * nc * 8), (size_t)pieces * nc * hd * 4};
 }
 
 template <int HD, int NT>
