@@ -1068,7 +1068,10 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) l[nt][k] += __shfl_xor_sync(0xffffffffu, l[nt][k], d);
                 const int c = nt * 8 + 2 * t + k;
-                if (g == 0) s_ml[warp][c] = make_float2(m[nt][k], l[nt][k]);
+                // Scores that are all NaN leave m at -inf, which says that the warp saw
+                // nothing of the column; any other m lets their NaN sums through.
+                const float seen = m[nt][k] == -INFINITY && l[nt][k] != 0.f ? 0.f : m[nt][k];
+                if (g == 0) s_ml[warp][c] = make_float2(seen, l[nt][k]);
                 float *dst = states + (warp * kCols + c) * C::kRow + g * (HD / 8);
 #pragma unroll
                 for (int j = 0; j < kSteps; j += 2)
