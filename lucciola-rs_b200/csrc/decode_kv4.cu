@@ -340,8 +340,9 @@ __device__ __forceinline__ void write_row(const DecodeKv4Params &p, const ChunkI
     const int kvh = kv_head(p, ch.seg), col = (ch.seg - kvh * p.slices) * Cfg<HD, NT>::kCols + c;
     if (col >= p.cols) return;
     const int qi = col / p.group, h = col - qi * p.group;
-    // a row without tokens gets zeros
-    const float r = j.l == 0.f ? 0.f : p.v_scale / j.l;
+    // A row without tokens gets zeros; one whose scores are all -inf has l = 0 too, and
+    // its 0 / 0 stays NaN.
+    const float r = ch.n <= p.tokens - 1 - qi ? 0.f : p.v_scale / j.l;
     bf16 *dst = p.out + ((int64_t)ch.b * p.tokens + qi) * p.out_stride +
                 (int64_t)(kvh * p.group + h) * HD + lane * kPer;
     uint32_t v[kPer / 2];

@@ -1,5 +1,5 @@
 """What is not a number stays visible in lc_paged_decode_kv4's rows, also where all
-that one warp, one CTA or the whole row sees is NaN."""
+that one warp, one CTA or the whole row sees is NaN or minus infinity."""
 import numpy as np
 import pytest
 
@@ -76,3 +76,20 @@ def test_nan_keys_leave_rows_alone_that_do_not_see_them(hd):
         nan_key(pool, tables, b, n - 1, 0, hd)
         nan[3 * b + 2, :2] = True
     check(q, pool, tables, lens, hd, 3, nan)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n", [1, 40, 5000])
+def test_scores_of_minus_infinity_only_are_not_an_empty_row(n, hd):
+    """softmax over scores that are all -inf is 0 / 0, as lc_paged_decode has it; a row
+    without tokens is zeros."""
+    rng, lens, tables, pool = make([n, 0], hd, n)
+    k = R.unpack(pool[..., :R.half_bytes(hd)], hd, 1.0)
+    k[..., 5] = -np.abs(k[..., 5]) - 0.5 * np.abs(k).max(-1)
+    pool[..., :R.half_bytes(hd)] = R.pack(k, 1.0)
+    q = randn_bf16(rng, (2, HQ, hd))
+    q[0, 1, 5] = 0x7f80
+    q[1, :, 5] = 0x7f80
+    nan = np.zeros((2, HQ), bool)
+    nan[0, 1] = True
+    check(q, pool, tables, lens, hd, 1, nan)
