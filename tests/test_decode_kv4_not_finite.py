@@ -93,3 +93,11 @@ def test_scores_of_minus_infinity_only_are_not_an_empty_row(n, hd):
     nan = np.zeros((2, HQ), bool)
     nan[0, 1] = True
     check(q, pool, tables, lens, hd, 1, nan)
+
+
+def test_a_scale_that_is_not_a_number():
+    """A NaN factor gives NaN, not the mean of the values; rows without tokens stay zeros."""
+    rng, lens, tables, pool = make([50, 0], 64, 3)
+    q = randn_bf16(rng, (2, HQ, 64))
+    got = run_decode(q, pool, 0, tables, lens, HKV, 64, sm_scale=float("nan"))
+    assert np.isnan(got[0]).all() and not got[1].any()
