@@ -30,6 +30,9 @@ namespace {
 constexpr int kStepThreads = 512;
 constexpr int kStepWarps = kStepThreads / 32;
 constexpr int kStepMaxBatch = 8192;  // four ints of shared memory per request
+// Dynamic shared memory that a launch gets without asking: 48 KB less room for the
+// kernels' static arrays (under 200 bytes), which count against the same limit.
+constexpr int kSmemUnasked = 47 * 1024;
 constexpr int kTokenSegment = 128;   // token rows of a warp's task
 constexpr int kRowTurns = 2;         // 16-byte reads per lane in flight
 constexpr int kRowSegment = 128 * kRowTurns;  // table entries of a warp's task
@@ -404,7 +407,7 @@ extern "C" int lc_step_tables(int *block_tables, int table_stride, int num_slots
     p.ticket = (int *)workspace;
     p.status = dev_status;
     const int smem = (4 * batch + 1) * (int)sizeof(int);
-    if (smem > 48 * 1024) {
+    if (smem > kSmemUnasked) {
         const int rc = ensure_smem_attr((const void *)step_tables_kernel, smem);
         if (rc) return rc;
     }
@@ -439,7 +442,7 @@ extern "C" int lc_step_release(int *free_pages, const int *free_count, int64_t n
     ReleaseParams p{free_pages, free_count, (int)num_blocks, block_tables, table_stride, num_slots,
                     slots, context_lens, count, free_count_out, (int *)workspace, dev_status};
     const int smem = std::max(2 * count * (int)sizeof(int), 4);
-    if (smem > 48 * 1024) {
+    if (smem > kSmemUnasked) {
         const int rc = ensure_smem_attr((const void *)step_release_kernel, smem);
         if (rc) return rc;
     }
