@@ -115,17 +115,22 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 // corrected once by its exact remainder (P. Markstein, "Computation of elementary
 // functions on the IBM RISC System/6000 processor", 1990) gives it in three
 // operations per pair: equal to the divided value for every one of 18 million tried
-// around the boundaries. Groups whose scale is at its limit (quotients beyond 8)
+// around the boundaries. It is -x / step that is computed, and the codes' signs are
+// turned afterwards: a zero x then keeps its sign (the remainder is +0 for both zeros,
+// and +0 times the negative reciprocal added to a zero leaves that as it is), where
+// x / step would make +0 of -0. Groups whose scale is at its limit (quotients beyond 8)
 // take the division.
 __device__ __forceinline__ uint32_t kv4_codes(const uint64_t (&x)[4], float step, uint32_t amax) {
     float y[8];
+    uint32_t signs = 0;
     if (step > 0.f && __uint_as_float(amax) <= 8.f * step) {
         const float r = __frcp_rn(step);
-        const uint64_t rr = pair2(r, r), neg = pair2(-step, -step);
+        const uint64_t rr = pair2(-r, -r), ss = pair2(step, step);
+        signs = 0x88888888u;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint64_t q = mul2(x[i], rr);
-            const float2 v = split2(fma2(fma2(q, neg, x[i]), rr, q));
+            const uint64_t q = mul2(x[i], rr);  // -x / step, nearly; x + q step is what is left
+            const float2 v = split2(fma2(fma2(q, ss, x[i]), rr, q));
             y[2 * i] = v.x, y[2 * i + 1] = v.y;
         }
     } else {
@@ -145,7 +150,7 @@ __device__ __forceinline__ uint32_t kv4_codes(const uint64_t (&x)[4], float step
         "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
         : "=r"(w)
         : "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7]));
-    return w;
+    return w ^ signs;
 }
 
 }  // namespace lc
