@@ -515,6 +515,7 @@ __device__ __forceinline__ bool finish_column(const DecodeKv4Params &p, int64_t 
     __syncwarp();
     const int last = lane == 0 && last_piece<Cfg<HD, NT>::kCols>(p, c0, pieces, mine, c, true);
     if (!__shfl_sync(0xffffffffu, last, 0)) return false;
+    __syncwarp();  // lane 0's count saw the groups; now the other lanes' reads do
     join_pieces<HD, NT>(p, seg + c0, (pieces + kTreeGroup - 1) / kTreeGroup, kTreeGroup, c, lane, buf,
                         j);
     return true;
@@ -1103,6 +1104,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
                 __syncwarp();
                 const int mine = lane == 0 && last_piece<kCols>(p, c0, pieces, cta - c0, c, false);
                 if (!__shfl_sync(0xffffffffu, mine, 0)) continue;
+                __syncwarp();  // lane 0's count saw the pieces; now the other lanes' reads do
                 if (!finish_column<HD, NT>(p, seg, c0, pieces, cta - c0, c, lane, join_buf, j))
                     continue;
             }
