@@ -37,8 +37,9 @@
 //     O^T[hd x 8 columns]       += V^T[hd x 16] . P^T
 // K and V unpack in registers, straight into the operand layout: e2m1 to fp16
 // is one conversion per pair, the scale one multiplication per pair, both exact
-// (kv4.cuh), so only p is rounded (to fp16, 2^-11) on its way into a product. q
-// is scaled to [1, 2) by a power of two per row, so that bf16 fits fp16.
+// (kv4.cuh). q is scaled by a power of two per row, its largest element to [2^14, 2^15),
+// so that fp16 holds all of its bits down to 2^-31 of that one: only p is rounded (to
+// fp16, 2^-11) on its way into a product.
 //  * K: a lane's operand elements are 4 dims per step of 2 tokens. The order of
 //    dims within the sum is free, so lane t of a quad takes the dims hd/4 * t ..
 //    and reads them as one 16-byte (8 at hd 64) load per token.
@@ -63,6 +64,7 @@ constexpr int kGroup = 2;             // pages of one warp at a time
 constexpr int kMinPages = 16;         // pages per CTA at least: a group for each of its warps
 constexpr int kEdgeUnits = 32;        // see edge_units
 constexpr float kLazy = 8.f;  // p may reach 2^8 before O and l are rescaled
+constexpr int kQTop = 14;  // exponent of a row's largest element of q
 
 struct DecodeKv4Params {
     bf16 *out;
@@ -749,7 +751,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
             // 2^-e and 2^e, kept within the normal numbers
-            const int e = min(max((int)(top >> 7) - 127, -126), 126);
+            const int e = max((int)(top >> 7) - 127 - kQTop, -126);
             const float down = __int_as_float((127 - e) << 23);
             // Never zero, so that a masked score stays -inf; a NaN scale stays NaN.
             if (t == 0) {
