@@ -435,7 +435,8 @@ size_t lc_paged_decode_kv4_workspace_size(int batch, int num_q_heads, int num_kv
  * n_b = context_lens[b] + len_offset, all of them in the cache. A row without
  * tokens gets zeros; one whose scores are NaN, or all -inf, gets NaN. K and V
  * enter the products exactly as stored, q too down to 2^-31 of its row's largest
- * element, the probabilities as fp16, sums are fp32. max_context_len (0: unknown) trims the grid for little work. Table
+ * element, the probabilities as fp16 (11 bits down to 2^-21 of the largest); sums
+ * are fp32. max_context_len (0: unknown) trims the grid for little work. Table
  * entries outside the pool (LC_DEV_BAD_BLOCK) read as zeros. */
 int lc_paged_decode_kv4(void *out, int64_t out_stride, const void *q, int64_t q_stride,
                         const void *kv_pool, int64_t num_blocks, int num_layers, int layer,

@@ -39,7 +39,8 @@
 // is one conversion per pair, the scale one multiplication per pair, both exact
 // (kv4.cuh). q is scaled by a power of two per row, its largest element to [2^14, 2^15),
 // so that fp16 holds all of its bits down to 2^-31 of that one: only p is rounded (to
-// fp16, 2^-11) on its way into a product.
+// fp16, 2^-11) on its way into a product, and its powers too are laid towards fp16's
+// upper end (kLift).
 //  * K: a lane's operand elements are 4 dims per step of 2 tokens. The order of
 //    dims within the sum is free, so lane t of a quad takes the dims hd/4 * t ..
 //    and reads them as one 16-byte (8 at hd 64) load per token.
@@ -63,7 +64,10 @@ namespace {
 constexpr int kGroup = 2;             // pages of one warp at a time
 constexpr int kMinPages = 16;         // pages per CTA at least: a group for each of its warps
 constexpr int kEdgeUnits = 32;        // see edge_units
-constexpr float kLazy = 8.f;  // p may reach 2^8 before O and l are rescaled
+// p is 2^(s - m) with m kLift below the largest score when it is set, and may grow by
+// 2^kLazy before O and l are rescaled: up to 2^15, so that fp16 keeps 11 bits of p down to
+// 2^-21 of the largest, and its last one down to 2^-31.
+constexpr float kLift = 7.f, kLazy = 8.f;
 constexpr int kQTop = 14;  // exponent of a row's largest element of q
 
 struct DecodeKv4Params {
@@ -927,7 +931,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
                                 s[pg][nt][k] = -INFINITY;
             }
 
-            // running maximum: raised only where some p would pass 2^kLazy
+            // running maximum less kLift: raised only where some p would pass 2^15
             bool raise = false;
             float top[NT][2];
 #pragma unroll
@@ -939,7 +943,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
                     for (int pg = 1; pg < kGroup; ++pg)
                         x = fmaxf(x, fmaxf(s[pg][nt][k], s[pg][nt][k + 2]));
                     top[nt][k] = x * f[nt][k];
-                    raise |= top[nt][k] > m[nt][k] + kLazy;
+                    raise |= top[nt][k] > m[nt][k] + (kLift + kLazy);
                 }
             if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
@@ -950,7 +954,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1)
                             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-                        x = fmaxf(x, m[nt][k]);
+                        x = fmaxf(x - kLift, m[nt][k]);
                         const float r = m[nt][k] == -INFINITY ? 0.f : ex2(m[nt][k] - x);
                         m[nt][k] = x;
                         off[nt][k] = x == -INFINITY ? 0.f : x;

@@ -1,5 +1,5 @@
-"""lc_paged_decode_kv4 over rows of q of a wide range: they go through fp16, whose ends
-must not show."""
+"""lc_paged_decode_kv4 over rows of q and over probabilities of a wide range: both go
+through fp16, whose ends must not show."""
 import numpy as np
 import pytest
 
@@ -51,3 +51,26 @@ def test_q_of_any_exponent(exponent):
     got = run_decode(q, pool, 0, tables, lens, hkv, hd, sm_scale=sm_scale)
     want, bound = R.decode(R.bf16_f64(q), pool, 0, tables, lens, hkv, hd, 1, 1.0, 1.0, sm_scale)
     assert R.rounds_to(got, want, bound).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("bits", [0.3, 9.7, 14.4, 16.6, 18.3, 19.7, 20.7])
+def test_small_probabilities_beside_a_large_one(bits, hd):
+    """31 tokens 2^-bits as probable as the first, whose value is zero: the row is what
+    these bring. fp16 keeps 11 bits of them (2^-12 after rounding to nearest); fp32 scores
+    of 20 and their ex2 add under 2^-17, the quotient and the sums under 2^-20."""
+    n, rng = 32, np.random.default_rng(1)
+    tables, nb = make_tables(np.array([2]), rng)
+    k = np.zeros((nb, 1, 1, 16, hd))
+    k[tables[0, 0], 0, 0, 0, :] = 6.0
+    v = np.full(k.shape, 6.0)
+    v[tables[0, 0], 0, 0, 0, :] = 0.0
+    pool = np.concatenate([R.pack(k, 1.0), R.pack(v, 1.0)], -1)
+    q = np.zeros((1, 1, hd), np.float32)
+    q[0, 0, 5] = 1.0
+    sm_scale = bits * np.log(2.0) / 6.0
+    got = run_decode(O.f32_to_bf16(q), pool, 0, tables, np.array([n], np.int32), 1, hd,
+                     sm_scale=sm_scale)
+    want = 31 * 6.0 * 2.0 ** -bits / (1 + 31 * 2.0 ** -bits)
+    slack = want * (2.0 ** -12 + 2.0 ** -16)
+    assert R.rounds_to(got, np.full(got.shape, want), slack).all(), (got[0, 0, 0], want)
