@@ -408,7 +408,8 @@ int lc_qk_norm_rope_append_kv4(void *q_out, int64_t q_out_stride, const void *qk
  * j of sequence b becomes page b * P + j, P = ceil(max_context_len / 16), of
  * k_out and v_out (bf16 [batch * P][1][num_kv_heads][16][head_dim]). Tokens past
  * the sequence's n_b = context_lens[b] + len_offset in its last page are zeros;
- * pages past it are left alone. lc_paged_prefill over these pools (num_layers
+ * pages past it are left alone; tokens past P pages are left out
+ * (LC_DEV_BAD_POS). lc_paged_prefill over these pools (num_layers
  * 1, layer 0, table row b = b * P, b * P + 1, ...) is the attention of a prompt
  * that continues a cached context. Table entries outside the pool give zeros
  * (LC_DEV_BAD_BLOCK). max_context_len must not exceed a table row. */

@@ -40,9 +40,9 @@ __global__ void __launch_bounds__(kUnpackThreads) unpack_kv4_kernel(UnpackParams
     t /= p.num_kv_heads;
     const int page = (int)(t % p.pages), b = (int)(t / p.pages);
     int64_t n = (int64_t)__ldg(p.ctx_lens + b) + p.len_offset;
-    if (n > (int64_t)p.table_stride * kBlockSize) {
+    if (n > (int64_t)p.pages * kBlockSize) {  // more than the output takes; a table row is no shorter
         if (page == 0 && head == 0 && !is_v && lane == 0) set_status(p.status, LC_DEV_BAD_POS);
-        n = (int64_t)p.table_stride * kBlockSize;
+        n = (int64_t)p.pages * kBlockSize;
     }
     const int64_t held = n - (int64_t)page * kBlockSize;  // tokens of this page
     if (held <= 0) return;
