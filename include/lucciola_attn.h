@@ -364,7 +364,8 @@ int lc_step_release(int *free_pages, const int *free_count, int64_t num_blocks,
  * apart; it may be the qkv rows themselves), k and v + bias to the pools at
  * slot_map[r] = page * 16 + offset. Each bias and each norm weight may be NULL
  * (none). slot_map[r] = -1: the row's k and v are not stored. positions[r] =
- * -1: a padding row, nothing is read or written for it. A position outside the
+ * -1: a padding row, whose qkv may hold anything (all num_rows rows are memory
+ * that can be read) and for which nothing is written. A position outside the
  * tables (LC_DEV_BAD_POS) leaves the row alone, a slot outside the pool
  * (LC_DEV_BAD_BLOCK) its k and v. Rows may come from any mix of sequences, in
  * any order. All pointers 16-byte aligned, strides multiples of 8. */

@@ -153,7 +153,8 @@ __global__ void __launch_bounds__(kNormRopeThreads, kNormRopeCtas)
         k.a = k.b = make_uint4(0, 0, 0, 0);
         k.pos = k.slot = -1;
         if (k.row >= p.rows) return;
-        // plain loads: q_out may be these rows
+        // Padding rows too are loaded: waiting for the position first costs 0.2 us of a decode
+        // step's 2.4 and 0.5 to 1.1 us of prompts. Plain loads: q_out may be these rows.
         const bf16 *src = p.qkv + (int64_t)k.row * p.row_stride + (int64_t)k.h * HD + c8;
         k.a = *reinterpret_cast<const uint4 *>(src);
         k.b = *reinterpret_cast<const uint4 *>(src + kHalf);
