@@ -347,8 +347,9 @@ __device__ __forceinline__ void write_row(const DecodeKv4Params &p, const ChunkI
     if (col >= p.cols) return;
     const int qi = col / p.group, h = col - qi * p.group;
     // A row without tokens gets zeros; one whose scores are all -inf has l = 0 too, and
-    // its 0 / 0 stays NaN.
-    const float r = ch.n <= p.tokens - 1 - qi ? 0.f : p.v_scale / j.l;
+    // its 0 / 0 stays NaN. (Asking for the length alone costs the products 1.5 %: ptxas
+    // spills other registers then.)
+    const float r = j.l == 0.f && ch.n <= p.tokens - 1 - qi ? 0.f : p.v_scale / j.l;
     bf16 *dst = p.out + ((int64_t)ch.b * p.tokens + qi) * p.out_stride +
                 (int64_t)(kvh * p.group + h) * HD + lane * kPer;
     uint32_t v[kPer / 2];
