@@ -14,12 +14,16 @@
 // not depend on timing.
 //
 // Bounds. 64 sequences of 1024 .. 16384 tokens, 64/8 heads of 128: 122 us, 5.0 TB/s
-// of pages (77 % of a device copy's rate); 32 of 8192, 28/4 heads: 37.5 us, 3.9 TB/s. A
-// page of 128 dims costs 300 instructions of a warp, about half of them at half
-// rate, nearly the issue slots of the time that it takes from memory: unpacking
-// binds before the bytes do. Short work is bound by its ends, length -> table ->
-// page before the first product (3.6 us) and the join after the last (2 to 4 us): one
-// sequence of 1024 tokens 6.4 us.
+// of pages (77 % of a device copy's rate); 32 of 8192, 28/4 heads: 37.5 us, 3.9 TB/s.
+// There a page of 128 dims costs 309 instructions of a warp (8 columns): 54 % of the issue
+// slots, the ALU pipe 47 %, the tensor pipe 22 %, its ends included. About 8 of the 37.5 us
+// are ends; between them the pages come at 78 % of the copy's rate and two thirds of the
+// issue slots are taken, so that no one unit binds, the warps' own chain (load, convert,
+// multiply, product) with four of them per scheduler does. With 24 columns a page costs
+// 390 instructions, 45 % of the issue slots and 44 % of the tensor pipe, with two warps
+// per scheduler. Short work is bound by its ends, length -> table -> page before the
+// first product (3.6 us) and the join after the last (2 to 4 us): one sequence of 1024
+// tokens 6.7 us.
 //
 // Inside a CTA eight warps compute, taking groups of kGroup pages in turn, each
 // from a ring of its own. A loading warp fills the rings, one lane per page of a
