@@ -761,12 +761,12 @@ __global__ void __launch_bounds__(Cfg<HD, NT>::kThreads, Cfg<HD, NT>::kCtasPerSm
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
             // 2^-e and 2^e, kept within the normal numbers
             const int e = max((int)(top >> 7) - 127 - kQTop, -126);
-            const float down = __int_as_float((127 - e) << 23);
-            // Never zero, so that a masked score stays -inf; a NaN scale stays NaN.
-            if (t == 0) {
-                const float f = p.scale_log2 * __int_as_float((127 + e) << 23);
-                s_f[buf][edge * 8 + g] = f < FLT_MIN ? FLT_MIN : f;
-            }
+            // A NaN scale goes into q, so that the masked scores, which it must not reach, stay
+            // -inf; for their sake the factor is never zero either.
+            const float down = p.scale_log2 == p.scale_log2 ? __int_as_float((127 - e) << 23) : NAN;
+            if (t == 0)
+                s_f[buf][edge * 8 + g] =
+                    fmaxf(p.scale_log2 * __int_as_float((127 + e) << 23), FLT_MIN);
             uint2 *dst = reinterpret_cast<uint2 *>(q_ops + buf * C::kQ) + edge * kSteps * 32 + lane;
 #pragma unroll
             for (int k = 0; k < HD / 16; ++k) {

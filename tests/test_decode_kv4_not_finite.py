@@ -101,3 +101,7 @@ def test_a_scale_that_is_not_a_number():
     q = randn_bf16(rng, (2, HQ, 64))
     got = run_decode(q, pool, 0, tables, lens, HKV, 64, sm_scale=float("nan"))
     assert np.isnan(got[0]).all() and not got[1].any()
+    rng, lens, tables, pool = make([50, 1], 64, 4)
+    q = randn_bf16(rng, (6, HQ, 64))
+    got = run_decode(q, pool, 0, tables, lens, HKV, 64, 3, sm_scale=float("nan"))
+    assert np.isnan(got[[0, 1, 2, 5]]).all() and not got[3:5].any()
