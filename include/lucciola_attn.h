@@ -449,6 +449,64 @@ int lc_paged_decode_kv4(void *out, int64_t out_stride, const void *q, int64_t q_
                         size_t workspace_bytes, int *dev_status, lc_stream_t stream);
 
 /* ------------------------------------------------------------------------- */
+/* The cache in 8 bits.                                                       */
+/* ------------------------------------------------------------------------- */
+/* kv_pool: uint8 [num_blocks][num_layers][num_kv_heads][lc_kv8_page_bytes], 16-byte
+ * aligned: per page and kv head the K codes [16][head_dim] (e4m3), the V codes likewise,
+ * K's scale and V's (fp32), 8 unused bytes; 8.06 bits per element (8.125 for heads of
+ * 64), half of the bf16 pools. An element stands for code * scale, with one scale for
+ * the page's 16 tokens, a power of two from 2^-40 to 2^40. Dims 16 c .. 16 c + 15 of
+ * token t are bytes 16 c' .. 16 c' + 15 of its row, c' = c ^ ((t * head_dim / 64) &
+ * (head_dim / 16 - 2)). */
+size_t lc_kv8_page_bytes(int head_dim); /* 32 * head_dim + 16; 0 if unsupported */
+
+/* lc_qk_norm_rope_append into an 8-bit pool. The rows that a call adds to a page are
+ * adjacent and in rising order (as lc_step_tables lays them), and no page gets rows from
+ * two places of the call or from two calls at once. They are held at the smallest scale
+ * 2^e with 448 * 2^e at least their largest magnitude, K and V of each head by
+ * themselves; where the page holds tokens already, at the larger of that and its own, and
+ * if its own was smaller, the other tokens' codes are rounded again to the larger. A row
+ * at token 0 of a page begins it anew: what the page held no longer counts. Codes are to
+ * nearest even from the fp32 values; an infinity or NaN becomes NaN and does not count for
+ * the scale; magnitudes above 448 * 2^40 become that. A row whose slot does not rise
+ * within its page is left out (its k and v, and those of the page's rows after it) and
+ * reported (LC_DEV_BAD_BLOCK). */
+int lc_qk_norm_rope_append_kv8(void *q_out, int64_t q_out_stride, const void *qkv,
+                               int64_t row_stride, int num_rows, const int *positions,
+                               const int *slot_map, const void *q_bias, const void *k_bias,
+                               const void *v_bias, const void *q_norm, const void *k_norm,
+                               float eps, const float *cos_cache, const float *sin_cache,
+                               int rope_rows, void *kv_pool, int64_t num_blocks, int num_layers,
+                               int layer, int num_q_heads, int num_kv_heads, int head_dim,
+                               int *dev_status, lc_stream_t stream);
+
+/* lc_unpack_kv4 for an 8-bit pool; the unpacked bf16 values are exact. */
+int lc_unpack_kv8(void *k_out, void *v_out, const void *kv_pool, int64_t num_blocks,
+                  int num_layers, int layer, int num_kv_heads, int head_dim,
+                  const int *block_tables, int table_stride, const int *context_lens,
+                  int len_offset, int batch, int max_context_len, int *dev_status,
+                  lc_stream_t stream);
+
+/* Workspace of lc_paged_decode_kv8 on the current device, as that of lc_paged_decode_kv4:
+ * zeroed once, and again after LC_DEV_TIMEOUT; one of the largest call's size serves calls of
+ * any shapes that are ordered on one stream. */
+size_t lc_paged_decode_kv8_workspace_size(int batch, int num_q_heads, int num_kv_heads,
+                                          int head_dim, int tokens_per_seq);
+
+/* lc_paged_decode_kv4 over an 8-bit pool: the same rows, lengths, limits and results for
+ * rows without tokens, NaN scores and table entries outside the pool. K and V enter the
+ * products exactly as stored, q too down to 2^-31 of its row's largest element, the
+ * probabilities as fp16 (11 bits down to 2^-21 of the largest product of a probability and
+ * its page's V scale); sums are fp32. */
+int lc_paged_decode_kv8(void *out, int64_t out_stride, const void *q, int64_t q_stride,
+                        const void *kv_pool, int64_t num_blocks, int num_layers, int layer,
+                        int num_q_heads, int num_kv_heads, int head_dim,
+                        const int *block_tables, int table_stride, const int *context_lens,
+                        int len_offset, int batch, int tokens_per_seq, int max_context_len,
+                        float sm_scale, void *workspace, size_t workspace_bytes,
+                        int *dev_status, lc_stream_t stream);
+
+/* ------------------------------------------------------------------------- */
 /* Host-side mirror of the reference's Rust layer API (owning objects).       */
 /* ------------------------------------------------------------------------- */
 
@@ -559,6 +617,23 @@ size_t lc_sample_workspace_size(int batch, int top_k);
 int lc_sample_top_p(const void *logits, int64_t row_stride, int vocab, int batch, int top_k,
                     const float *top_p, const float *rand_vals, unsigned *out_idx,
                     void *workspace, size_t workspace_bytes, lc_stream_t stream);
+
+/* Sampling with every row's own parameters (device arrays of `batch`; NULL: temperature 1
+ * and no filter). Row b's tokens are ordered by logit (larger first), then index; weights
+ * are w = exp((x - max) / temperature) of the logits above -1e30, the others (and NaN) are
+ * never chosen. Kept are the first top_k[b] tokens (all where it is not positive), of
+ * these the shortest prefix whose weight reaches top_p[b] of theirs (one token at least;
+ * all for 1 and above, or NaN), of these the ones with w >= min_p[b] (the first token at
+ * least; all for 0 and below, or NaN). out_idx[b] is the first at which the kept tokens'
+ * running weight exceeds rand_vals[b] (in [0, 1)) times their whole weight. A temperature
+ * that is not positive takes the first token of the order. 0xffffffff where no logit
+ * exceeds -1e30. Weights and sums are in 64 bits: the choice does not depend on the
+ * batch, and equals the formula's but where rand times the weight lies within 1e-12 of a
+ * border. bf16 rows, any stride and alignment. One launch, no workspace. */
+int lc_sample(const void *logits, int64_t row_stride, int vocab, int batch,
+              const float *temperature, const int *top_k, const float *top_p,
+              const float *min_p, const float *rand_vals, unsigned *out_idx,
+              lc_stream_t stream);
 
 /* ------------------------------------------------------------------------- */
 /* Batched token-step driver: many sequences in one paged pool.               */

@@ -1,6 +1,7 @@
 // norm_rope.cu - per-head RMS norm of queries and keys, rotate-half RoPE and the
 // append of K and V, one pass over the qkv rows. K and V go to the bf16 pools
-// (lc_qk_norm_rope_append) or to the 4-bit pool (lc_qk_norm_rope_append_kv4).
+// (lc_qk_norm_rope_append), to the 4-bit pool (lc_qk_norm_rope_append_kv4) or to the
+// 8-bit pool (lc_qk_norm_rope_append_kv8, a kernel of its own further down).
 //
 // For a head x of a row at position pos, with bias b and norm weight w (each
 // optional), c = cos[pos], s = sin[pos]:
@@ -35,6 +36,7 @@
 #include <climits>
 
 #include "kv4.cuh"
+#include "kv8.cuh"
 #include "lc_host.h"
 
 namespace lc {
@@ -57,7 +59,7 @@ struct NormRopeParams {
     const float *cos_t, *sin_t;
     int rope_rows;
     bf16 *k_pool, *v_pool;  // bf16 pools
-    uint8_t *kv_pool;       // 4-bit pool
+    uint8_t *kv_pool;       // 4-bit or 8-bit pool
     float k_scale, v_scale;
     int64_t num_blocks;
     int num_layers, layer, num_q_heads, num_kv_heads;
@@ -272,7 +274,262 @@ int launch(const NormRopeParams &p, int head_dim, cudaStream_t stream) {
     return head_dim == 64 ? launch_dim<64, KV4>(p, stream) : launch_dim<128, KV4>(p, stream);
 }
 
-// The checks both entries share; fills everything but the pools.
+// ---------------------------------------------------------------- 8-bit pool --
+// A page of a kv head has one scale for its 16 tokens, so the rows that a call adds to a
+// page are one piece of work: a run, adjacent rows of one page with rising offsets. The
+// warp that has the run takes K or V of one head: the rows' values stay in its registers,
+// their largest magnitude and the page's old scale give the new one, and where that grew
+// the page's other tokens are moved to it. Run starts are found from the slots: a warp
+// looks at `window` rows and works on the runs that start there.
+//
+// The first kv_blocks CTAs do so, the others the queries, as above.
+constexpr int kMaxWindow = 8;  // a run's 16 rows from the last of 8 end within a warp's lanes
+
+template <int HD>
+__device__ __forceinline__ void add_bias(const bf16 *bias, uint64_t (&x1)[4], uint64_t (&x2)[4]) {
+    uint64_t t1[4], t2[4];
+    unpack8(ldg16(bias), t1);
+    unpack8(ldg16(bias + HD / 2), t2);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        x1[e] = add2(x1[e], t1[e]);
+        x2[e] = add2(x2[e], t2[e]);
+    }
+}
+
+// Norm (w: this lane's weights, or none) and rotation of a head. All lanes of the warp call it.
+template <int HD>
+__device__ __forceinline__ void norm_rotate(const bf16 *w, float eps, uint64_t one,
+                                            uint64_t minus_one, const uint64_t (&cs)[4],
+                                            const uint64_t (&sn)[4], uint64_t (&x1)[4],
+                                            uint64_t (&x2)[4]) {
+    if (w) {
+        const float r = rms_factor<HD>(x1, x2, eps, one);
+        const uint64_t rr = pair2(r, r);
+        uint64_t t1[4], t2[4];
+        unpack8(ldg16(w), t1);
+        unpack8(ldg16(w + HD / 2), t2);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x1[e] = mul2(mul2(x1[e], rr), t1[e]);
+            x2[e] = mul2(mul2(x2[e], rr), t2[e]);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint64_t y1 = x1[e], y2 = x2[e];
+        x1[e] = fma2(mul2(y2, sn[e]), minus_one, mul2(y1, cs[e]));
+        x2[e] = fma2(mul2(y1, sn[e]), one, mul2(y2, cs[e]));
+    }
+}
+
+// Largest finite magnitude of eight values as float bits; `odd`: some are not finite.
+__device__ __forceinline__ uint32_t finite_amax(const uint64_t (&x)[4], bool &odd) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float2 v = split2(x[e]);
+        const uint32_t a = __float_as_uint(v.x) & 0x7fffffffu, b = __float_as_uint(v.y) & 0x7fffffffu;
+        if (a >= 0x7f800000u || b >= 0x7f800000u) odd = true;
+        m = max(m, max(a < 0x7f800000u ? a : 0u, b < 0x7f800000u ? b : 0u));
+    }
+    return m;
+}
+
+// Codes of eight values at the scale 1 / `inv`, a power of two; what is not finite is NaN.
+__device__ __forceinline__ uint2 kv8_codes(const uint64_t (&x)[4], float inv, bool odd) {
+    float y[8];
+    const uint64_t ii = pair2(inv, inv);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float2 v = split2(mul2(x[e], ii));
+        y[2 * e] = v.x, y[2 * e + 1] = v.y;
+    }
+    uint2 c = make_uint2(kv8_codes4(y[0], y[1], y[2], y[3]), kv8_codes4(y[4], y[5], y[6], y[7]));
+    if (odd) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (!(fabsf(y[e]) <= FLT_MAX)) (e < 4 ? c.x : c.y) |= kKv8Nan << e % 4 * 8;
+    }
+    return c;
+}
+
+// The rows [r0, r0 + n) of one page, K or V (is_v) of head hl. Lane i of `pos` and `slot`
+// holds row r0 - first + i's; all of the run's are valid.
+template <int HD>
+__device__ __forceinline__ void append_run(const NormRopeParams &p, int r0, int first, int n,
+                                           int pos, int slot, bool is_v, int hl) {
+    constexpr int kLanes = HD / 16, kHeads = 32 / kLanes, kHalf = HD / 2;
+    constexpr int kChunks = kBlockSize / kHeads;  // rows at a time: kHeads
+    const int lane = threadIdx.x & 31, c8 = lane % kLanes * 8, grp = lane / kLanes;
+    const uint64_t one = pair2(p.one, p.one), minus_one = pair2(-p.one, -p.one);
+    const int phys = __shfl_sync(0xffffffffu, slot, first) / kBlockSize;
+    uint8_t *page = p.kv_pool + kv8_offset(phys, p.layer, hl, p.num_layers, p.num_kv_heads, HD);
+    uint32_t *scale = reinterpret_cast<uint32_t *>(page + 2 * kv8_half_bytes(HD)) + is_v;
+    const bool fresh = __shfl_sync(0xffffffffu, slot, first) % kBlockSize == 0;
+    const uint32_t old = fresh ? 0u : *scale;
+    page += is_v * kv8_half_bytes(HD);
+    const int col = p.num_q_heads + (is_v ? p.num_kv_heads : 0) + hl;  // head within the row
+    uint64_t x1[kChunks][4], x2[kChunks][4];
+    int off[kChunks];
+    uint4 raw[kChunks][2];
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+        raw[c][0] = raw[c][1] = make_uint4(0, 0, 0, 0);
+        const int i = c * kHeads + grp;
+        if (i < n) {
+            const bf16 *src = p.qkv + (int64_t)(r0 + i) * p.row_stride + (int64_t)col * HD + c8;
+            raw[c][0] = *reinterpret_cast<const uint4 *>(src);
+            raw[c][1] = *reinterpret_cast<const uint4 *>(src + kHalf);
+        }
+    }
+    const bf16 *bias = is_v ? p.v_bias : p.k_bias;
+    bool odd = false;
+    uint32_t amax = 0, mine = 0;  // mine: offsets of this lane's rows
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+        const int i = c * kHeads + grp, from = min(first + i, 31);
+        const int row_pos = __shfl_sync(0xffffffffu, pos, from);
+        off[c] = __shfl_sync(0xffffffffu, slot, from) % kBlockSize;
+        unpack8(raw[c][0], x1[c]);
+        unpack8(raw[c][1], x2[c]);
+        if (c * kHeads >= n) continue;  // the whole warp
+        if (bias && i < n) add_bias<HD>(bias + (int64_t)hl * HD + c8, x1[c], x2[c]);
+        if (!is_v) {
+            uint64_t cs[4] = {}, sn[4] = {};
+            if (i < n) {
+                load8f(p.cos_t + (int64_t)row_pos * kHalf + c8, cs);
+                load8f(p.sin_t + (int64_t)row_pos * kHalf + c8, sn);
+            }
+            norm_rotate<HD>(p.k_norm ? p.k_norm + c8 : nullptr, p.eps, one, minus_one, cs, sn, x1[c],
+                            x2[c]);
+        }
+        if (i >= n) continue;
+        amax = max(amax, max(finite_amax(x1[c], odd), finite_amax(x2[c], odd)));
+        mine |= 1u << off[c];
+    }
+    int e = kv8_exponent(__reduce_max_sync(0xffffffffu, amax));
+    const int was = kv8_scale_exp(old);
+    if (!fresh && was >= e) e = was;
+    else if (!fresh) {  // the other tokens move to the larger scale
+        const uint32_t run = __reduce_or_sync(0xffffffffu, mine);
+        const float down = kv8_scale(was - e);
+        for (int v = lane; v < HD; v += 32) {  // 16-byte pieces
+            if (run >> (v / (HD / 16)) & 1) continue;
+            uint4 *at = reinterpret_cast<uint4 *>(page) + v;
+            uint4 w = *at;
+            w.x = kv8_rescale4(w.x, down), w.y = kv8_rescale4(w.y, down);
+            w.z = kv8_rescale4(w.z, down), w.w = kv8_rescale4(w.w, down);
+            *at = w;
+        }
+    }
+    const float inv = kv8_scale(-e);
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+        if (c * kHeads + grp >= n) continue;
+        uint8_t *to = page + off[c] * HD + c8 % 16;
+        *reinterpret_cast<uint2 *>(to + kv8_piece(HD, off[c], c8 / 16) * 16) = kv8_codes(x1[c], inv, odd);
+        *reinterpret_cast<uint2 *>(to + kv8_piece(HD, off[c], (c8 + kHalf) / 16) * 16) =
+            kv8_codes(x2[c], inv, odd);
+    }
+    if (lane == 0) *scale = __float_as_uint(kv8_scale(e));
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kNormRopeThreads)
+    norm_rope_append_kv8_kernel(NormRopeParams p, int window, int kv_blocks) {
+    constexpr int kLanes = HD / 16, kHeads = 32 / kLanes, kHalf = HD / 2;
+    constexpr int kWarps = kNormRopeThreads / 32;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if ((int)blockIdx.x < kv_blocks) {
+        const int kinds = 2 * p.num_kv_heads;
+        const int tasks = (int)(((int64_t)p.rows + window - 1) / window * kinds);
+        for (int task = blockIdx.x * kWarps + warp; task < tasks; task += kv_blocks * kWarps) {
+            const int kind = task % kinds, row0 = task / kinds * window;
+            const int row = row0 - 1 + lane;  // lane 0: the row before the window
+            int pos = -1, slot = -1;
+            if (row >= 0 && row < p.rows) {
+                pos = __ldg(p.positions + row);
+                slot = __ldg(p.slot_map + row);
+            }
+            const bool valid = pos >= 0 && pos < p.rope_rows && slot >= 0 &&
+                               slot < p.num_blocks * kBlockSize;
+            const int page = valid ? slot / kBlockSize : -1;
+            const int prev = __shfl_up_sync(0xffffffffu, page, 1);
+            const int prev_slot = __shfl_up_sync(0xffffffffu, slot, 1);
+            const bool same = lane > 0 && valid && page == prev;
+            const uint32_t sames = __ballot_sync(0xffffffffu, same);
+            const uint32_t rises = __ballot_sync(0xffffffffu, same && slot > prev_slot);
+            uint32_t starts =
+                __ballot_sync(0xffffffffu, valid && !same && lane >= 1 && lane <= window);
+            while (starts) {
+                const int first = __ffs(starts) - 1;
+                starts &= starts - 1;
+                const int n = __ffs(~(rises >> (first + 1)));  // 1 .. 16
+                // a row of the page that does not rise: it and what follows is left out
+                if (kind == 0 && lane == 0 && (sames >> (first + n) & 1))
+                    set_status(p.status, LC_DEV_BAD_BLOCK);
+                append_run<HD>(p, row0 - 1 + first, first, n, pos, slot, kind >= p.num_kv_heads,
+                               kind >= p.num_kv_heads ? kind - p.num_kv_heads : kind);
+            }
+        }
+        return;
+    }
+    // ---- queries
+    const int c8 = (lane % kLanes) * 8, hq = p.num_q_heads;
+    const uint64_t one = pair2(p.one, p.one), minus_one = pair2(-p.one, -p.one);
+    const uint32_t total = (uint32_t)p.rows * hq;
+    const uint32_t step = (gridDim.x - kv_blocks) * kWarps * kHeads;
+    for (uint32_t base = ((blockIdx.x - kv_blocks) * kWarps + warp) * kHeads; base < total; base += step) {
+        const uint32_t item = base + lane / kLanes;
+        const bool in = item < total;
+        const int row = in ? (int)(item / hq) : 0, h = in ? (int)(item - (uint32_t)row * hq) : 0;
+        const int pos = in ? __ldg(p.positions + row) : -1;
+        const bool live = pos >= 0 && pos < p.rope_rows;
+        if (in && h == 0 && c8 == 0) {
+            const int slot = __ldg(p.slot_map + row);
+            if (!live && pos != -1) set_status(p.status, LC_DEV_BAD_POS);
+            if (live && slot != -1 && (slot < 0 || slot >= p.num_blocks * kBlockSize))
+                set_status(p.status, LC_DEV_BAD_BLOCK);
+        }
+        uint64_t x1[4] = {}, x2[4] = {}, cs[4] = {}, sn[4] = {};
+        if (live) {
+            const bf16 *src = p.qkv + (int64_t)row * p.row_stride + (int64_t)h * HD + c8;
+            unpack8(*reinterpret_cast<const uint4 *>(src), x1);
+            unpack8(*reinterpret_cast<const uint4 *>(src + kHalf), x2);
+            load8f(p.cos_t + (int64_t)pos * kHalf + c8, cs);
+            load8f(p.sin_t + (int64_t)pos * kHalf + c8, sn);
+            if (p.q_bias) add_bias<HD>(p.q_bias + (int64_t)h * HD + c8, x1, x2);
+        }
+        norm_rotate<HD>(p.q_norm ? p.q_norm + c8 : nullptr, p.eps, one, minus_one, cs, sn, x1, x2);
+        if (live) {
+            bf16 *dst = p.q_out + (int64_t)row * p.q_out_stride + (int64_t)h * HD + c8;
+            *reinterpret_cast<uint4 *>(dst) = pack8(x1);
+            *reinterpret_cast<uint4 *>(dst + kHalf) = pack8(x2);
+        }
+    }
+}
+
+template <int HD>
+int launch_kv8(const NormRopeParams &p, cudaStream_t stream) {
+    constexpr int kHeads = 32 / (HD / 16), kWarps = kNormRopeThreads / 32, kCtas = 4;
+    const int64_t total = (int64_t)p.rows * (p.num_q_heads + 2 * p.num_kv_heads);
+    if (total > INT_MAX / 2) return LC_ERR_UNSUPPORTED_SHAPE;
+    const int64_t warps = (int64_t)sm_count() * kCtas * kWarps;
+    // decode steps, a run per row: one row per warp while there are warps for them
+    int window = 1;
+    while (window < kMaxWindow && (int64_t)p.rows * 2 * p.num_kv_heads > 4 * warps * window) window *= 2;
+    const int64_t kv_tasks = ((int64_t)p.rows + window - 1) / window * 2 * p.num_kv_heads;
+    const int64_t q_tasks = ((int64_t)p.rows * p.num_q_heads + kHeads - 1) / kHeads;
+    const int64_t most = (int64_t)sm_count() * kCtas;
+    const int64_t kv_blocks = std::min((kv_tasks + kWarps - 1) / kWarps, most);
+    const int64_t q_blocks = std::min((q_tasks + kWarps - 1) / kWarps, most);
+    norm_rope_append_kv8_kernel<HD><<<(unsigned)(kv_blocks + q_blocks), kNormRopeThreads, 0, stream>>>(
+        p, window, (int)kv_blocks);
+    return launch_status();
+}
+
+// The checks the entries share; fills everything but the pools.
 int fill(NormRopeParams &p, void *q_out, int64_t q_out_stride, const void *qkv,
          int64_t row_stride, int num_rows, const int *positions, const int *slot_map,
          const void *q_bias, const void *k_bias, const void *v_bias, const void *q_norm,
@@ -368,4 +625,24 @@ extern "C" int lc_qk_norm_rope_append_kv4(
     p.k_scale = k_scale;
     p.v_scale = v_scale;
     return launch<true>(p, head_dim, as_stream(stream));
+}
+
+extern "C" int lc_qk_norm_rope_append_kv8(
+    void *q_out, int64_t q_out_stride, const void *qkv, int64_t row_stride, int num_rows,
+    const int *positions, const int *slot_map, const void *q_bias, const void *k_bias,
+    const void *v_bias, const void *q_norm, const void *k_norm, float eps,
+    const float *cos_cache, const float *sin_cache, int rope_rows, void *kv_pool,
+    int64_t num_blocks, int num_layers, int layer, int num_q_heads, int num_kv_heads,
+    int head_dim, int *dev_status, lc_stream_t stream) {
+    NormRopeParams p{};
+    if (!kv_pool) return LC_ERR_INVALID_ARGUMENT;
+    const int rc = fill(p, q_out, q_out_stride, qkv, row_stride, num_rows, positions, slot_map,
+                        q_bias, k_bias, v_bias, q_norm, k_norm, eps, cos_cache, sin_cache,
+                        rope_rows, num_blocks, num_layers, layer, num_q_heads, num_kv_heads,
+                        head_dim, dev_status);
+    if (rc) return rc;
+    if (!aligned16(kv_pool)) return LC_ERR_MISALIGNED;
+    if (num_rows == 0) return LC_OK;
+    p.kv_pool = (uint8_t *)kv_pool;
+    return head_dim == 64 ? launch_kv8<64>(p, as_stream(stream)) : launch_kv8<128>(p, as_stream(stream));
 }

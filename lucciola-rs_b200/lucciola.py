@@ -75,6 +75,16 @@ SIGNATURES = {
     "lc_paged_decode_kv4": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _i32, _i32,
                                    _vp, _i32, _vp, _i32, _i32, _i32, _i32, _f32, _f32, _f32, _vp,
                                    _sz, _vp, _vp]),
+    "lc_kv8_page_bytes": (_sz, [_i32]),
+    "lc_qk_norm_rope_append_kv8": (_i32, [_vp, _i64, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp,
+                                          _vp, _vp, _f32, _vp, _vp, _i32, _vp, _i64, _i32, _i32,
+                                          _i32, _i32, _i32, _vp, _vp]),
+    "lc_unpack_kv8": (_i32, [_vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i32, _vp, _i32,
+                             _i32, _i32, _vp, _vp]),
+    "lc_paged_decode_kv8_workspace_size": (_sz, [_i32, _i32, _i32, _i32, _i32]),
+    "lc_paged_decode_kv8": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _i32, _i32,
+                                   _vp, _i32, _vp, _i32, _i32, _i32, _i32, _f32, _vp, _sz, _vp,
+                                   _vp]),
     "lc_rope_table_host": (None, [_i32, _i32, _f32, _f32, _vp, _vp]),
     "lc_rope_cache_new": (_i32, [_i32, _i32, _f32, _f32, _vp, C.POINTER(_vp)]),
     "lc_rope_cache_cos": (_vp, [_vp]),
@@ -98,6 +108,7 @@ SIGNATURES = {
     "lc_argmax": (_i32, [_vp, _i64, _i32, _i32, _vp, _vp]),
     "lc_sample_workspace_size": (_sz, [_i32, _i32]),
     "lc_sample_top_p": (_i32, [_vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "lc_sample": (_i32, [_vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "lc_block_alloc_new": (_i32, [_i64, _i32, _i32, C.POINTER(_vp)]),
     "lc_block_alloc_add_seq": (_i32, [_vp, _pi32]),
     "lc_block_alloc_release_seq": (_i32, [_vp, _i32]),
@@ -465,6 +476,66 @@ def paged_decode_kv4(out, q, kv_pool, num_blocks, num_layers, layer, num_q_heads
                                   _stream(stream)), "lc_paged_decode_kv4")
 
 
+def kv8_page_bytes(head_dim) -> int:
+    return lib.lc_kv8_page_bytes(head_dim)
+
+
+def alloc_kv8_pool(num_blocks, num_layers, num_kv_heads, head_dim, device="cuda"):
+    """Zeroed 8-bit pool: uint8 [num_blocks][num_layers][Hkv][page bytes]."""
+    import torch
+    nbytes = kv8_page_bytes(head_dim)
+    if nbytes == 0:
+        raise LucciolaError(2, "lc_kv8_page_bytes")
+    return torch.zeros(num_blocks, num_layers, num_kv_heads, nbytes, dtype=torch.uint8,
+                       device=device)
+
+
+def qk_norm_rope_append_kv8(q_out, qkv, positions, slot_map, cos, sin, kv_pool, num_blocks,
+                            num_layers, layer, num_q_heads, num_kv_heads, head_dim, q_norm=None,
+                            k_norm=None, eps=1e-6, q_bias=None, k_bias=None, v_bias=None,
+                            dev_status=None, stream=None):
+    """qk_norm_rope_append into an 8-bit pool; a page's rows are adjacent and rise."""
+    check(lib.lc_qk_norm_rope_append_kv8(
+        _p(q_out), q_out.stride()[0], _p(qkv), qkv.stride()[0], positions.shape[0], _p(positions),
+        _p(slot_map), _p(q_bias), _p(k_bias), _p(v_bias), _p(q_norm), _p(k_norm), eps, _p(cos),
+        _p(sin), cos.shape[0], _p(kv_pool), num_blocks, num_layers, layer, num_q_heads,
+        num_kv_heads, head_dim, _p(dev_status), _stream(stream)), "lc_qk_norm_rope_append_kv8")
+
+
+def unpack_kv8(k_out, v_out, kv_pool, num_blocks, num_layers, layer, num_kv_heads, head_dim,
+               block_tables, context_lens, max_context_len, len_offset=0, dev_status=None,
+               stream=None):
+    """The sequences' 8-bit pages as bf16 pages [batch * P][1][Hkv][16][hd]."""
+    check(lib.lc_unpack_kv8(_p(k_out), _p(v_out), _p(kv_pool), num_blocks, num_layers, layer,
+                            num_kv_heads, head_dim, _p(block_tables), block_tables.stride()[0],
+                            _p(context_lens), len_offset, context_lens.shape[0], max_context_len,
+                            _p(dev_status), _stream(stream)), "lc_unpack_kv8")
+
+
+def alloc_decode_kv8_workspace(batch, num_q_heads, num_kv_heads, head_dim, tokens_per_seq=1,
+                               device="cuda"):
+    """Zeroed workspace for paged_decode_kv8."""
+    import torch
+    n = lib.lc_paged_decode_kv8_workspace_size(batch, num_q_heads, num_kv_heads, head_dim,
+                                               tokens_per_seq)
+    return torch.zeros(n, dtype=torch.uint8, device=device)
+
+
+def paged_decode_kv8(out, q, kv_pool, num_blocks, num_layers, layer, num_q_heads, num_kv_heads,
+                     head_dim, block_tables, context_lens, max_context_len=0, tokens_per_seq=1,
+                     sm_scale=None, len_offset=0, workspace=None, dev_status=None, stream=None):
+    """Attention of each sequence's newest tokens_per_seq tokens over an 8-bit pool."""
+    if sm_scale is None:
+        sm_scale = 1.0 / math.sqrt(head_dim)
+    check(lib.lc_paged_decode_kv8(_p(out), out.stride()[0], _p(q), q.stride()[0], _p(kv_pool),
+                                  num_blocks, num_layers, layer, num_q_heads, num_kv_heads,
+                                  head_dim, _p(block_tables), block_tables.stride()[0],
+                                  _p(context_lens), len_offset, context_lens.shape[0],
+                                  tokens_per_seq, max_context_len, sm_scale, _p(workspace),
+                                  _nbytes(workspace), _p(dev_status), _stream(stream)),
+          "lc_paged_decode_kv8")
+
+
 # ------------------------------------------------------------ host mirrors --
 
 def rope_table_host(max_pos, head_dim, base, scale_factor=0.0):
@@ -756,6 +827,16 @@ def sample_top_p(out_idx, logits, top_k, top_p, rand_vals, workspace, stream=Non
     check(lib.lc_sample_top_p(_p(logits), logits.stride(0), vocab, batch, top_k, _p(top_p),
                               _p(rand_vals), _p(out_idx), _p(workspace), workspace.numel(),
                               _stream(stream)), "lc_sample_top_p")
+
+
+def sample(out_idx, logits, rand_vals, temperature=None, top_k=None, top_p=None, min_p=None,
+           stream=None):
+    """A draw per row with its own temperature, top-k, top-p and min-p (device tensors [batch]:
+    top_k int32, the others float32; None: temperature 1, no filter)."""
+    batch, vocab = logits.shape
+    check(lib.lc_sample(_p(logits), logits.stride()[0], vocab, batch, _p(temperature), _p(top_k),
+                        _p(top_p), _p(min_p), _p(rand_vals), _p(out_idx), _stream(stream)),
+          "lc_sample")
 
 
 def pool_blocks_for_budget(num_layers, num_kv_heads, head_dim, free_bytes, total_bytes,
