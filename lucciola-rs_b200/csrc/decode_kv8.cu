@@ -1,94 +1,173 @@
 // decode_kv8.cu - attention of the newest tokens of each sequence over the 8-bit
-// paged cache (kv8.cuh). For query token i of T of sequence b, which holds n
-// tokens with them, and query head h of kv head h / (Hq / Hkv):
-//     out = softmax_t(q . k_t * sm_scale) . v_t    over t < n - (T - 1 - i)
-// in one pass: a running maximum m and sum l per query row, the output rescaled
-// when m rises. One warp per query row and head, its lanes over the dims.
-#include <climits>
-#include <cmath>
-
+// paged cache (kv8.cuh): decode_stream.cuh with its pages.
+//
+// Unpacking. e4m3 to fp16 is one exact conversion per pair; the page's scales do not touch
+// the elements (decode_stream.cuh: page_scales).
+//  * K: lane t of a quad takes two 16-dim pieces of a token (one at hd 64), t and t + 4, as
+//    16-byte loads; a word is one step of the product.
+//  * V: a lane holds hd/8 consecutive dims of 4 tokens and needs pairs of tokens per dim:
+//    two tokens' words are interleaved by bytes first, then converted.
+#include "decode_stream.cuh"
 #include "kv8.cuh"
-#include "lc_host.h"
 
 namespace lc {
 namespace {
 
-struct DecodeKv8Params {
-    bf16 *out;
-    int64_t out_stride;
-    const bf16 *q;
-    int64_t q_stride;
-    const uint8_t *kv_pool;
-    int64_t num_blocks;
-    int num_layers, layer, num_q_heads, num_kv_heads;
-    const int *tables;
-    int table_stride;
-    const int *ctx_lens;
-    int len_offset, batch, tokens;
-    float sm_scale;
-    int *status;
-};
+// The 8-bit pages, for decode_stream.cuh.
+template <int D>
+struct Kv8 {
+    static constexpr int kDim = D;
+    static constexpr int kPage = kv8_page_bytes(D);  // K and V of one kv head
+    template <int NT>
+    static constexpr int kGroup = D == 64 || NT == 2 ? 2 : 1;
+    static constexpr int kStages = 2;
+    static constexpr int kMinPages = 16;  // pages per CTA at least
+    static constexpr int kEdgeUnits = 20;
+    static constexpr bool kPageScales = true;
+    static constexpr int kSteps = D / 16, kWords = D / 16;  // words per token and lane (K)
 
-template <int HD>
-__global__ void __launch_bounds__(128) decode_kv8_kernel(const DecodeKv8Params p) {
-    constexpr int kPer = HD / 32;
-    const int lane = threadIdx.x & 31;
-    const int64_t task = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (task >= (int64_t)p.batch * p.tokens * p.num_q_heads) return;
-    const int h = (int)(task % p.num_q_heads);
-    const int64_t row = task / p.num_q_heads;
-    const int b = (int)(row / p.tokens), i = (int)(row % p.tokens);
-    const int kvh = h / (p.num_q_heads / p.num_kv_heads);
-    long long n = (long long)__ldg(p.ctx_lens + b) + p.len_offset;
-    if (n > (long long)p.table_stride * kBlockSize) {
-        if (h == 0 && i == 0 && lane == 0) set_status(p.status, LC_DEV_BAD_POS);
-        n = (long long)p.table_stride * kBlockSize;
+    static __device__ __forceinline__ int64_t offset(int64_t phys, int layer, int head, int layers,
+                                                     int heads) {
+        return kv8_offset(phys, layer, head, layers, heads, D);
     }
-    const int seen = (int)max(n - (p.tokens - 1 - i), 0ll);
-    float q[kPer], o[kPer], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int d = 0; d < kPer; ++d) {
-        q[d] = __bfloat162float(p.q[row * p.q_stride + (int64_t)h * HD + lane * kPer + d]);
-        o[d] = 0.f;
+    // Lane t's dims of q, eight at a time: its pieces in turn.
+    static __device__ __forceinline__ int q_dim(int t, int k) { return k / 2 * 64 + t * 16 + k % 2 * 8; }
+
+    // K's scale, log2 of V's and 1 / V's, from whatever the page holds.
+    static __device__ __forceinline__ void page_scales(const uint8_t *page, float &ks, float &lv,
+                                                       float &out_v) {
+        const uint2 sc = *reinterpret_cast<const uint2 *>(page + 2 * kv8_half_bytes(D));
+        ks = kv8_scale(kv8_scale_exp(sc.x));
+        const int e = kv8_scale_exp(sc.y);
+        lv = (float)e;
+        out_v = kv8_scale(-e);
     }
-    const int piece = lane * kPer / 16, in_piece = lane * kPer % 16;
-    for (int t0 = 0; t0 < seen; t0 += kBlockSize) {
-        const int phys = __ldg(p.tables + (int64_t)b * p.table_stride + t0 / kBlockSize);
-        const bool ok = phys >= 0 && phys < p.num_blocks;
-        if (!ok && lane == 0) set_status(p.status, LC_DEV_BAD_BLOCK);
-        const uint8_t *page =
-            p.kv_pool + kv8_offset(ok ? phys : 0, p.layer, kvh, p.num_layers, p.num_kv_heads, HD);
-        const uint32_t *sc = reinterpret_cast<const uint32_t *>(page + 2 * kv8_half_bytes(HD));
-        const float ks = kv8_scale(kv8_scale_exp(sc[0])), vs = kv8_scale(kv8_scale_exp(sc[1]));
-        for (int t = 0; t < min(kBlockSize, seen - t0); ++t) {
-            const uint8_t *at = page + t * HD + kv8_piece(HD, t, piece) * 16 + in_piece;
-            float s = 0.f, v[kPer];
+
+    template <int NT, int kGroup>
+    static __device__ __forceinline__ void scores(const uint8_t *st, const uint2 *qs, int pi0, int t,
+                                                  float (&s)[kGroup][NT][4]) {
+        uint32_t wa[kGroup][kWords], wb[kGroup][kWords];  // tokens pi0 and pi0 + 8
+        const int at = pi0 * D + kv8_piece(D, pi0, t) * 16;
 #pragma unroll
-            for (int d = 0; d < kPer; d += 2) {
-                const uint32_t k2 = ok ? kv8_half2(*reinterpret_cast<const uint16_t *>(at + d)) : 0u;
-                const uint32_t v2 = ok ? kv8_half2(*reinterpret_cast<const uint16_t *>(
-                                             at + kv8_half_bytes(HD) + d)) : 0u;
-                const float2 k = __half22float2(*reinterpret_cast<const __half2 *>(&k2));
-                const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&v2));
-                s = fmaf(q[d], k.x, fmaf(q[d + 1], k.y, s));
-                v[d] = x.x * vs, v[d + 1] = x.y * vs;
+        for (int pg = 0; pg < kGroup; ++pg) {
+#pragma unroll
+            for (int i = 0; i < kWords; i += 4) {  // piece t + i, whose place differs in that bit
+                const uint8_t *kp = st + pg * kPage + (at ^ (i * 16));
+                const uint4 a = *reinterpret_cast<const uint4 *>(kp);
+                const uint4 b = *reinterpret_cast<const uint4 *>(kp + 8 * D);
+                wa[pg][i] = a.x, wa[pg][i + 1] = a.y, wa[pg][i + 2] = a.z, wa[pg][i + 3] = a.w;
+                wb[pg][i] = b.x, wb[pg][i + 1] = b.y, wb[pg][i + 2] = b.z, wb[pg][i + 3] = b.w;
             }
+        }
 #pragma unroll
-            for (int w = 16; w; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-            s *= ks * p.sm_scale;
-            const float top = fmaxf(m, s), off = top == -INFINITY ? 0.f : top;
-            const float down = m == -INFINITY ? 0.f : expf(m - top), w = expf(s - off);
-            m = top;
-            l = fmaf(l, down, w);
+        for (int w = 0; w < kWords; ++w) {
+            uint2 qf[NT];
 #pragma unroll
-            for (int d = 0; d < kPer; ++d) o[d] = fmaf(o[d], down, w * v[d]);
+            for (int nt = 0; nt < NT; ++nt) qf[nt] = qs[(nt * kSteps + w) * 32];
+#pragma unroll
+            for (int pg = 0; pg < kGroup; ++pg) {
+                uint32_t a0, a1, a2, a3;
+                kv8_half4(wa[pg][w], a0, a2);
+                kv8_half4(wb[pg][w], a1, a3);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                    if (w == 0)
+                        mma_f16_first(s[pg][nt], a0, a1, a2, a3, qf[nt].x, qf[nt].y);
+                    else
+                        mma_f16(s[pg][nt], a0, a1, a2, a3, qf[nt].x, qf[nt].y);
+            }
         }
     }
-    const float r = seen == 0 ? 0.f : 1.f / l;
-    bf16 *dst = p.out + row * p.out_stride + (int64_t)h * HD + lane * kPer;
+
+    // Bytes of a word that are NaN codes, a bit each.
+    static __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
+        const uint32_t is = __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu);
+        return (is & 1u) | (is >> 7 & 2u) | (is >> 14 & 4u) | (is >> 21 & 8u);
+    }
+
+    // Page pg of the group at token tok0. `held`: tokens of the chunk's pages, `all`: that every
+    // column sees, lim: that a column sees.
+    template <int NT, bool kTail>
+    static __device__ __forceinline__ void values(const uint8_t *st, int pg, int g, int t,
+                                                  const uint32_t (&pf)[NT][2],
+                                                  float (&o)[kSteps][NT][4], int tok0, int held,
+                                                  int all, int drafts, const int (&lim)[NT][2]) {
+        constexpr int kVWords = D / 32;  // 4 dims each
+        const uint8_t *vp = st + pg * kPage + kv8_half_bytes(D);
+        uint32_t v[4][kVWords];
 #pragma unroll
-    for (int d = 0; d < kPer; ++d) dst[d] = __float2bfloat16(o[d] * r);
-}
+        for (int i = 0; i < 4; ++i) {
+            const int row = (i & 1 ? 7 - t : t) + (i >> 1) * 8;
+            if constexpr (D == 128) {
+                const uint4 x =
+                    *reinterpret_cast<const uint4 *>(vp + row * D + kv8_piece(D, row, g) * 16);
+                v[i][0] = x.x, v[i][1] = x.y, v[i][2] = x.z, v[i][3] = x.w;
+            } else {
+                const uint2 x = *reinterpret_cast<const uint2 *>(
+                    vp + row * D + kv8_piece(D, row, g / 2) * 16 + g % 2 * 8);
+                v[i][0] = x.x, v[i][1] = x.y;
+            }
+        }
+        if constexpr (kTail) {
+            const int first = tok0 + pg * kBlockSize, left = held - first, common = all - first;
+            uint32_t nan[4] = {};  // by dim
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = (i & 1 ? 7 - t : t) + (i >> 1) * 8;
+                // tokens past the end hold anything: zeros
+                const bool in = row < left;
+#pragma unroll
+                for (int w = 0; w < kVWords; ++w) v[i][w] = in ? v[i][w] : 0u;
+                if (drafts > 1 && row >= common) {
+                    // Of the last tokens, which not every column sees, NaN must reach the
+                    // columns that see it only, not as 0 * NaN the others.
+#pragma unroll
+                    for (int w = 0; w < kVWords; ++w) {
+                        const uint32_t is = nan_bytes(v[i][w]);
+                        nan[i] |= is << 4 * w;
+                        v[i][w] &= ~((is & 1u) * 0xffu | (is >> 1 & 1u) * 0xff00u |
+                                     (is >> 2 & 1u) * 0xff0000u | (is >> 3 & 1u) * 0xff000000u);
+                    }
+                }
+            }
+            if (drafts > 1 && __any_sync(0xffffffffu, nan[0] | nan[1] | nan[2] | nan[3])) {
+#pragma unroll 1
+                for (int from = 0; from < 4; ++from) {  // lane of the quad
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t dims = __shfl_sync(0xffffffffu, nan[i], g * 4 + from);
+                        const int row = (i & 1 ? 7 - from : from) + (i >> 1) * 8;
+                        if (dims == 0) continue;
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int k = 0; k < 2; ++k)
+                                if (row < lim[nt][k] - first)
+#pragma unroll
+                                    for (int j = 0; j < kSteps; ++j) {
+                                        if (dims >> 2 * j & 1) o[j][nt][k] = NAN;
+                                        if (dims >> (2 * j + 1) & 1) o[j][nt][k + 2] = NAN;
+                                    }
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int w = 0; w < kVWords; ++w) {
+            uint32_t a[4], b[4];  // dims 4 w ..: tokens t, 7 - t | 8 + t, 15 - t
+            kv8_half4(__byte_perm(v[0][w], v[1][w], 0x5140), a[0], a[1]);
+            kv8_half4(__byte_perm(v[0][w], v[1][w], 0x7362), a[2], a[3]);
+            kv8_half4(__byte_perm(v[2][w], v[3][w], 0x5140), b[0], b[1]);
+            kv8_half4(__byte_perm(v[2][w], v[3][w], 0x7362), b[2], b[3]);
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                    mma_f16(o[2 * w + k][nt], a[2 * k], a[2 * k + 1], b[2 * k], b[2 * k + 1], pf[nt][0],
+                            pf[nt][1]);
+        }
+    }
+};
 
 }  // namespace
 }  // namespace lc
@@ -97,10 +176,7 @@ using namespace lc;
 
 extern "C" size_t lc_paged_decode_kv8_workspace_size(int batch, int num_q_heads, int num_kv_heads,
                                                      int head_dim, int tokens_per_seq) {
-    if (batch <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads ||
-        tokens_per_seq <= 0 || (head_dim != 64 && head_dim != 128))
-        return 0;
-    return 256;
+    return decode_workspace(batch, num_q_heads, num_kv_heads, head_dim, tokens_per_seq);
 }
 
 extern "C" int lc_paged_decode_kv8(void *out, int64_t out_stride, const void *q, int64_t q_stride,
@@ -112,31 +188,12 @@ extern "C" int lc_paged_decode_kv8(void *out, int64_t out_stride, const void *q,
                                    void *workspace, size_t workspace_bytes, int *dev_status,
                                    lc_stream_t stream) {
     if (!out || !q || !kv_pool || !block_tables || !context_lens) return LC_ERR_INVALID_ARGUMENT;
-    if (head_dim != 64 && head_dim != 128) return LC_ERR_UNSUPPORTED_HEAD_DIM;
-    if (batch < 0 || tokens_per_seq <= 0 || num_layers <= 0 || layer < 0 || layer >= num_layers ||
-        num_q_heads <= 0 || num_kv_heads <= 0 || num_blocks <= 0 || table_stride <= 0 ||
-        max_context_len < 0 || len_offset < 0 || len_offset > 1)
-        return LC_ERR_INVALID_ARGUMENT;
-    if (num_q_heads % num_kv_heads) return LC_ERR_UNSUPPORTED_SHAPE;
-    if (table_stride > INT_MAX / kBlockSize || num_blocks > INT_MAX ||
-        (int64_t)batch * tokens_per_seq > INT_MAX / num_q_heads / head_dim)
-        return LC_ERR_INVALID_ARGUMENT;
-    if (q_stride < (int64_t)num_q_heads * head_dim || out_stride < (int64_t)num_q_heads * head_dim)
-        return LC_ERR_INVALID_ARGUMENT;
-    if (!aligned16(kv_pool) || !aligned16(q) || (q_stride & 7) || ((uintptr_t)out & 1))
-        return LC_ERR_MISALIGNED;
-    if (batch == 0) return LC_OK;
-    if (!workspace || workspace_bytes < 256) return LC_ERR_WORKSPACE_TOO_SMALL;
-    if (!aligned16(workspace)) return LC_ERR_MISALIGNED;
-    DecodeKv8Params p{(bf16 *)out, out_stride, (const bf16 *)q, q_stride, (const uint8_t *)kv_pool,
-                      num_blocks, num_layers, layer, num_q_heads, num_kv_heads, block_tables,
-                      table_stride, context_lens, len_offset, batch, tokens_per_seq, sm_scale,
-                      dev_status};
-    const int64_t tasks = (int64_t)batch * tokens_per_seq * num_q_heads;
-    const unsigned blocks = (unsigned)((tasks + 3) / 4);
-    if (head_dim == 64)
-        decode_kv8_kernel<64><<<blocks, 128, 0, as_stream(stream)>>>(p);
-    else
-        decode_kv8_kernel<128><<<blocks, 128, 0, as_stream(stream)>>>(p);
-    return launch_status();
+    DecodeParams p{};
+    p.scale_log2 = std::fabs(sm_scale) * 1.4426950408889634f;
+    p.q_sign = std::signbit(sm_scale) ? 0x80008000u : 0u;
+    p.v_scale = 1.f;
+    return decode_stream<Kv8>(p, out, out_stride, q, q_stride, kv_pool, num_blocks, num_layers, layer,
+                              num_q_heads, num_kv_heads, head_dim, block_tables, table_stride,
+                              context_lens, len_offset, batch, tokens_per_seq, max_context_len,
+                              workspace, workspace_bytes, dev_status, stream);
 }
