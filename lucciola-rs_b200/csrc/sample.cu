@@ -16,10 +16,11 @@
 // running weight along it, and only the last step, the r-th token of one value, looks at
 // tokens again.
 //
-// The histogram has a bin for each value of a magnitude in [2^-23, 2^10) and one for zero,
-// 8449 in all: 34 KB of shared memory, where all 65536 would fill more than an SM has. A row
-// with a logit elsewhere (not counting those that are never chosen) takes the slow way,
-// window by window of the values.
+// The histogram has a bin for each value of a magnitude in [2^-22, 2^10), one for zero and
+// one for each of the four ranges beside them, 8197 in all: 33 KB of shared memory, where all
+// 65536 would fill more than an SM has. In such a range a row may have one token (a tiny logit
+// turns up in one of 100 rows of 151936 normal ones); a row with more in one takes the slow
+// way, window by window of the values.
 //
 // One cluster of CTAs per row (one CTA where there are rows enough): each counts a slice,
 // the others add their bins to the first one's, that one answers the questions, and all look
@@ -37,10 +38,14 @@ namespace {
 constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kMaxChunks = 1024;  // of a slice
-constexpr int kHotLow = 0x3400, kHotHigh = 0x4480, kHot = kHotHigh - kHotLow;  // magnitudes, as bits
-constexpr int kBins = 2 * kHot + 1;
+constexpr int kAhead = 4;         // words of 16 bytes that a lane loads at a time
+constexpr int kHotLow = 0x3480, kHotHigh = 0x4480, kHot = kHotHigh - kHotLow;  // magnitudes, as bits
+static_assert(kHot == 4096);  // see count_token
+constexpr int kRanges = 4;  // beyond kHotHigh, below kHotLow, and the same of the negative ones
+constexpr int kBins = 2 * kHot + 1 + kRanges;
 constexpr int kOwn = 17;  // bins of a thread
-static_assert(kOwn * kSampleThreads >= kBins && kOwn <= 32);
+constexpr int kCounters = (kBins + 32 + 3) / 4 * 4;
+constexpr int kBinades = kHot / 128;  // of either sign
 // Of the slow way: windows of the values, which are numbered by their rank.
 constexpr int kWindowBins = 4096, kWindows = 65536 / kWindowBins;
 constexpr int kWindowOwn = kWindowBins / kSampleThreads;
@@ -69,24 +74,78 @@ __device__ __forceinline__ double value_of(int rank) {
     const uint32_t bits = rank & 0x8000 ? (uint32_t)rank : (uint32_t)rank ^ 0x7fffu;
     return (double)__uint_as_float(bits << 16);
 }
-// Rank of the histogram's d-th value, the largest first, and the word that counts it.
-__device__ __forceinline__ int rank_of_bin(int d) {
-    return d < kHot ? d + 0x8000 - kHotHigh : d == kHot ? kZeroRank : d - kHot - 1 + 0x8000 + kHotLow;
-}
-__device__ __forceinline__ int word_of_bin(int d) {
-    return d < kHot ? kHot - 1 - d : d == kHot ? 2 * kHot : d - 1;
+// Which bins a thread has, from the largest values on: thread 0 the range beyond the
+// histogram's positive values, then these, then one thread the tiny ones, zero and the tiny
+// negative ones, then the negative values, then the range beyond. A thread's bins of either
+// sign are of one binade or two, and so its weights are two geometric sequences.
+constexpr int kHalfThreads = (kHot + kOwn - 1) / kOwn;
+constexpr int kThreadPos = 1, kThreadZero = kThreadPos + kHalfThreads, kThreadNeg = kThreadZero + 1,
+              kThreadLow = kThreadNeg + kHalfThreads;
+static_assert(kThreadLow < kSampleThreads && kOwn <= 32 && kOwn <= 128);
+constexpr int kRankPos = 0x8000 - kHotHigh, kRankNeg = 0x8000 + kHotLow;  // the first ones
+// After the words of the values come those of the first range, the second, zero, the others.
+constexpr int kWordZero = 2 * kHot + 2;
+__device__ __forceinline__ int word_of_range(int range) { return 2 * kHot + range + (range >= 2); }
+// A thread's bins: words word0, word0 + down, .. of the histogram.
+struct Place {
+    bool sign;              // of one sign's values, their ranks one after the other
+    int word0, down, bins, rank0;
+    __device__ __forceinline__ explicit Place(int t) {
+        const bool pos = t >= kThreadPos && t < kThreadZero, neg = t >= kThreadNeg && t < kThreadLow;
+        sign = pos || neg;
+        word0 = pos   ? kHot - 1 - (t - kThreadPos) * kOwn
+                : neg ? kHot + (t - kThreadNeg) * kOwn
+                      : 2 * kHot + (t == 0 ? 0 : t == kThreadZero ? 1 : 4);
+        down = pos ? -1 : 1;
+        bins = pos   ? min(kOwn, word0 + 1)
+               : neg ? min(kOwn, 2 * kHot - word0)
+                     : t == kThreadZero ? 3 : t == 0 || t == kThreadLow ? 1 : 0;
+        rank0 = pos ? kRankPos + kHot - 1 - word0 : kRankNeg + word0 - kHot;
+    }
+    __device__ __forceinline__ int word(int j) const { return word0 + j * down; }
+    // `in_range`: the ranks of the tokens in the ranges
+    __device__ __forceinline__ int rank(int j, const int *in_range) const {
+        if (sign) return rank0 + j;
+        return word0 + j == kWordZero ? kZeroRank : in_range[word0 + j - 2 * kHot - (word0 + j > kWordZero)];
+    }
+};
+__device__ __forceinline__ int range_of(uint32_t bits) {
+    const bool tiny = (bits & 0x7fffu) < (uint32_t)kHotLow;
+    return bits & 0x8000u ? (tiny ? 2 : 3) : (tiny ? 1 : 0);
 }
 
 // Weights of the values of a row.
 struct Weights {
     int best;         // rank of the largest
     double top, inv;  // its logit, 1 / temperature
+    __device__ __forceinline__ double exponent(double x) const {
+        const double d = x - top;  // -inf below an infinite logit
+        return d == -INFINITY ? d : d * inv;
+    }
     __device__ __forceinline__ double operator()(int rank) const {
-        if (rank == best) return 1.0;
-        const double d = value_of(rank) - top;  // -inf below an infinite logit
-        return d == -INFINITY ? 0.0 : exp(d * inv);
+        return rank == best ? 1.0 : exp(exponent(value_of(rank)));
     }
 };
+
+// What a row is sampled with. Read before the logits, so that the reads' latency is theirs.
+struct RowParams {
+    float temperature, top_p, min_p;
+    int top_k;
+    double rand;
+    __device__ __forceinline__ RowParams(const SampleParams &p, int b)
+        : temperature(p.temperature ? __ldg(p.temperature + b) : 1.f),
+          top_p(p.top_p ? __ldg(p.top_p + b) : 1.f), min_p(p.min_p ? __ldg(p.min_p + b) : 0.f),
+          top_k(p.top_k ? __ldg(p.top_k + b) : 0), rand(__ldg(p.rand_vals + b)) {}
+};
+
+// c ? a : b without a branch
+__device__ __forceinline__ double select(bool c, double a, double b) {
+    double x;
+    asm("{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %3, 0;\n\tselp.f64 %0, %1, %2, p;\n\t}"
+        : "=d"(x)
+        : "d"(a), "d"(b), "r"((int)c));
+    return x;
+}
 
 struct Mass {
     int count;
@@ -95,7 +154,7 @@ struct Mass {
 
 struct Shared {
     union {
-        unsigned hist[kBins];
+        alignas(16) unsigned hist[kCounters];  // the bins, then a word per lane for what has none
         int in_chunk[kMaxChunks];  // tokens of the value sought, once the histogram is done with
     };
     double upto_weight[kSampleThreads];  // inclusive, of the bins of threads 0 .. t
@@ -105,13 +164,43 @@ struct Shared {
     int warp_count[kSampleWarps];
     Mass before[kWindows + 1];  // slow way: of all windows before
     int in_window[kWindows], built, number;
-    unsigned cold;  // a logit outside the histogram
+    int in_range[kRanges];  // rank of the token in each range
     int best;
+    double ratio[2 * kBinades], first[2 * kBinades + 2];  // see choose
     // the value sought, which of its tokens, whether it has several; rank -1: no token
     int rank, at, several;
-    double weight;
+    double weight;  // up to that token
+    int at_least;
     int found[kMaxCluster];  // tokens of that value in each slice
 };
+
+// The larger of two pairs of logits; a NaN is smaller than all others.
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+// All ones in the halves of two pairs of logits that are equal (as +0 and -0 are).
+__device__ __forceinline__ uint32_t equal_bf16x2(uint32_t a, uint32_t b) {
+    return __heq2_mask(*reinterpret_cast<const __nv_bfloat162 *>(&a),
+                       *reinterpret_cast<const __nv_bfloat162 *>(&b));
+}
+
+// Counts a token; true for one without a bin, but not for logits of -1e30 and below. z: four
+// times its bits; `trash`: this lane's word for what has no bin, as bytes; hist: where the
+// histogram lies. With y = z - 4 kHotLow a magnitude has a bin if 4 * 4096 and the next two
+// bits of y are zero, and its word is that of the magnitude's low 12 bits, of the second half
+// where the sign, three bits on, is set. No branch; an atom whose result nobody reads takes
+// two instructions less than a red (38.9 million tokens: 23.1 us, 26.0; with a branch 27.2).
+__device__ __forceinline__ bool count_token(uint32_t z, uint32_t trash, uint32_t hist) {
+    const uint32_t y = z - 4 * kHotLow;
+    const bool hot = (y & 0x1c000u) == 0;
+    const uint32_t at = hot ? (y & 0x3fffu) | (y >> 3 & ~0x3fffu) : trash;
+    asm volatile("{\n\t.reg .b32 old;\n\tatom.shared.add.u32 old, [%0], 1;\n\t}" ::"r"(at + hist)
+                 : "memory");
+    return !hot && z <= 4 * kLastRank;
+}
 
 // A row as 16-byte words from an aligned address on; tokens before and after it are -inf.
 struct Row {
@@ -132,6 +221,12 @@ struct Row {
             x[e] = lo | hi << 16;
         }
         return make_uint4(x[0], x[1], x[2], x[3]);
+    }
+    __device__ __forceinline__ bool inside(int w0, int w1) const {  // words without such tokens
+        return (w0 > 0 || skip == 0) && (int64_t)w1 * 8 - skip <= vocab;
+    }
+    __device__ __forceinline__ uint4 inner(int w) const {
+        return __ldg(reinterpret_cast<const uint4 *>(p) + w);
     }
     // f(bits) for all tokens, by one CTA
     template <class F>
@@ -157,8 +252,8 @@ __device__ __forceinline__ uint32_t in_cta(const void *p, int rank) {
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
     return a;
 }
-__device__ __forceinline__ void remote_add(uint32_t at, unsigned v) {
-    asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+__device__ __forceinline__ void remote_add(uint32_t at, uint64_t v) {
+    asm volatile("red.relaxed.cluster.shared::cluster.add.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory");
 }
 __device__ __forceinline__ void remote_store(uint32_t at, int v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
@@ -175,10 +270,20 @@ __device__ __forceinline__ void running(int c, double w, Shared &s) {
     }
     if (lane == 31) s.warp_count[warp] = c, s.warp_weight[warp] = w;
     __syncthreads();
-    double before = 0.0;
-    for (int i = 0; i < warp; ++i) c += s.warp_count[i], before += s.warp_weight[i];
+    int cs = lane < kSampleWarps ? s.warp_count[lane] : 0;
+    double ws = lane < kSampleWarps ? s.warp_weight[lane] : 0.0;
+#pragma unroll
+    for (int d = 1; d < kSampleWarps; d <<= 1) {
+        const int uc = __shfl_up_sync(0xffffffffu, cs, d);
+        const double uw = __shfl_up_sync(0xffffffffu, ws, d);
+        if (lane >= d) cs += uc, ws += uw;
+    }
+    if (warp > 0) {
+        c += __shfl_sync(0xffffffffu, cs, warp - 1);
+        w += __shfl_sync(0xffffffffu, ws, warp - 1);
+    }
     s.upto_count[tid] = c;
-    s.upto_weight[tid] = before + w;
+    s.upto_weight[tid] = w;
     __syncthreads();
 }
 
@@ -207,7 +312,7 @@ __device__ __noinline__ void build(const Row &row, int window, const Weights &we
 }
 
 // The value chosen and which of its tokens into s.rank and s.at, by the whole CTA.
-__device__ __noinline__ void choose_slowly(const SampleParams &p, int b, const Row &row, Shared &s) {
+__device__ __noinline__ void choose_slowly(const RowParams &r, const Row &row, Shared &s) {
     const int tid = threadIdx.x;
     __syncthreads();
     if (tid == 0) s.best = INT_MAX, s.built = -1;
@@ -224,7 +329,7 @@ __device__ __noinline__ void choose_slowly(const SampleParams &p, int b, const R
     if ((tid & 31) == 0) atomicMin(&s.best, best);
     __syncthreads();
     best = s.best;
-    const float t = p.temperature ? p.temperature[b] : 1.f;
+    const float t = r.temperature;
     if (best == INT_MAX || !(t > 0.f)) {
         __syncthreads();
         if (tid == 0) s.rank = best == INT_MAX ? -1 : best, s.at = 0, s.several = 1;
@@ -309,9 +414,8 @@ __device__ __noinline__ void choose_slowly(const SampleParams &p, int b, const R
     };
     const int all = s.before[kWindows].count;
     int keep = all;
-    const int k = p.top_k ? p.top_k[b] : 0;
-    if (k > 0) keep = min(keep, k);
-    const float tp = p.top_p ? p.top_p[b] : 1.f;
+    if (r.top_k > 0) keep = min(keep, r.top_k);
+    const float tp = r.top_p;
     if (tp <= 0.f) {
         keep = 1;
     } else if (tp < 1.f) {
@@ -322,7 +426,7 @@ __device__ __noinline__ void choose_slowly(const SampleParams &p, int b, const R
         }
         keep = min(keep, min(by_weight((double)tp * kept, false), INT_MAX - 1) + 1);
     }
-    const float mp = p.min_p ? p.min_p[b] : 0.f;
+    const float mp = r.min_p;
     if (mp > 0.f) {
         // the weights fall along the order: the first value whose weight is below min_p
         int lo = best, hi = kLastRank + 1;
@@ -345,174 +449,172 @@ __device__ __noinline__ void choose_slowly(const SampleParams &p, int b, const R
         __syncthreads();
     }
     by_count(keep - 1);
-    const double goal = (double)p.rand_vals[b] * s.weight;
+    const double goal = r.rand * s.weight;
     __syncthreads();
     const int n = by_weight(goal > 0.0 ? goal : 0.0, true);
     by_count(min(n, keep - 1));
 }
 
 // ------------------------------------------------------------ the fast way --
-// One warp's questions to the histogram.
-struct Asker {
-    const Shared &s;
-    const Weights &weight;
-    int lane;
-
-    struct Bins {  // of thread t, bin j in lane j
-        int h, c;  // tokens, and those up to it with the threads before
-        double each, w;
-    };
-    __device__ __forceinline__ Bins bins(int t) const {
-        Bins x;
-        const int d = t * kOwn + lane;
-        x.h = lane < kOwn && d < kBins ? (int)s.hist[word_of_bin(d)] : 0;
-        x.each = x.h ? weight(rank_of_bin(d)) : 0.0;
-        x.c = x.h;
-        x.w = x.h * x.each;
-#pragma unroll
-        for (int k = 1; k < 32; k <<= 1) {
-            const int uc = __shfl_up_sync(0xffffffffu, x.c, k);
-            const double uw = __shfl_up_sync(0xffffffffu, x.w, k);
-            if (lane >= k) x.c += uc, x.w += uw;
-        }
-        if (t) x.c += s.upto_count[t - 1], x.w += s.upto_weight[t - 1];
-        return x;
-    }
-    // First thread whose running value passes `test`; the last one where none does.
-    template <class T>
-    __device__ __forceinline__ int first_thread(T test) const {
-        constexpr int kEach = kSampleThreads / 32;
-        uint32_t m = __ballot_sync(0xffffffffu, test(lane * kEach + kEach - 1));
-        if (m == 0) return kSampleThreads - 1;
-        const int at = (__ffs(m) - 1) * kEach;
-        m = __ballot_sync(0xffffffffu, lane < kEach && test(at + min(lane, kEach - 1)));
-        return at + __ffs(m) - 1;
-    }
-    struct Token {
-        int d, at, h;   // its value's bin, which of its tokens, and how many it has
-        int number;     // of the order
-        double weight;  // up to it
-    };
-    // Token number n of the order.
-    __device__ __forceinline__ Token by_count(int n) const {
-        const int t = first_thread([&](int i) { return s.upto_count[i] > n; });
-        const Bins x = bins(t);
-        const int j = __ffs(__ballot_sync(0xffffffffu, x.c > n)) - 1;
-        Token k;
-        k.d = t * kOwn + j;
-        k.h = __shfl_sync(0xffffffffu, x.h, j);
-        k.at = n - (__shfl_sync(0xffffffffu, x.c, j) - k.h);
-        k.number = n;
-        k.weight = __shfl_sync(0xffffffffu, x.w - (x.h - 1 - k.at) * x.each, j);
-        return k;
-    }
-    // The first token at which the running weight reaches (or, strict, exceeds) x; the last
-    // one of the row where none does.
-    __device__ __forceinline__ Token by_weight(double x, bool strict) const {
-        auto reached = [&](double y) { return strict ? y > x : y >= x; };
-        int t = first_thread([&](int i) { return reached(s.upto_weight[i]); });
-        while (t > 0 && s.upto_count[t] == s.upto_count[t - 1]) --t;  // none reaches it
-        const Bins b = bins(t);
-        const uint32_t full = __ballot_sync(0xffffffffu, b.h > 0);
-        uint32_t m = __ballot_sync(0xffffffffu, b.h > 0 && reached(b.w));
-        const bool some = m != 0;  // not: the thread's sum was another rounding's
-        const int j = some ? __ffs(m) - 1 : 31 - __clz(full);
-        Token k;
-        k.d = t * kOwn + j;
-        k.h = __shfl_sync(0xffffffffu, b.h, j);
-        const double each = __shfl_sync(0xffffffffu, b.each, j);
-        const double from = __shfl_sync(0xffffffffu, b.w, j) - k.h * each;
-        const double y = strict ? floor((x - from) / each) : ceil((x - from) / each) - 1;
-        k.at = some ? (int)fmin(fmax(y, 0.0), k.h - 1.0) : k.h - 1;
-        k.number = __shfl_sync(0xffffffffu, b.c, j) - k.h + k.at;
-        k.weight = from + (k.at + 1) * each;
-        return k;
-    }
-    // Tokens with weight >= mp. The weights fall along the order (and are above 1 before it).
-    __device__ __forceinline__ int at_least(double mp) const {
-        int lo = 0, hi = kBins;  // the first bin below mp lies in lo .. hi
-        while (lo < hi) {
-            const int each = (hi - lo + 31) / 32, d = lo + lane * each;
-            const uint32_t below = __ballot_sync(0xffffffffu, d < hi && !(weight(rank_of_bin(d)) >= mp));
-            const int probes = (hi - lo + each - 1) / each;
-            const int not_below = below ? __ffs(below) - 1 : probes;
-            if (below) hi = lo + not_below * each;
-            if (not_below) lo += (not_below - 1) * each + 1;
-        }
-        return count_before(lo);
-    }
-    __device__ __forceinline__ int count_before(int d) const {
-        const int t = min(d / kOwn, kSampleThreads - 1);
-        const int k = t * kOwn + lane;
-        const int h = k < d && k < kBins ? (int)s.hist[word_of_bin(k)] : 0;
-        return __reduce_add_sync(0xffffffffu, h) + (t ? s.upto_count[t - 1] : 0);
-    }
-};
-
 // The value chosen and which of its tokens into s.rank, s.at and s.several, from the
-// histogram, by the whole CTA.
-__device__ __forceinline__ void choose(const SampleParams &p, int b, float t, Shared &s) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    int c = 0, first = INT_MAX;
-    for (int j = kOwn - 1; j >= 0; --j) {
-        const int d = tid * kOwn + j, n = d < kBins ? (int)s.hist[word_of_bin(d)] : 0;
-        c += n;
-        if (n) first = d;
-    }
-    first = __reduce_min_sync(0xffffffffu, first);
-    if (lane == 0) atomicMin(&s.best, first);
-    __syncthreads();
+// histogram, by the whole CTA. A thread adds up its bins, whose weights are two geometric
+// sequences at most; a question (a number of tokens, or a weight) goes to all threads, and the
+// warp in whose bins the answer lies looks at them one by lane. Most rows fill a fifth of the
+// bins: warps without tokens skip the sums.
+__device__ __forceinline__ void choose(const RowParams &r, Shared &s) {
+    const int tid = threadIdx.x, lane = tid & 31;
     const int best = s.best;
-    if (best == INT_MAX) {
+    if (best > kLastRank) {
         if (tid == 0) s.rank = -1;
         return;
     }
-    const Weights weight{rank_of_bin(best), value_of(rank_of_bin(best)), 1.0 / (double)t};
-    double w = 0.0;
+    const Weights weight{best, value_of(best), 1.0 / (double)r.temperature};
+    const Place mine(tid);
+    int c = 0;
+    for (int j = 0; j < mine.bins; ++j) c += (int)s.hist[mine.word(j)];
+    const bool pos = mine.sign && mine.down < 0;
+    const int i0 = pos ? mine.word0 : mine.word0 - kHot;  // magnitude of bin 0 - kHotLow
+    // Two rounds of exponentials. First, by a thread each: the ratio of a binade's neighbours
+    // and the weight of its first value, the weight of zero and the ratio of the tiny negative
+    // token's to it. Then each thread's first weight.
+    double each = 0.0;
 #pragma unroll 1
-    for (int j = 0; j < kOwn; ++j) {
-        const int d = tid * kOwn + j;
-        const unsigned n = d < kBins ? s.hist[word_of_bin(d)] : 0u;
-        if (n) w += n * weight(rank_of_bin(d));
+    for (int round = 0; round < 2; ++round) {
+        double x = 0.0;
+        if (round == 0) {
+            const int k = tid % (2 * kBinades), binade = k % kBinades;
+            const bool positive = k < kBinades;
+            const int mag = kHotLow + binade * 128 + (positive ? 127 : 0);
+            if (tid < 2 * kBinades)
+                x = -__longlong_as_double((int64_t)((mag >> 7) - 134 + 1023) << 52) * weight.inv;
+            else if (tid < 4 * kBinades)
+                x = weight.exponent(value_of(positive ? mag ^ 0x7fff : mag | 0x8000));
+            else
+                x = tid == 4 * kBinades ? weight.exponent(0.0) : value_of(s.in_range[2]) * weight.inv;
+        } else if (c) {
+            x = weight.exponent(value_of(mine.rank(0, s.in_range)));
+        }
+        if (round == 0 || __any_sync(0xffffffffu, c > 0)) x = exp(x);
+        if (round == 1) each = x;
+        else if (tid < 2 * kBinades) s.ratio[tid] = x;
+        else if (tid < 4 * kBinades + 2) s.first[tid - 2 * kBinades] = x;
+        __syncthreads();
     }
+    const float tp = r.top_p, mp = r.min_p;
+    int n_least = 0;
+    double w = 0.0;
+    if (__any_sync(0xffffffffu, c > 0)) {
+        double by = 0.0, other, other_by;
+        int next = 1, at_best = -1;
+        if (mine.sign) {
+            const int binade = i0 >> 7, in = i0 & 127, base = pos ? 0 : kBinades;
+            const int following = min(max(binade + mine.down, 0), kBinades - 1);
+            next = pos ? in + 1 : 128 - in;
+            at_best = best - mine.rank0;
+            by = s.ratio[base + binade];
+            other = s.first[base + following], other_by = s.ratio[base + following];
+        } else {
+            for (int j = 0; j < mine.bins; ++j)
+                if (mine.rank(j, s.in_range) == best) at_best = j;
+            other = s.first[2 * kBinades], other_by = s.first[2 * kBinades + 1];
+        }
+        // four counts at a time: read and converted one by one they would wait for one another
+#pragma unroll 1
+        for (int j0 = 0; j0 < mine.bins; j0 += 4) {
+            int h[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) h[i] = j0 + i < mine.bins ? (int)s.hist[mine.word(j0 + i)] : 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int j = j0 + i;
+                each = select(j == next, other, each * select(j == 0, 1.0, by));
+                by = select(j == next, other_by, by);
+                each = select(j == at_best, 1.0, each);  // what lies before the best has no tokens
+                w = fma((double)h[i], select(h[i] != 0, each, 0.0), w);
+                n_least += (int)(each >= (double)mp) * h[i];
+            }
+        }
+    }
+    n_least = __reduce_add_sync(0xffffffffu, n_least);
+    if (lane == 0) atomicAdd(&s.at_least, n_least);
     running(c, w, s);
-    if (warp != 0) return;
-    const Asker ask{s, weight, lane};
+    const int upto_c = s.upto_count[tid], from_c = upto_c - c;
+    const double upto_w = s.upto_weight[tid], from_w = tid ? s.upto_weight[tid - 1] : 0.0;
     const int all = s.upto_count[kSampleThreads - 1];
+    // The token number n of the order (by_count), or the first one at which the running weight
+    // reaches (strict: exceeds) x, or the last one: into s.rank, s.at, s.several, s.number,
+    // s.weight.
+    auto ask = [&](bool by_count, bool strict, int n, double x) {
+        auto reached = [&](int count, double y) {
+            return by_count ? count > n : strict ? y > x : y >= x;
+        };
+        const uint32_t here = __ballot_sync(
+            0xffffffffu, c > 0 && (from_c == 0 || !reached(from_c, from_w)) &&
+                             (reached(upto_c, upto_w) || upto_c == all));
+        __syncthreads();  // the last answer has been read
+        if (here) {
+            const int from = __ffs(here) - 1;
+            const Place in(tid - lane + from);
+            int h = lane < in.bins ? (int)s.hist[in.word(lane)] : 0;
+            const int rank = lane < in.bins ? in.rank(lane, s.in_range) : 0;
+            const double each = h ? weight(rank) : 0.0;
+            int count = h;
+            double sum = h * each;
+#pragma unroll 1
+            for (int k = 1; k < 32; k <<= 1) {
+                const int uc = __shfl_up_sync(0xffffffffu, count, k);
+                const double uw = __shfl_up_sync(0xffffffffu, sum, k);
+                if (lane >= k) count += uc, sum += uw;
+            }
+            count += __shfl_sync(0xffffffffu, from_c, from);
+            sum += __shfl_sync(0xffffffffu, from_w, from);
+            const uint32_t full = __ballot_sync(0xffffffffu, h > 0);
+            const uint32_t m = __ballot_sync(0xffffffffu, h > 0 && reached(count, sum));
+            if (lane == (m ? __ffs(m) - 1 : 31 - __clz(full))) {
+                // h tokens of weight `each` up to number `count` and weight `sum`
+                double at = h - 1;  // not reached: the thread's sum was another rounding's
+                if (m && h > 1) {
+                    const double y = (x - (sum - h * each)) / each;
+                    at = by_count ? n - (count - h) : strict ? floor(y) : ceil(y) - 1;
+                }
+                s.at = (int)fmin(fmax(at, 0.0), h - 1.0);
+                s.number = count - h + s.at;
+                s.weight = sum - (h - 1 - s.at) * each;
+                s.several = h > 1;
+                s.rank = rank;
+            }
+        }
+        __syncthreads();
+    };
+    // top-k, top-p, min-p, the draw, and the last token kept where the draw lies behind it
     int keep = all;
     double kept = s.upto_weight[kSampleThreads - 1];
-    const int k = p.top_k ? p.top_k[b] : 0;
-    const float tp = p.top_p ? p.top_p[b] : 1.f, mp = p.min_p ? p.min_p[b] : 0.f;
-    const double u = p.rand_vals[b];
-    if (k > 0 && k < keep) {
-        keep = k;
-        kept = ask.by_count(keep - 1).weight;
-    }
-    if (tp < 1.f) {
-        const int n = tp > 0.f ? ask.by_weight((double)tp * kept, false).number + 1 : 1;
-        if (n < keep) {
-            keep = n;
-            kept = ask.by_count(keep - 1).weight;
+    const int n_min = mp > 0.f ? max(1, s.at_least) : all;
+#pragma unroll 1
+    for (int step = 0; step < 5; ++step) {
+        if (step == 0) {
+            if (r.top_k <= 0 || r.top_k >= keep) continue;
+            keep = r.top_k;
+        } else if (step == 1) {
+            if (tp <= 0.f) keep = 1, kept = 1.0;
+            if (!(tp < 1.f) || tp <= 0.f) continue;
+        } else if (step == 2) {
+            if (n_min >= keep) continue;
+            keep = n_min;
+        } else if (step == 4) {
+            if (s.number < keep) break;
         }
-    }
-    if (mp > 0.f) {
-        const int n = max(1, ask.at_least((double)mp));
-        if (n < keep) {
-            keep = n;
-            kept = ask.by_count(keep - 1).weight;
+        const double goal = step == 1 ? (double)tp * kept : fmax(r.rand * kept, 0.0);
+        ask(step != 1 && step != 3, step == 3, keep - 1, goal);
+        if (step == 1) {
+            if (s.number + 1 < keep) keep = s.number + 1, kept = s.weight;
+        } else if (step != 3) {
+            kept = s.weight;
         }
-    }
-    const double goal = u * kept;
-    Asker::Token got = ask.by_weight(goal > 0.0 ? goal : 0.0, true);
-    if (got.number >= keep) got = ask.by_count(keep - 1);
-    if (lane == 0) {
-        s.rank = rank_of_bin(got.d);
-        s.at = got.at;
-        s.several = got.h > 1;
     }
 }
 
-__global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, int ctas, int chunk_words) {
+__global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleParams p, int ctas, int chunk_words) {
     __shared__ Shared s;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int b = blockIdx.x / ctas, cta = blockIdx.x % ctas;  // a cluster is a row's CTAs
@@ -521,72 +623,94 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
     const int words = row.words(), chunks_in_all = (words + chunk_words - 1) / chunk_words;
     const int per = (chunks_in_all + ctas - 1) / ctas;
     const int chunk0 = min(chunks_in_all, cta * per), chunks = min(chunks_in_all, chunk0 + per) - chunk0;
-    const float t = p.temperature ? __ldg(p.temperature + b) : 1.f;
-    const bool greedy = !(t > 0.f);
+    const RowParams with(p, b);
+    const bool greedy = !(with.temperature > 0.f);
 
-    for (int i = tid; i < kBins; i += kSampleThreads) s.hist[i] = 0;
-    if (tid == 0) s.cold = 0, s.best = INT_MAX;
+#pragma unroll 1
+    for (int i = tid; i < kCounters / 4; i += kSampleThreads)
+        reinterpret_cast<uint4 *>(s.hist)[i] = make_uint4(0, 0, 0, 0);
+    if (tid < kRanges) s.in_range[tid] = kLastRank;
+    if (tid == 0) s.best = INT_MAX, s.at_least = 0;
     __syncthreads();
     if (ctas > 1) cluster_arrive();
-    bool cold = false;
+    const uint32_t hist = smem_u32(s.hist), trash = (kBins + lane) * 4;
+    // one word of a chunk: its largest logits go into `most`, its tokens into the histogram
+    auto take = [&](const uint4 &u, uint32_t &most) {
+        const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) most = max_bf16x2(most, x[e]);
+        if (greedy) return;
+        bool other = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            other |= count_token(x[e] << 2 & 0x3fffcu, trash, hist);
+            other |= count_token(x[e] >> 14 & 0x3fffcu, trash, hist);
+        }
+        if (!other) return;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t bits = x[e / 2] >> e % 2 * 16 & 0xffffu;
+            if ((bits & 0x7fffu) - kHotLow < (uint32_t)kHot) continue;
+            if ((bits & 0x7fffu) == 0) {
+                atomicAdd(&s.hist[kWordZero], 1u);
+            } else if (eligible(rank_of(bits))) {
+                const int range = range_of(bits);
+                atomicAdd(&s.hist[word_of_range(range)], 1u);
+                s.in_range[range] = rank_of(bits);  // of one token, where one is there
+            }
+        }
+    };
     for (int c = warp; c < chunks; c += kSampleWarps) {
+        uint32_t most = 0xff80ff80u;
         const int w0 = (chunk0 + c) * chunk_words, w1 = min(words, w0 + chunk_words);
-        uint32_t least = 0xffffffffu;  // ranks, two at a time
-        for (int w = w0 + lane; w < w1; w += 32) {
-            const uint4 u = row.word(w);
-            const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+        if (row.inside(w0, w0 + chunk_words)) {
+            for (int w = w0 + lane; w < w1; w += 32 * kAhead) {
+                uint4 u[kAhead];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t neg = (x[e] >> 15 & 0x00010001u) * 0x7fffu;
-                least = __vminu2(least, x[e] ^ 0x7fff7fffu ^ neg);
-            }
-            if (greedy) continue;
+                for (int i = 0; i < kAhead; ++i) u[i] = row.inner(w + 32 * i);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t bits = e & 1 ? x[e / 2] >> 16 : x[e / 2] & 0xffffu;
-                const uint32_t m = bits & 0x7fffu, i = m - kHotLow;
-                if (i < (uint32_t)kHot) {
-                    atomicAdd(&s.hist[i + (bits >> 15) * kHot], 1u);
-                } else if (m == 0) {
-                    atomicAdd(&s.hist[2 * kHot], 1u);
-                } else {
-                    cold |= eligible(rank_of(bits));
-                }
+                for (int i = 0; i < kAhead; ++i) take(u[i], most);
             }
+        } else {
+            for (int w = w0 + lane; w < w1; w += 32) take(row.word(w), most);
         }
-        least = __reduce_min_sync(0xffffffffu, min(least & 0xffffu, least >> 16));
-        if (least == 0x8000u) least = kZeroRank;
-        if (lane == 0) {
-            s.best_of[c] = (uint16_t)least;
-            if (greedy) atomicMin(&s.best, (int)least);
-        }
+        const int least =
+            __reduce_min_sync(0xffffffffu, min(rank_of(most & 0xffffu), rank_of(most >> 16)));
+        if (lane != 0) continue;
+        s.best_of[c] = (uint16_t)least;
+        atomicMin(&s.best, least);
     }
-    if (__any_sync(0xffffffffu, cold) && lane == 0) s.cold = 1;
     __syncthreads();
     if (ctas > 1) {
         cluster_wait();  // the first CTA's histogram was zero before this
         if (cta != 0) {
             const uint32_t to = in_cta(s.hist, 0);
-            if (!greedy)
-                for (int i = tid; i < kBins; i += kSampleThreads)
-                    if (s.hist[i]) remote_add(to + 4 * i, s.hist[i]);
-            if (tid == 0) {
-                if (s.cold) remote_add(in_cta(&s.cold, 0), 1);
-                if (greedy)
-                    asm volatile("red.relaxed.cluster.shared::cluster.min.s32 [%0], %1;" ::"r"(
-                                     in_cta(&s.best, 0)), "r"(s.best) : "memory");
+            if (!greedy) {
+#pragma unroll 4
+                for (int i = tid; i < (kBins + 1) / 2; i += kSampleThreads) {  // two bins at a time
+                    const uint64_t two = reinterpret_cast<const uint64_t *>(s.hist)[i];
+                    if (two) remote_add(to + 8 * i, two);
+                }
+                if (tid < kRanges && s.hist[word_of_range(tid)])
+                    remote_store(in_cta(&s.in_range[tid], 0), s.in_range[tid]);
             }
+            if (tid == 0)
+                asm volatile("red.relaxed.cluster.shared::cluster.min.s32 [%0], %1;" ::"r"(
+                                 in_cta(&s.best, 0)), "r"(s.best) : "memory");
         }
         cluster_arrive();
         cluster_wait();
     }
     if (cta == 0) {
-        if (s.cold || (greedy && s.best < kFirstRank)) {  // NaN counts as a value that is looked for
-            choose_slowly(p, b, row, s);
+        bool slow = false;
+        if (!greedy)
+            for (int i = 0; i < kRanges; ++i) slow |= s.hist[word_of_range(i)] > 1;
+        if (slow) {
+            choose_slowly(with, row, s);
         } else if (greedy) {
             if (tid == 0) s.rank = s.best <= kLastRank ? s.best : -1, s.at = 0, s.several = 1;
         } else {
-            choose(p, b, t, s);
+            choose(with, s);
         }
         __syncthreads();
         if (tid < 3 * (ctas - 1)) {
@@ -604,12 +728,15 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
     if (want < 0) {
         if (cta == 0 && tid == 0) p.out[b] = 0xffffffffu;
     }
-    auto matches = [&](int w) {  // bits of the word's tokens that have the value
-        const uint4 u = row.word(w);
-        const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+    const uint32_t want2 = (uint32_t)(want & 0x8000 ? want : want ^ 0x7fff) * 0x10001u;
+    auto matches = [&](const uint4 &u) {  // bits of the word's tokens that have the value
+        const uint32_t x[4] = {equal_bf16x2(u.x, want2), equal_bf16x2(u.y, want2),
+                               equal_bf16x2(u.z, want2), equal_bf16x2(u.w, want2)};
         uint32_t m = 0;
+        if (x[0] | x[1] | x[2] | x[3]) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) m |= (uint32_t)(rank_of(x[e / 2] >> e % 2 * 16 & 0xffffu) == want) << e;
+            for (int e = 0; e < 4; ++e) m |= (x[e] & 1u) << 2 * e | (x[e] >> 31) << (2 * e + 1);
+        }
         return m;
     };
     if (want >= 0) {
@@ -617,12 +744,16 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
             int n = 0;
             if (s.best_of[c] <= want) {
                 const int w0 = (chunk0 + c) * chunk_words, w1 = min(words, w0 + chunk_words);
+                const bool inside = row.inside(w0, w1);
+                bool any = false;
                 for (int w = w0 + lane; w < w1; w += 32) {
-                    const uint32_t m = matches(w);
-                    if (m && !several) p.out[b] = (unsigned)(w * 8 - row.skip + __ffs(m) - 1);
+                    const uint32_t m = matches(inside ? row.inner(w) : row.word(w));
+                    if (m == 0) continue;
+                    if (!several) p.out[b] = (unsigned)(w * 8 - row.skip + __ffs(m) - 1);
                     n += __popc(m);
+                    any = true;
                 }
-                n = __reduce_add_sync(0xffffffffu, n);
+                n = __any_sync(0xffffffffu, any) ? __reduce_add_sync(0xffffffffu, n) : 0;
             }
             if (lane == 0) s.in_chunk[c] = n;
         }
@@ -660,7 +791,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
         at -= __shfl_sync(0xffffffffu, upto - n, j);
         const int w0 = (chunk0 + c0 + j) * chunk_words, w1 = min(words, w0 + chunk_words);
         for (int w = w0; w < w1; w += 32) {
-            const uint32_t in = w + lane < w1 ? matches(w + lane) : 0u;
+            const uint32_t in = w + lane < w1 ? matches(row.word(w + lane)) : 0u;
             int sum = __popc(in);
 #pragma unroll
             for (int k = 1; k < 32; k <<= 1) {
@@ -696,12 +827,12 @@ extern "C" int lc_sample(const void *logits, int64_t row_stride, int vocab, int 
     if (batch == 0) return LC_OK;
     SampleParams p{(const uint16_t *)logits, row_stride, vocab, temperature, top_k, top_p, min_p,
                    rand_vals, out_idx};
-    // CTAs per row: as many as run at once (four to an SM), of 4096 tokens at least
+    // CTAs per row: as many as run at once (two to an SM), of 4096 tokens at least
     int ctas = 1;
-    while (ctas < kMaxCluster && (int64_t)batch * ctas * 2 <= (int64_t)sm_count() * 4 &&
+    while (ctas < kMaxCluster && (int64_t)batch * ctas * 2 <= (int64_t)sm_count() * 2 &&
            vocab >= 4096 * ctas * 2)
         ctas *= 2;
-    int64_t chunk_words = 32;  // a warp's load
+    int64_t chunk_words = 32 * kAhead;  // what a warp loads at a time
     const int64_t words = ((int64_t)vocab + 7 + 7) / 8;
     while ((words + chunk_words - 1) / chunk_words > (int64_t)kMaxChunks * ctas) chunk_words *= 2;
     cudaLaunchConfig_t cfg = {};
