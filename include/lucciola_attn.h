@@ -635,6 +635,18 @@ int lc_sample(const void *logits, int64_t row_stride, int vocab, int batch,
               const float *min_p, const float *rand_vals, unsigned *out_idx,
               lc_stream_t stream);
 
+/* The same calls with their arguments in one block of num_words 8-byte words, in order:
+ * integers sign-extended, pointers, floats as doubles. For bindings whose foreign calls cost
+ * by the argument. Status of the call; LC_ERR_INVALID_ARGUMENT for another entry or number
+ * of words. */
+enum lc_packed_entry {
+    LC_PACKED_QK_NORM_ROPE_APPEND_KV8 = 0,
+    LC_PACKED_UNPACK_KV8 = 1,
+    LC_PACKED_PAGED_DECODE_KV8 = 2,
+    LC_PACKED_SAMPLE = 3
+};
+int lc_call_packed(int entry, const void *words, int num_words);
+
 /* ------------------------------------------------------------------------- */
 /* Batched token-step driver: many sequences in one paged pool.               */
 /* ------------------------------------------------------------------------- */

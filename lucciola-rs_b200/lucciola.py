@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from pathlib import Path
 
 _HERE = Path(__file__).resolve().parent
@@ -109,6 +110,7 @@ SIGNATURES = {
     "lc_sample_workspace_size": (_sz, [_i32, _i32]),
     "lc_sample_top_p": (_i32, [_vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
     "lc_sample": (_i32, [_vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "lc_call_packed": (_i32, [_i32, C.c_char_p, _i32]),
     "lc_block_alloc_new": (_i32, [_i64, _i32, _i32, C.POINTER(_vp)]),
     "lc_block_alloc_add_seq": (_i32, [_vp, _pi32]),
     "lc_block_alloc_release_seq": (_i32, [_vp, _i32]),
@@ -171,6 +173,32 @@ class LucciolaError(RuntimeError):
 def check(status: int, where: str) -> None:
     if status != LC_OK:
         raise LucciolaError(status, where)
+
+
+def _packed(name: str, entry: int):
+    """The C function `name` through lc_call_packed: one struct.pack and three converted
+    arguments. NULL is 0 here."""
+    kinds = SIGNATURES[name][1]
+    pack = struct.Struct("".join("d" if k is _f32 else "Q" if k in (_vp, _sz) else "q"
+                                 for k in kinds)).pack
+    call, n = lib.lc_call_packed, len(kinds)
+
+    def run(*args):
+        status = call(entry, pack(*args), n)
+        if status:
+            raise LucciolaError(status, name)
+    return run
+
+
+_append_kv8 = _packed("lc_qk_norm_rope_append_kv8", 0)
+_unpack_kv8 = _packed("lc_unpack_kv8", 1)
+_decode_kv8 = _packed("lc_paged_decode_kv8", 2)
+_sample = _packed("lc_sample", 3)
+
+
+def _p0(t):
+    """Device pointer of a tensor, 0 for None."""
+    return 0 if t is None else t.data_ptr()
 
 
 def set_dependent_launch(mode: int) -> int:
@@ -495,21 +523,21 @@ def qk_norm_rope_append_kv8(q_out, qkv, positions, slot_map, cos, sin, kv_pool, 
                             k_norm=None, eps=1e-6, q_bias=None, k_bias=None, v_bias=None,
                             dev_status=None, stream=None):
     """qk_norm_rope_append into an 8-bit pool; a page's rows are adjacent and rise."""
-    check(lib.lc_qk_norm_rope_append_kv8(
-        _p(q_out), q_out.stride()[0], _p(qkv), qkv.stride()[0], positions.shape[0], _p(positions),
-        _p(slot_map), _p(q_bias), _p(k_bias), _p(v_bias), _p(q_norm), _p(k_norm), eps, _p(cos),
-        _p(sin), cos.shape[0], _p(kv_pool), num_blocks, num_layers, layer, num_q_heads,
-        num_kv_heads, head_dim, _p(dev_status), _stream(stream)), "lc_qk_norm_rope_append_kv8")
+    _append_kv8(q_out.data_ptr(), q_out.stride()[0], qkv.data_ptr(), qkv.stride()[0],
+                positions.shape[0], positions.data_ptr(), slot_map.data_ptr(), _p0(q_bias),
+                _p0(k_bias), _p0(v_bias), _p0(q_norm), _p0(k_norm), eps, cos.data_ptr(),
+                sin.data_ptr(), cos.shape[0], kv_pool.data_ptr(), num_blocks, num_layers, layer,
+                num_q_heads, num_kv_heads, head_dim, _p0(dev_status), _stream(stream))
 
 
 def unpack_kv8(k_out, v_out, kv_pool, num_blocks, num_layers, layer, num_kv_heads, head_dim,
                block_tables, context_lens, max_context_len, len_offset=0, dev_status=None,
                stream=None):
     """The sequences' 8-bit pages as bf16 pages [batch * P][1][Hkv][16][hd]."""
-    check(lib.lc_unpack_kv8(_p(k_out), _p(v_out), _p(kv_pool), num_blocks, num_layers, layer,
-                            num_kv_heads, head_dim, _p(block_tables), block_tables.stride()[0],
-                            _p(context_lens), len_offset, context_lens.shape[0], max_context_len,
-                            _p(dev_status), _stream(stream)), "lc_unpack_kv8")
+    _unpack_kv8(k_out.data_ptr(), v_out.data_ptr(), kv_pool.data_ptr(), num_blocks, num_layers,
+                layer, num_kv_heads, head_dim, block_tables.data_ptr(), block_tables.stride()[0],
+                context_lens.data_ptr(), len_offset, context_lens.shape[0], max_context_len,
+                _p0(dev_status), _stream(stream))
 
 
 def alloc_decode_kv8_workspace(batch, num_q_heads, num_kv_heads, head_dim, tokens_per_seq=1,
@@ -527,13 +555,11 @@ def paged_decode_kv8(out, q, kv_pool, num_blocks, num_layers, layer, num_q_heads
     """Attention of each sequence's newest tokens_per_seq tokens over an 8-bit pool."""
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(head_dim)
-    check(lib.lc_paged_decode_kv8(_p(out), out.stride()[0], _p(q), q.stride()[0], _p(kv_pool),
-                                  num_blocks, num_layers, layer, num_q_heads, num_kv_heads,
-                                  head_dim, _p(block_tables), block_tables.stride()[0],
-                                  _p(context_lens), len_offset, context_lens.shape[0],
-                                  tokens_per_seq, max_context_len, sm_scale, _p(workspace),
-                                  _nbytes(workspace), _p(dev_status), _stream(stream)),
-          "lc_paged_decode_kv8")
+    _decode_kv8(out.data_ptr(), out.stride()[0], q.data_ptr(), q.stride()[0], kv_pool.data_ptr(),
+                num_blocks, num_layers, layer, num_q_heads, num_kv_heads, head_dim,
+                block_tables.data_ptr(), block_tables.stride()[0], context_lens.data_ptr(),
+                len_offset, context_lens.shape[0], tokens_per_seq, max_context_len, sm_scale,
+                _p0(workspace), _nbytes(workspace), _p0(dev_status), _stream(stream))
 
 
 # ------------------------------------------------------------ host mirrors --
@@ -834,9 +860,8 @@ def sample(out_idx, logits, rand_vals, temperature=None, top_k=None, top_p=None,
     """A draw per row with its own temperature, top-k, top-p and min-p (device tensors [batch]:
     top_k int32, the others float32; None: temperature 1, no filter)."""
     batch, vocab = logits.shape
-    check(lib.lc_sample(_p(logits), logits.stride()[0], vocab, batch, _p(temperature), _p(top_k),
-                        _p(top_p), _p(min_p), _p(rand_vals), _p(out_idx), _stream(stream)),
-          "lc_sample")
+    _sample(logits.data_ptr(), logits.stride()[0], vocab, batch, _p0(temperature), _p0(top_k),
+            _p0(top_p), _p0(min_p), rand_vals.data_ptr(), out_idx.data_ptr(), _stream(stream))
 
 
 def pool_blocks_for_budget(num_layers, num_kv_heads, head_dim, free_bytes, total_bytes,

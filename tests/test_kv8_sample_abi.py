@@ -93,3 +93,21 @@ def test_sizes():
     assert size(4, 14, 2, 64, 1) > 0
     assert [size(0, 14, 2, 64, 1), size(4, 15, 2, 64, 1), size(4, 14, 2, 96, 1),
             size(4, 14, 2, 64, 0), size(4, 0, 2, 64, 1)] == [0] * 5
+
+
+def test_packed_calls():
+    """Arguments in one block: the same refusals, and the block's own."""
+    import struct
+    call = L.lib.lc_call_packed
+    words = struct.pack("QqqqQQQQQQQ", FAKE, 1000, 1000, 0, 0, 0, 0, 0, FAKE, FAKE, 0)
+    assert call(3, words, 11) == 0
+    assert call(3, words, 10) == INVALID and call(4, words, 11) == INVALID
+    assert call(-1, words, 11) == INVALID and call(3, None, 11) == INVALID
+    assert call(3, struct.pack("QqqqQQQQQQQ", FAKE, 999, 1000, 0, 0, 0, 0, 0, FAKE, FAKE, 0), 11) == INVALID
+    assert call(3, struct.pack("QqqqQQQQQQQ", FAKE, 1000, 1000, -1, 0, 0, 0, 0, FAKE, FAKE, 0), 11) == INVALID
+    eps = [FAKE, 14 * 64, FAKE, 18 * 64, 0, FAKE, FAKE, 0, 0, 0, 0, 0, float("nan"), FAKE, FAKE, 4096,
+           FAKE, 64, 2, 1, 14, 2, 64, 0, 0]
+    fmt = "QqQqqQQQQQQQdQQqQqqqqqqQQ"
+    assert call(0, struct.pack(fmt, *eps), 25) == INVALID
+    eps[12] = 1e-6
+    assert call(0, struct.pack(fmt, *eps), 25) == 0
