@@ -22,7 +22,7 @@ struct Kv8 {
     static constexpr int kGroup = D == 64 || NT == 2 ? 2 : 1;
     static constexpr int kStages = 2;
     static constexpr int kMinPages = 16;  // pages per CTA at least
-    static constexpr int kEdgeUnits = 20;
+    static constexpr int kEdgeUnits = D == 64 ? 48 : 24;
     static constexpr bool kPageScales = true;
     static constexpr int kSteps = D / 16, kWords = D / 16;  // words per token and lane (K)
 

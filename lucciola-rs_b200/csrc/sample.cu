@@ -43,9 +43,9 @@ constexpr int kHotLow = 0x3480, kHotHigh = 0x4480, kHot = kHotHigh - kHotLow;  /
 static_assert(kHot == 4096);  // see count_token
 constexpr int kRanges = 4;  // beyond kHotHigh, below kHotLow, and the same of the negative ones
 constexpr int kBins = 2 * kHot + 1 + kRanges;
-constexpr int kOwn = 17;  // bins of a thread
+constexpr int kOwn = 16;  // bins of a thread, in a binade
+static_assert(2 * kHot == kOwn * kSampleThreads);
 constexpr int kCounters = (kBins + 32 + 3) / 4 * 4;
-constexpr int kBinades = kHot / 128;  // of either sign
 // Of the slow way: windows of the values, which are numbered by their rank.
 constexpr int kWindowBins = 4096, kWindows = 65536 / kWindowBins;
 constexpr int kWindowOwn = kWindowBins / kSampleThreads;
@@ -74,41 +74,35 @@ __device__ __forceinline__ double value_of(int rank) {
     const uint32_t bits = rank & 0x8000 ? (uint32_t)rank : (uint32_t)rank ^ 0x7fffu;
     return (double)__uint_as_float(bits << 16);
 }
-// Which bins a thread has, from the largest values on: thread 0 the range beyond the
-// histogram's positive values, then these, then one thread the tiny ones, zero and the tiny
-// negative ones, then the negative values, then the range beyond. A thread's bins of either
-// sign are of one binade or two, and so its weights are two geometric sequences.
-constexpr int kHalfThreads = (kHot + kOwn - 1) / kOwn;
-constexpr int kThreadPos = 1, kThreadZero = kThreadPos + kHalfThreads, kThreadNeg = kThreadZero + 1,
-              kThreadLow = kThreadNeg + kHalfThreads;
-static_assert(kThreadLow < kSampleThreads && kOwn <= 32 && kOwn <= 128);
-constexpr int kRankPos = 0x8000 - kHotHigh, kRankNeg = 0x8000 + kHotLow;  // the first ones
+// Ranks of the first bins of either sign.
+constexpr int kRankPos = 0x8000 - kHotHigh, kRankNeg = 0x8000 + kHotLow;
 // After the words of the values come those of the first range, the second, zero, the others.
 constexpr int kWordZero = 2 * kHot + 2;
 __device__ __forceinline__ int word_of_range(int range) { return 2 * kHot + range + (range >= 2); }
-// A thread's bins: words word0, word0 + down, .. of the histogram.
-struct Place {
-    bool sign;              // of one sign's values, their ranks one after the other
-    int word0, down, bins, rank0;
-    __device__ __forceinline__ explicit Place(int t) {
-        const bool pos = t >= kThreadPos && t < kThreadZero, neg = t >= kThreadNeg && t < kThreadLow;
-        sign = pos || neg;
-        word0 = pos   ? kHot - 1 - (t - kThreadPos) * kOwn
-                : neg ? kHot + (t - kThreadNeg) * kOwn
-                      : 2 * kHot + (t == 0 ? 0 : t == kThreadZero ? 1 : 4);
-        down = pos ? -1 : 1;
-        bins = pos   ? min(kOwn, word0 + 1)
-               : neg ? min(kOwn, 2 * kHot - word0)
-                     : t == kThreadZero ? 3 : t == 0 || t == kThreadLow ? 1 : 0;
-        rank0 = pos ? kRankPos + kHot - 1 - word0 : kRankNeg + word0 - kHot;
-    }
-    __device__ __forceinline__ int word(int j) const { return word0 + j * down; }
-    // `in_range`: the ranks of the tokens in the ranges
-    __device__ __forceinline__ int rank(int j, const int *in_range) const {
-        if (sign) return rank0 + j;
-        return word0 + j == kWordZero ? kZeroRank : in_range[word0 + j - 2 * kHot - (word0 + j > kWordZero)];
-    }
+
+// What a thread has of the histogram: from the largest values on 16 bins each, and before or
+// after them, as items 0 and 17 or 18, the bins beside the values of a sign.
+constexpr int kItems = kOwn + 3, kHalfThreads = kSampleThreads / 2;
+struct Item {
+    int word, rank;  // word -1: none
 };
+__device__ __forceinline__ Item item_of(int t, int i, const int *in_range) {
+    if (i >= 1 && i <= kOwn)
+        return t < kHalfThreads
+                   ? Item{kHot - t * kOwn - i, kRankPos + t * kOwn + i - 1}
+                   : Item{kHot + (t - kHalfThreads) * kOwn + i - 1, kRankNeg + (t - kHalfThreads) * kOwn + i - 1};
+    if (t == kHalfThreads - 1 && i == kOwn + 2) return Item{kWordZero, kZeroRank};
+    const int range = t == 0 && i == 0                         ? 0
+                      : t == kHalfThreads - 1 && i == kOwn + 1 ? 1
+                      : t == kHalfThreads && i == 0            ? 2
+                      : t == kSampleThreads - 1 && i == kOwn + 1 ? 3 : -1;
+    return range < 0 ? Item{-1, 0} : Item{word_of_range(range), in_range[range]};
+}
+// The thread that has the item of a rank.
+__device__ __forceinline__ int thread_of(int rank) {
+    if (rank <= kZeroRank) return min(max(rank - kRankPos, 0) / kOwn, kHalfThreads - 1);
+    return kHalfThreads + min(max(rank - kRankNeg, 0) / kOwn, kHalfThreads - 1);
+}
 __device__ __forceinline__ int range_of(uint32_t bits) {
     const bool tiny = (bits & 0x7fffu) < (uint32_t)kHotLow;
     return bits & 0x8000u ? (tiny ? 2 : 3) : (tiny ? 1 : 0);
@@ -138,15 +132,6 @@ struct RowParams {
           top_k(p.top_k ? __ldg(p.top_k + b) : 0), rand(__ldg(p.rand_vals + b)) {}
 };
 
-// c ? a : b without a branch
-__device__ __forceinline__ double select(bool c, double a, double b) {
-    double x;
-    asm("{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %3, 0;\n\tselp.f64 %0, %1, %2, p;\n\t}"
-        : "=d"(x)
-        : "d"(a), "d"(b), "r"((int)c));
-    return x;
-}
-
 struct Mass {
     int count;
     double weight;
@@ -166,11 +151,10 @@ struct Shared {
     int in_window[kWindows], built, number;
     int in_range[kRanges];  // rank of the token in each range
     int best;
-    double ratio[2 * kBinades], first[2 * kBinades + 2];  // see choose
     // the value sought, which of its tokens, whether it has several; rank -1: no token
     int rank, at, several;
     double weight;  // up to that token
-    int at_least;
+    int below, at_least;  // first rank below min_p, tokens before it
     int found[kMaxCluster];  // tokens of that value in each slice
 };
 
@@ -456,91 +440,120 @@ __device__ __noinline__ void choose_slowly(const RowParams &r, const Row &row, S
 }
 
 // ------------------------------------------------------------ the fast way --
+// The first rank whose weight is below mp > 0, by one warp: the weights fall along the ranks,
+// and it lies where the logarithm says, or beside it.
+__device__ __forceinline__ int first_below(const Weights &weight, double mp) {
+    const int lane = threadIdx.x & 31;
+    if (weight.inv == 0.0) return mp <= 1.0 ? kLastRank + 1 : kFirstRank;
+    const float x = (float)fmin(fmax(weight.top + log(mp) / weight.inv, -3e38), 3e38);
+    int at = rank_of(__float_as_uint(x) >> 16) - 16;
+    for (;;) {
+        const int r = at + lane;
+        const bool below = r > kLastRank || (r >= kFirstRank && !(weight(r) >= mp));
+        const uint32_t m = __ballot_sync(0xffffffffu, below);
+        if ((m & 1) && at <= kFirstRank) return kFirstRank;
+        if (m & 1) at -= 31;
+        else if (m == 0) at += 31;
+        else return at + __ffs(m) - 1;
+    }
+}
+
 // The value chosen and which of its tokens into s.rank, s.at and s.several, from the
-// histogram, by the whole CTA. A thread adds up its bins, whose weights are two geometric
-// sequences at most; a question (a number of tokens, or a weight) goes to all threads, and the
-// warp in whose bins the answer lies looks at them one by lane. Most rows fill a fifth of the
-// bins: warps without tokens skip the sums.
+// histogram, by the whole CTA. A thread's 16 bins lie in one binade: their values are evenly
+// spaced, their weights a geometric sequence, and their sum is a polynomial in its ratio (two
+// exponentials, not 16). A question (a number of tokens, or a weight) goes to all threads, and
+// the warp of the one in whose bins the answer lies looks at them one by lane. Most rows fill
+// a fifth of the bins; warps without tokens skip the sums.
 __device__ __forceinline__ void choose(const RowParams &r, Shared &s) {
-    const int tid = threadIdx.x, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int best = s.best;
     if (best > kLastRank) {
         if (tid == 0) s.rank = -1;
         return;
     }
     const Weights weight{best, value_of(best), 1.0 / (double)r.temperature};
-    const Place mine(tid);
-    int c = 0;
-    for (int j = 0; j < mine.bins; ++j) c += (int)s.hist[mine.word(j)];
-    const bool pos = mine.sign && mine.down < 0;
-    const int i0 = pos ? mine.word0 : mine.word0 - kHot;  // magnitude of bin 0 - kHotLow
-    // Two rounds of exponentials. First, by a thread each: the ratio of a binade's neighbours
-    // and the weight of its first value, the weight of zero and the ratio of the tiny negative
-    // token's to it. Then each thread's first weight.
-    double each = 0.0;
-#pragma unroll 1
-    for (int round = 0; round < 2; ++round) {
-        double x = 0.0;
-        if (round == 0) {
-            const int k = tid % (2 * kBinades), binade = k % kBinades;
-            const bool positive = k < kBinades;
-            const int mag = kHotLow + binade * 128 + (positive ? 127 : 0);
-            if (tid < 2 * kBinades)
-                x = -__longlong_as_double((int64_t)((mag >> 7) - 134 + 1023) << 52) * weight.inv;
-            else if (tid < 4 * kBinades)
-                x = weight.exponent(value_of(positive ? mag ^ 0x7fff : mag | 0x8000));
-            else
-                x = tid == 4 * kBinades ? weight.exponent(0.0) : value_of(s.in_range[2]) * weight.inv;
-        } else if (c) {
-            x = weight.exponent(value_of(mine.rank(0, s.in_range)));
-        }
-        if (round == 0 || __any_sync(0xffffffffu, c > 0)) x = exp(x);
-        if (round == 1) each = x;
-        else if (tid < 2 * kBinades) s.ratio[tid] = x;
-        else if (tid < 4 * kBinades + 2) s.first[tid - 2 * kBinades] = x;
-        __syncthreads();
-    }
     const float tp = r.top_p, mp = r.min_p;
-    int n_least = 0;
+    // One thread's items, one per lane: tokens, weight of each.
+    struct Seen {
+        int h, rank;
+        double each;
+    };
+    auto look = [&](int t) {
+        const Item item = lane < kItems ? item_of(t, lane, s.in_range) : Item{-1, 0};
+        Seen x;
+        x.rank = item.rank;
+        x.h = item.word >= 0 ? (int)s.hist[item.word] : 0;
+        x.each = x.h ? weight(item.rank) : 0.0;
+        return x;
+    };
+    int c = 0;
     double w = 0.0;
-    if (__any_sync(0xffffffffu, c > 0)) {
-        double by = 0.0, other, other_by;
-        int next = 1, at_best = -1;
-        if (mine.sign) {
-            const int binade = i0 >> 7, in = i0 & 127, base = pos ? 0 : kBinades;
-            const int following = min(max(binade + mine.down, 0), kBinades - 1);
-            next = pos ? in + 1 : 128 - in;
-            at_best = best - mine.rank0;
-            by = s.ratio[base + binade];
-            other = s.first[base + following], other_by = s.ratio[base + following];
-        } else {
-            for (int j = 0; j < mine.bins; ++j)
-                if (mine.rank(j, s.in_range) == best) at_best = j;
-            other = s.first[2 * kBinades], other_by = s.first[2 * kBinades + 1];
+    const bool pos = tid < kHalfThreads;
+    const int word0 = pos ? kHot - (tid + 1) * kOwn : kHot + (tid - kHalfThreads) * kOwn;  // lowest one
+    const uint4 *quads = reinterpret_cast<const uint4 *>(s.hist);
+    uint32_t any = 0;  // of the warp's 512 bins, read side by side
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint4 q = quads[(word0 - (pos ? 31 - lane : lane) * kOwn) / 4 + i * 32 + lane];
+        any |= q.x | q.y | q.z | q.w;
+    }
+    int extra = 0;  // tokens beside the bins
+    if (tid == 0) extra = (int)s.hist[word_of_range(0)];
+    if (tid == kHalfThreads - 1) extra = (int)(s.hist[word_of_range(1)] + s.hist[kWordZero]);
+    if (tid == kHalfThreads) extra = (int)s.hist[word_of_range(2)];
+    if (tid == kSampleThreads - 1) extra = (int)s.hist[word_of_range(3)];
+    if (__any_sync(0xffffffffu, any != 0 || extra != 0)) {
+        const int mag = kHotLow + (pos ? word0 + kOwn - 1 : word0 - kHot);  // of the largest value
+        const double step = __longlong_as_double((int64_t)((mag >> 7) - 134 + 1023) << 52);
+        const double by = exp(-step * weight.inv);
+        const double first = exp(weight.exponent(value_of(pos ? mag ^ 0x7fff : mag | 0x8000)));
+        const double by2 = by * by, by4 = by2 * by2, by8 = by4 * by4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int q = (i + lane / 2) & 3;  // in turns: side by side they hit the same banks
+            const uint4 h = quads[word0 / 4 + q];
+            // from the largest value on
+            const uint32_t a0 = pos ? h.w : h.x, a1 = pos ? h.z : h.y, a2 = pos ? h.y : h.z,
+                           a3 = pos ? h.x : h.w;
+            c += (int)(a0 + a1 + a2 + a3);
+            const double sum = fma(fma(fma((double)a3, by, (double)a2), by, (double)a1), by, (double)a0);
+            const int turn = pos ? 3 - q : q;
+            w = fma(sum, (turn & 1 ? by4 : 1.0) * (turn & 2 ? by8 : 1.0), w);
         }
-        // four counts at a time: read and converted one by one they would wait for one another
-#pragma unroll 1
-        for (int j0 = 0; j0 < mine.bins; j0 += 4) {
-            int h[4];
+        w = c ? w * first : 0.0;
+        // A thread with the best value (above it the sequence may overflow) or with tokens beside
+        // its bins is looked at.
+        const int rank0 = pos ? kRankPos + tid * kOwn : kRankNeg + (tid - kHalfThreads) * kOwn;
+        uint32_t odd = __ballot_sync(0xffffffffu, extra || (best >= rank0 && best < rank0 + kOwn));
+        while (odd) {
+            const int from = __ffs(odd) - 1;
+            odd &= odd - 1;
+            const Seen x = look(tid - lane + from);
+            double sum = x.h * x.each;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) h[i] = j0 + i < mine.bins ? (int)s.hist[mine.word(j0 + i)] : 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int j = j0 + i;
-                each = select(j == next, other, each * select(j == 0, 1.0, by));
-                by = select(j == next, other_by, by);
-                each = select(j == at_best, 1.0, each);  // what lies before the best has no tokens
-                w = fma((double)h[i], select(h[i] != 0, each, 0.0), w);
-                n_least += (int)(each >= (double)mp) * h[i];
-            }
+            for (int k = 16; k; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+            const int count = __reduce_add_sync(0xffffffffu, x.h);
+            if (lane == from) c = count, w = sum;
         }
     }
-    n_least = __reduce_add_sync(0xffffffffu, n_least);
-    if (lane == 0) atomicAdd(&s.at_least, n_least);
+    if (mp > 0.f && warp == kSampleWarps - 1) {  // the smallest logits' warp, which has time
+        const int below = first_below(weight, mp);
+        if (lane == 0) s.below = below;
+    }
     running(c, w, s);
     const int upto_c = s.upto_count[tid], from_c = upto_c - c;
     const double upto_w = s.upto_weight[tid], from_w = tid ? s.upto_weight[tid - 1] : 0.0;
     const int all = s.upto_count[kSampleThreads - 1];
+    if (mp > 0.f) {
+        const int t = thread_of(s.below);
+        if (t / 32 == warp) {
+            const Seen x = look(t);
+            const int n = __reduce_add_sync(0xffffffffu, x.rank < s.below ? x.h : 0) +
+                          __shfl_sync(0xffffffffu, from_c, t % 32);
+            if (lane == 0) s.at_least = n;
+        }
+        __syncthreads();
+    }
     // The token number n of the order (by_count), or the first one at which the running weight
     // reaches (strict: exceeds) x, or the last one: into s.rank, s.at, s.several, s.number,
     // s.weight.
@@ -554,13 +567,11 @@ __device__ __forceinline__ void choose(const RowParams &r, Shared &s) {
         __syncthreads();  // the last answer has been read
         if (here) {
             const int from = __ffs(here) - 1;
-            const Place in(tid - lane + from);
-            int h = lane < in.bins ? (int)s.hist[in.word(lane)] : 0;
-            const int rank = lane < in.bins ? in.rank(lane, s.in_range) : 0;
-            const double each = h ? weight(rank) : 0.0;
+            const Seen seen = look(tid - lane + from);
+            const int h = seen.h;
             int count = h;
-            double sum = h * each;
-#pragma unroll 1
+            double sum = h * seen.each;
+#pragma unroll
             for (int k = 1; k < 32; k <<= 1) {
                 const int uc = __shfl_up_sync(0xffffffffu, count, k);
                 const double uw = __shfl_up_sync(0xffffffffu, sum, k);
@@ -574,14 +585,14 @@ __device__ __forceinline__ void choose(const RowParams &r, Shared &s) {
                 // h tokens of weight `each` up to number `count` and weight `sum`
                 double at = h - 1;  // not reached: the thread's sum was another rounding's
                 if (m && h > 1) {
-                    const double y = (x - (sum - h * each)) / each;
+                    const double y = (x - (sum - h * seen.each)) / seen.each;
                     at = by_count ? n - (count - h) : strict ? floor(y) : ceil(y) - 1;
                 }
                 s.at = (int)fmin(fmax(at, 0.0), h - 1.0);
                 s.number = count - h + s.at;
-                s.weight = sum - (h - 1 - s.at) * each;
+                s.weight = sum - (h - 1 - s.at) * seen.each;
                 s.several = h > 1;
-                s.rank = rank;
+                s.rank = seen.rank;
             }
         }
         __syncthreads();
@@ -630,7 +641,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleParams 
     for (int i = tid; i < kCounters / 4; i += kSampleThreads)
         reinterpret_cast<uint4 *>(s.hist)[i] = make_uint4(0, 0, 0, 0);
     if (tid < kRanges) s.in_range[tid] = kLastRank;
-    if (tid == 0) s.best = INT_MAX, s.at_least = 0;
+    if (tid == 0) s.best = INT_MAX;
     __syncthreads();
     if (ctas > 1) cluster_arrive();
     const uint32_t hist = smem_u32(s.hist), trash = (kBins + lane) * 4;
