@@ -57,7 +57,7 @@ class Engine:
         s = self.stack = stack
         self.slots, self.num_blocks = slots, num_blocks
         self.width = -(-max_len // PAGE)  # pages of one sequence at most
-        self.pool = L.alloc_kv4_pool(num_blocks, s.layers, s.hkv, s.hd)
+        self.pool = self._alloc_pool()
 
         def ints(*shape, fill=0):
             return torch.full(shape, fill, dtype=torch.int32, device="cuda")
@@ -79,6 +79,32 @@ class Engine:
         qkv = torch.empty(x.shape[0], (s.hq + 2 * s.hkv) * s.hd, dtype=torch.bfloat16, device="cuda")
         L.proj_gemm(qkv, x, s.w_qkv[layer])
         return qkv
+
+    # what the cache's format decides (examples/serve_kv8.py has another)
+    def _alloc_pool(self):
+        s = self.stack
+        return L.alloc_kv4_pool(self.num_blocks, s.layers, s.hkv, s.hd)
+
+    def _alloc_workspace(self, batch):
+        s = self.stack
+        return L.alloc_decode_kv4_workspace(batch, s.hq, s.hkv, s.hd)
+
+    def _unpack(self, tables, lens, longest, layer):
+        s = self.stack
+        L.unpack_kv4(self.k16, self.v16, self.pool, self.num_blocks, s.layers, layer, s.hkv, s.hd,
+                     tables, lens, longest, k_scale=self.K_SCALE, v_scale=self.V_SCALE,
+                     dev_status=self.status)
+
+    def _attend(self, out, q, layer):
+        s = self.stack
+        L.paged_decode_kv4(out, q, self.pool, self.num_blocks, s.layers, layer, s.hq, s.hkv, s.hd,
+                           self.step_rows, self.batch_lens, max_context_len=self.width * PAGE,
+                           k_scale=self.K_SCALE, v_scale=self.V_SCALE, workspace=self.ws,
+                           dev_status=self.status)
+
+    def choose(self, out, logits):
+        """The next token of each row."""
+        L.argmax(out, logits)
 
     def _append(self, qkv, positions, slot_map, layer):
         s = self.stack
@@ -104,9 +130,7 @@ class Engine:
         x = s.embed[tokens.long()]
         for layer in range(s.layers):
             q = self._append(self._project(x, layer), pos, slot_map, layer)
-            L.unpack_kv4(self.k16, self.v16, self.pool, self.num_blocks, s.layers, layer, s.hkv,
-                         s.hd, step, lens, start + n, k_scale=self.K_SCALE, v_scale=self.V_SCALE,
-                         dev_status=self.status)
+            self._unpack(step, lens, start + n, layer)
             out = torch.empty_like(q)
             L.paged_prefill(out, q, self.k16, self.v16, self.width, 1, 0, s.hq, s.hkv, s.hd,
                             self.own_pages, before, n, start, dev_status=self.status)
@@ -123,7 +147,7 @@ class Engine:
         self.step_rows = self.ints(b, self.width, fill=-1)
         self.pos, self.slot_map, self.starts = self.ints(b), self.ints(b), self.ints(b + 1)
         s = self.stack
-        self.ws = L.alloc_decode_kv4_workspace(b, s.hq, s.hkv, s.hd)
+        self.ws = self._alloc_workspace(b)
 
         def step():
             L.step_tables(self.tables, self.batch_lens, self.ones, self.free, self.free_count,
@@ -134,14 +158,11 @@ class Engine:
             for layer in range(s.layers):
                 q = self._append(self._project(x, layer), self.pos, self.slot_map, layer)
                 out = torch.empty_like(q)
-                L.paged_decode_kv4(out, q, self.pool, self.num_blocks, s.layers, layer, s.hq, s.hkv,
-                                   s.hd, self.step_rows, self.batch_lens,
-                                   max_context_len=self.width * PAGE, k_scale=self.K_SCALE,
-                                   v_scale=self.V_SCALE, workspace=self.ws, dev_status=self.status)
+                self._attend(out, q, layer)
                 L.proj_gemm(x, out, s.w_o[layer], residual=x)
             logits = torch.empty(b, s.embed.shape[0], dtype=torch.bfloat16, device="cuda")
             L.proj_gemm(logits, x, s.embed)
-            L.argmax(self.token, logits)
+            self.choose(self.token, logits)
             return x
         return step
 
@@ -164,12 +185,12 @@ def first_token(engine, hidden):
     logits = torch.empty(1, s.embed.shape[0], dtype=torch.bfloat16, device="cuda")
     L.proj_gemm(logits, hidden[-1:].contiguous(), s.embed)
     out = torch.zeros(1, dtype=torch.int32, device="cuda")
-    L.argmax(out, logits)
+    engine.choose(out, logits)
     return out
 
 
 def generate(engine, prompts, steps, chunk=256, graph=True):
-    """Greedy tokens [steps, len(prompts)] for a list of 1-d token tensors."""
+    """The engine's tokens [steps, len(prompts)] for a list of 1-d token tensors."""
     nxt = []
     for slot, p in enumerate(prompts):
         for at in range(0, p.shape[0], chunk):

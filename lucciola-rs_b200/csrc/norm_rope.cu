@@ -355,7 +355,8 @@ __device__ __forceinline__ uint2 kv8_codes(const uint64_t (&x)[4], float inv, bo
 }
 
 // The rows [r0, r0 + n) of one page, K or V (is_v) of head hl. Lane i of `pos` and `slot`
-// holds row r0 - first + i's; all of the run's are valid. The rows come kHeads at a time (a
+// holds row r0 - first + i's; all of the run's slots are valid, a row without a place in the
+// RoPE tables (pos -1) is left out. The rows come kHeads at a time (a
 // chunk) and twice where they are more: once for their largest magnitude, once for their
 // codes, the last chunk, whose values are still there, first. Kept in registers, a page's
 // values take 64 of them and leave the GPU a third of the warps (8192 rows of 28/4 heads of
@@ -366,7 +367,9 @@ __device__ __forceinline__ void append_run(const NormRopeParams &p, int r0, int 
     constexpr int kLanes = HD / 16, kHeads = 32 / kLanes, kHalf = HD / 2;
     const int lane = threadIdx.x & 31, c8 = lane % kLanes * 8, grp = lane / kLanes;
     const uint64_t one = pair2(p.one, p.one), minus_one = pair2(-p.one, -p.one);
-    const int slot0 = __shfl_sync(0xffffffffu, slot, first);
+    const uint32_t live = __ballot_sync(0xffffffffu, pos >= 0) >> first & ((1u << n) - 1);  // by row
+    if (live == 0) return;
+    const int slot0 = __shfl_sync(0xffffffffu, slot, first + __ffs(live) - 1);
     uint8_t *page = p.kv_pool + kv8_offset(slot0 / kBlockSize, p.layer, hl, p.num_layers,
                                            p.num_kv_heads, HD);
     uint32_t *scale = reinterpret_cast<uint32_t *>(page + 2 * kv8_half_bytes(HD)) + is_v;
@@ -381,7 +384,8 @@ __device__ __forceinline__ void append_run(const NormRopeParams &p, int r0, int 
     uint4 a, b;
     auto fetch = [&](int c) {
         a = b = make_uint4(0, 0, 0, 0);
-        if (c * kHeads + grp >= n) return;
+        const int i = c * kHeads + grp;
+        if (!(live >> i & 1)) return;
         a = *reinterpret_cast<const uint4 *>(src + (int64_t)c * kHeads * p.row_stride);
         b = *reinterpret_cast<const uint4 *>(src + (int64_t)c * kHeads * p.row_stride + kHalf);
     };
@@ -389,7 +393,7 @@ __device__ __forceinline__ void append_run(const NormRopeParams &p, int r0, int 
     // Values of chunk c, whose row is in a and b; then next's row is on its way.
     auto values = [&](int c, int next) {
         const int i = c * kHeads + grp;
-        const bool in = i < n;
+        const bool in = live >> i & 1;
         const int row_pos = __shfl_sync(0xffffffffu, pos, min(first + i, 31));
         uint64_t cs[4] = {}, sn[4] = {};
         if (!is_v && in) {
@@ -416,7 +420,7 @@ __device__ __forceinline__ void append_run(const NormRopeParams &p, int r0, int 
     if (!fresh && was >= e) {
         e = was;
     } else if (!fresh) {  // the other tokens move to the larger scale
-        const bool in_run = lane >= first && lane < first + n;
+        const bool in_run = lane >= first && lane < first + n && pos >= 0;
         const uint32_t run = __reduce_or_sync(0xffffffffu, in_run ? 1u << slot % kBlockSize : 0u);
         const float down = kv8_scale(was - e);
         for (int v = lane; v < HD; v += 32) {  // 16-byte pieces
@@ -435,7 +439,7 @@ __device__ __forceinline__ void append_run(const NormRopeParams &p, int r0, int 
         if (c < last) values(c, c - 1);
         const int i = c * kHeads + grp;
         const int off = __shfl_sync(0xffffffffu, slot, min(first + i, 31)) % kBlockSize;
-        if (i >= n) continue;
+        if (!(live >> i & 1)) continue;
         uint8_t *to = page + off * HD + c8 % 16;
         *reinterpret_cast<uint2 *>(to + kv8_piece(HD, off, c8 / 16) * 16) = kv8_codes(x1, inv, odd);
         *reinterpret_cast<uint2 *>(to + kv8_piece(HD, off, (c8 + kHalf) / 16) * 16) =
@@ -443,7 +447,7 @@ __device__ __forceinline__ void append_run(const NormRopeParams &p, int r0, int 
     }
 }
 
-constexpr int kMaxTurns = 8;  // of a warp at the queries, with its next heads on their way
+constexpr int kMaxTurns = 4;  // of a warp at the queries, with its next heads on their way
 
 template <int HD>
 __global__ void __launch_bounds__(kNormRopeThreads, kNormRopeCtas)
@@ -463,8 +467,8 @@ __global__ void __launch_bounds__(kNormRopeThreads, kNormRopeCtas)
             pos = __ldg(p.positions + row);
             slot = __ldg(p.slot_map + row);
         }
-        const bool valid = pos >= 0 && pos < p.rope_rows && slot >= 0 &&
-                           slot < p.num_blocks * kBlockSize;
+        const bool valid = pos != -1 && slot >= 0 && slot < p.num_blocks * kBlockSize;
+        if (pos >= p.rope_rows) pos = -1;  // left alone, but within its page's run
         const int page = valid ? slot / kBlockSize : -1;
         const int prev = __shfl_up_sync(0xffffffffu, page, 1);
         const int prev_slot = __shfl_up_sync(0xffffffffu, slot, 1);

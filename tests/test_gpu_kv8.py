@@ -246,6 +246,26 @@ def test_append_in_place_padding_and_bad_rows():
 
 
 @pytest.mark.parametrize("hd", [64, 128])
+def test_append_with_bad_positions_inside_a_page(hd):
+    """Rows without a place in the RoPE tables are left alone; their page's other rows are
+    held as if they were not there, at one scale."""
+    hq, hkv, nb = 2, 2, 8
+    rng = np.random.default_rng(14)
+    cos, sin = O.rope_table(64, hd, 1e6)
+    vec = dict.fromkeys(("q_bias", "k_bias", "v_bias", "q_norm", "k_norm"))
+    slot = np.array([32, 33, 34, 35, 36, 69, 70, 71, 100, 101, 7, 112, 48, 49], np.int32)
+    pos = np.array([0, 64, 2, 99, 4, -7, 6, 7, 64, 64, 3, 70, 64, 1], np.int32)
+    qkv = randn_bf16(rng, (len(slot), (hq + 2 * hkv) * hd))
+    qkv[[1, 3, 5, 8, 9, 11, 12]] = 0x5000  # large, and not looked at
+    before = R.make_pool(rng, nb, 1, hkv, hd)
+    _, got, word = run_append(qkv, pos, slot, before, 0, hq, hkv, hd, vec, cos, sin)
+    assert word == L.LC_DEV_BAD_POS
+    keep = (pos >= 0) & (pos < 64)
+    _, want, word = run_append(qkv[keep], pos[keep], slot[keep], before, 0, hq, hkv, hd, vec, cos, sin)
+    assert word == 0 and np.array_equal(got, want)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
 def test_append_leaves_out_rows_that_do_not_rise(hd):
     """The same slot twice, and a falling one: the page keeps the rows before."""
     hq, hkv, nb = 2, 1, 8
