@@ -155,6 +155,11 @@ struct Shared {
     int rank, at, several;
     double weight;  // up to that token
     int below, at_least;  // first rank below min_p, tokens before it
+    double inv;           // 1 / temperature
+    struct Answer {
+        double weight;  // up to and with the token
+        int rank, at, several, number;
+    } answers[2];  // in turns
     int found[kMaxCluster];  // tokens of that value in each slice
 };
 
@@ -471,7 +476,7 @@ __device__ __forceinline__ void choose(const RowParams &r, Shared &s) {
         if (tid == 0) s.rank = -1;
         return;
     }
-    const Weights weight{best, value_of(best), 1.0 / (double)r.temperature};
+    const Weights weight{best, value_of(best), s.inv};
     const float tp = r.top_p, mp = r.min_p;
     // One thread's items, one per lane: tokens, weight of each.
     struct Seen {
@@ -555,16 +560,17 @@ __device__ __forceinline__ void choose(const RowParams &r, Shared &s) {
         __syncthreads();
     }
     // The token number n of the order (by_count), or the first one at which the running weight
-    // reaches (strict: exceeds) x, or the last one: into s.rank, s.at, s.several, s.number,
-    // s.weight.
-    auto ask = [&](bool by_count, bool strict, int n, double x) {
+    // reaches (strict: exceeds) x, or the last one.
+    int turn = 0;
+    auto ask = [&](bool by_count, bool strict, int n, double x) -> const Shared::Answer & {
         auto reached = [&](int count, double y) {
             return by_count ? count > n : strict ? y > x : y >= x;
         };
+        // an answer stays while the next one is worked out, so one barrier is enough
+        Shared::Answer &answer = s.answers[turn ^= 1];
         const uint32_t here = __ballot_sync(
             0xffffffffu, c > 0 && (from_c == 0 || !reached(from_c, from_w)) &&
                              (reached(upto_c, upto_w) || upto_c == all));
-        __syncthreads();  // the last answer has been read
         if (here) {
             const int from = __ffs(here) - 1;
             const Seen seen = look(tid - lane + from);
@@ -577,52 +583,53 @@ __device__ __forceinline__ void choose(const RowParams &r, Shared &s) {
                 const double uw = __shfl_up_sync(0xffffffffu, sum, k);
                 if (lane >= k) count += uc, sum += uw;
             }
-            count += __shfl_sync(0xffffffffu, from_c, from);
-            sum += __shfl_sync(0xffffffffu, from_w, from);
+            count += __shfl_sync(0xffffffffu, from_c, from) - h;  // before this lane's tokens
+            sum += __shfl_sync(0xffffffffu, from_w, from) - h * seen.each;
             const uint32_t full = __ballot_sync(0xffffffffu, h > 0);
-            const uint32_t m = __ballot_sync(0xffffffffu, h > 0 && reached(count, sum));
+            const uint32_t m =
+                __ballot_sync(0xffffffffu, h > 0 && reached(count + h, sum + h * seen.each));
+            // where none reaches it, the thread's sum was another rounding's: the last token
             if (lane == (m ? __ffs(m) - 1 : 31 - __clz(full))) {
-                // h tokens of weight `each` up to number `count` and weight `sum`
-                double at = h - 1;  // not reached: the thread's sum was another rounding's
-                if (m && h > 1) {
-                    const double y = (x - (sum - h * seen.each)) / seen.each;
-                    at = by_count ? n - (count - h) : strict ? floor(y) : ceil(y) - 1;
+                int at = h - 1;
+                if (by_count) {
+                    at = n - count;
+                } else if (m && h > 1) {  // near it in 32 bits, then exactly
+                    at = (int)fminf(__fdividef((float)(x - sum), (float)seen.each), (float)(h - 1));
+                    at = max(at, 0);
+                    while (at > 0 && reached(0, sum + at * seen.each)) --at;
+                    while (at < h - 1 && !reached(0, sum + (at + 1) * seen.each)) ++at;
                 }
-                s.at = (int)fmin(fmax(at, 0.0), h - 1.0);
-                s.number = count - h + s.at;
-                s.weight = sum - (h - 1 - s.at) * seen.each;
-                s.several = h > 1;
-                s.rank = seen.rank;
+                answer.at = at;
+                answer.number = count + at;
+                answer.weight = sum + (at + 1) * seen.each;
+                answer.several = h > 1;
+                answer.rank = seen.rank;
             }
         }
         __syncthreads();
+        return answer;
     };
     // top-k, top-p, min-p, the draw, and the last token kept where the draw lies behind it
     int keep = all;
     double kept = s.upto_weight[kSampleThreads - 1];
     const int n_min = mp > 0.f ? max(1, s.at_least) : all;
-#pragma unroll 1
-    for (int step = 0; step < 5; ++step) {
-        if (step == 0) {
-            if (r.top_k <= 0 || r.top_k >= keep) continue;
-            keep = r.top_k;
-        } else if (step == 1) {
-            if (tp <= 0.f) keep = 1, kept = 1.0;
-            if (!(tp < 1.f) || tp <= 0.f) continue;
-        } else if (step == 2) {
-            if (n_min >= keep) continue;
-            keep = n_min;
-        } else if (step == 4) {
-            if (s.number < keep) break;
-        }
-        const double goal = step == 1 ? (double)tp * kept : fmax(r.rand * kept, 0.0);
-        ask(step != 1 && step != 3, step == 3, keep - 1, goal);
-        if (step == 1) {
-            if (s.number + 1 < keep) keep = s.number + 1, kept = s.weight;
-        } else if (step != 3) {
-            kept = s.weight;
-        }
+    if (r.top_k > 0 && r.top_k < keep) {
+        keep = r.top_k;
+        kept = ask(true, false, keep - 1, 0.0).weight;
     }
+    if (tp <= 0.f) {
+        keep = 1, kept = 1.0;
+    } else if (tp < 1.f) {
+        const Shared::Answer &last = ask(false, false, 0, (double)tp * kept);
+        if (last.number + 1 < keep) keep = last.number + 1, kept = last.weight;
+    }
+    if (n_min < keep) {
+        keep = n_min;
+        kept = ask(true, false, keep - 1, 0.0).weight;
+    }
+    const Shared::Answer *got = &ask(false, true, 0, fmax(r.rand * kept, 0.0));
+    if (got->number >= keep) got = &ask(true, false, keep - 1, 0.0);
+    if (tid == 0) s.rank = got->rank, s.at = got->at, s.several = got->several;
 }
 
 __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleParams p, int ctas, int chunk_words) {
@@ -641,7 +648,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleParams 
     for (int i = tid; i < kCounters / 4; i += kSampleThreads)
         reinterpret_cast<uint4 *>(s.hist)[i] = make_uint4(0, 0, 0, 0);
     if (tid < kRanges) s.in_range[tid] = kLastRank;
-    if (tid == 0) s.best = INT_MAX;
+    if (tid == 0) s.best = INT_MAX, s.inv = 1.0 / (double)with.temperature;
     __syncthreads();
     if (ctas > 1) cluster_arrive();
     const uint32_t hist = smem_u32(s.hist), trash = (kBins + lane) * 4;
