@@ -175,30 +175,19 @@ def check(status: int, where: str) -> None:
         raise LucciolaError(status, where)
 
 
-def _packed(name: str, entry: int):
-    """The C function `name` through lc_call_packed: one struct.pack and three converted
-    arguments. NULL is 0 here."""
-    kinds = SIGNATURES[name][1]
-    pack = struct.Struct("".join("d" if k is _f32 else "Q" if k in (_vp, _sz) else "q"
-                                 for k in kinds)).pack
-    call, n = lib.lc_call_packed, len(kinds)
-
-    def run(*args):
-        status = call(entry, pack(*args), n)
-        if status:
-            raise LucciolaError(status, name)
-    return run
+def _packer(name: str):
+    """struct.pack of the C function's arguments as lc_call_packed takes them (NULL is 0)."""
+    return struct.Struct("".join("d" if k is _f32 else "Q" if k in (_vp, _sz) else "q"
+                                 for k in SIGNATURES[name][1])).pack
 
 
-_append_kv8 = _packed("lc_qk_norm_rope_append_kv8", 0)
-_unpack_kv8 = _packed("lc_unpack_kv8", 1)
-_decode_kv8 = _packed("lc_paged_decode_kv8", 2)
-_sample = _packed("lc_sample", 3)
-
-
-def _p0(t):
-    """Device pointer of a tensor, 0 for None."""
-    return 0 if t is None else t.data_ptr()
+# Calls through lc_call_packed: three converted arguments instead of two dozen. What is left of
+# a call is mostly reading the tensors, so the wrappers read each of them once and directly.
+_call_packed = lib.lc_call_packed
+_pack_append_kv8 = _packer("lc_qk_norm_rope_append_kv8")
+_pack_unpack_kv8 = _packer("lc_unpack_kv8")
+_pack_decode_kv8 = _packer("lc_paged_decode_kv8")
+_pack_sample = _packer("lc_sample")
 
 
 def set_dependent_launch(mode: int) -> int:
@@ -523,21 +512,29 @@ def qk_norm_rope_append_kv8(q_out, qkv, positions, slot_map, cos, sin, kv_pool, 
                             k_norm=None, eps=1e-6, q_bias=None, k_bias=None, v_bias=None,
                             dev_status=None, stream=None):
     """qk_norm_rope_append into an 8-bit pool; a page's rows are adjacent and rise."""
-    _append_kv8(q_out.data_ptr(), q_out.stride()[0], qkv.data_ptr(), qkv.stride()[0],
-                positions.shape[0], positions.data_ptr(), slot_map.data_ptr(), _p0(q_bias),
-                _p0(k_bias), _p0(v_bias), _p0(q_norm), _p0(k_norm), eps, cos.data_ptr(),
-                sin.data_ptr(), cos.shape[0], kv_pool.data_ptr(), num_blocks, num_layers, layer,
-                num_q_heads, num_kv_heads, head_dim, _p0(dev_status), _stream(stream))
+    status = _call_packed(0, _pack_append_kv8(
+        q_out.data_ptr(), q_out.stride()[0], qkv.data_ptr(), qkv.stride()[0], positions.numel(),
+        positions.data_ptr(), slot_map.data_ptr(), 0 if q_bias is None else q_bias.data_ptr(),
+        0 if k_bias is None else k_bias.data_ptr(), 0 if v_bias is None else v_bias.data_ptr(),
+        0 if q_norm is None else q_norm.data_ptr(), 0 if k_norm is None else k_norm.data_ptr(), eps,
+        cos.data_ptr(), sin.data_ptr(), cos.shape[0], kv_pool.data_ptr(), num_blocks, num_layers,
+        layer, num_q_heads, num_kv_heads, head_dim,
+        0 if dev_status is None else dev_status.data_ptr(), _stream(stream)), 25)
+    if status:
+        raise LucciolaError(status, "lc_qk_norm_rope_append_kv8")
 
 
 def unpack_kv8(k_out, v_out, kv_pool, num_blocks, num_layers, layer, num_kv_heads, head_dim,
                block_tables, context_lens, max_context_len, len_offset=0, dev_status=None,
                stream=None):
     """The sequences' 8-bit pages as bf16 pages [batch * P][1][Hkv][16][hd]."""
-    _unpack_kv8(k_out.data_ptr(), v_out.data_ptr(), kv_pool.data_ptr(), num_blocks, num_layers,
-                layer, num_kv_heads, head_dim, block_tables.data_ptr(), block_tables.stride()[0],
-                context_lens.data_ptr(), len_offset, context_lens.shape[0], max_context_len,
-                _p0(dev_status), _stream(stream))
+    status = _call_packed(1, _pack_unpack_kv8(
+        k_out.data_ptr(), v_out.data_ptr(), kv_pool.data_ptr(), num_blocks, num_layers, layer,
+        num_kv_heads, head_dim, block_tables.data_ptr(), block_tables.stride()[0],
+        context_lens.data_ptr(), len_offset, context_lens.numel(), max_context_len,
+        0 if dev_status is None else dev_status.data_ptr(), _stream(stream)), 16)
+    if status:
+        raise LucciolaError(status, "lc_unpack_kv8")
 
 
 def alloc_decode_kv8_workspace(batch, num_q_heads, num_kv_heads, head_dim, tokens_per_seq=1,
@@ -555,11 +552,16 @@ def paged_decode_kv8(out, q, kv_pool, num_blocks, num_layers, layer, num_q_heads
     """Attention of each sequence's newest tokens_per_seq tokens over an 8-bit pool."""
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(head_dim)
-    _decode_kv8(out.data_ptr(), out.stride()[0], q.data_ptr(), q.stride()[0], kv_pool.data_ptr(),
-                num_blocks, num_layers, layer, num_q_heads, num_kv_heads, head_dim,
-                block_tables.data_ptr(), block_tables.stride()[0], context_lens.data_ptr(),
-                len_offset, context_lens.shape[0], tokens_per_seq, max_context_len, sm_scale,
-                _p0(workspace), _nbytes(workspace), _p0(dev_status), _stream(stream))
+    status = _call_packed(2, _pack_decode_kv8(
+        out.data_ptr(), out.stride()[0], q.data_ptr(), q.stride()[0], kv_pool.data_ptr(),
+        num_blocks, num_layers, layer, num_q_heads, num_kv_heads, head_dim,
+        block_tables.data_ptr(), block_tables.stride()[0], context_lens.data_ptr(), len_offset,
+        context_lens.numel(), tokens_per_seq, max_context_len, sm_scale,
+        0 if workspace is None else workspace.data_ptr(),
+        0 if workspace is None else workspace.nbytes,
+        0 if dev_status is None else dev_status.data_ptr(), _stream(stream)), 23)
+    if status:
+        raise LucciolaError(status, "lc_paged_decode_kv8")
 
 
 # ------------------------------------------------------------ host mirrors --
@@ -860,8 +862,14 @@ def sample(out_idx, logits, rand_vals, temperature=None, top_k=None, top_p=None,
     """A draw per row with its own temperature, top-k, top-p and min-p (device tensors [batch]:
     top_k int32, the others float32; None: temperature 1, no filter)."""
     batch, vocab = logits.shape
-    _sample(logits.data_ptr(), logits.stride()[0], vocab, batch, _p0(temperature), _p0(top_k),
-            _p0(top_p), _p0(min_p), rand_vals.data_ptr(), out_idx.data_ptr(), _stream(stream))
+    status = _call_packed(3, _pack_sample(
+        logits.data_ptr(), logits.stride()[0], vocab, batch,
+        0 if temperature is None else temperature.data_ptr(),
+        0 if top_k is None else top_k.data_ptr(), 0 if top_p is None else top_p.data_ptr(),
+        0 if min_p is None else min_p.data_ptr(), rand_vals.data_ptr(), out_idx.data_ptr(),
+        _stream(stream)), 11)
+    if status:
+        raise LucciolaError(status, "lc_sample")
 
 
 def pool_blocks_for_budget(num_layers, num_kv_heads, head_dim, free_bytes, total_bytes,
