@@ -453,7 +453,7 @@ int lc_paged_decode_kv4(void *out, int64_t out_stride, const void *q, int64_t q_
 /* ------------------------------------------------------------------------- */
 /* kv_pool: uint8 [num_blocks][num_layers][num_kv_heads][lc_kv8_page_bytes], 16-byte
  * aligned: per page and kv head the K codes [16][head_dim] (e4m3), the V codes likewise,
- * K's scale and V's (fp32), 8 unused bytes; 8.06 bits per element (8.125 for heads of
+ * K's scale and V's (fp32), 8 unused bytes: 8.03 bits per element (8.06 for heads of
  * 64), half of the bf16 pools. An element stands for code * scale, with one scale for
  * the page's 16 tokens, a power of two from 2^-40 to 2^40. Dims 16 c .. 16 c + 15 of
  * token t are bytes 16 c' .. 16 c' + 15 of its row, c' = c ^ ((t * head_dim / 64) &

@@ -392,6 +392,7 @@ __device__ __forceinline__ void join_columns(const DecodeParams &p, const ChunkI
     const int own = edge + kEdges * (lane & 7);  // this lane's column
     float2 ml[kWarps];
     float m = -INFINITY, l = 0.f, r[kWarps], scale = 0.f;
+    uint32_t seen = 0;
     int64_t row = -1;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
@@ -403,6 +404,7 @@ __device__ __forceinline__ void join_columns(const DecodeParams &p, const ChunkI
         const bool some = ml[w].x != -INFINITY;  // not: saw nothing of this column
         r[w] = some ? ex2(ml[w].x - m) : 0.f;
         if (some) l = fmaf(ml[w].y, r[w], l);
+        seen |= (uint32_t)some << w;
     }
     if (whole) {  // as in write_row
         const int kvh = kv_head(p, ch.seg), col = (ch.seg - kvh * p.slices) * C::kCols + own;
@@ -415,7 +417,8 @@ __device__ __forceinline__ void join_columns(const DecodeParams &p, const ChunkI
 #pragma unroll 1
     for (int i = 0; i < 8; ++i) {
         const int c = edge + kEdges * i;
-        // all reads first; a warp that saw nothing left zeros
+        const uint32_t see = __shfl_sync(0xffffffffu, seen, i);
+        // all reads first
         float x[kWarps][kPer];
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
@@ -434,8 +437,9 @@ __device__ __forceinline__ void join_columns(const DecodeParams &p, const ChunkI
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             const float rw = __shfl_sync(0xffffffffu, r[w], i);
+            const bool some = see >> w & 1;
 #pragma unroll
-            for (int d = 0; d < kPer; ++d) j.o[d] = fmaf(x[w][d], rw, j.o[d]);
+            for (int d = 0; d < kPer; ++d) j.o[d] = some ? fmaf(x[w][d], rw, j.o[d]) : j.o[d];
         }
         if (whole) {
             const int64_t at = __shfl_sync(0xffffffffu, row, i);

@@ -501,6 +501,38 @@ def test_decode_of_what_is_not_finite(hd):
 
 
 @pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("group,tokens", [(1, 4), (8, 2), (8, 3), (5, 7)])
+def test_nan_values_reach_the_drafted_rows_that_see_them(group, tokens, hd):
+    """For 8, 16 and 24 columns at a time and several slices: V is NaN in one dim of each of the
+    newest tokens."""
+    hkv, n = 2, 85
+    rng = np.random.default_rng(group + tokens)
+    lens = np.array([n, 3, 32], np.int32)
+    tables, nb = make_tables(np.array([R.ceil16(k) for k in lens]), rng)
+    pool = R.make_pool(rng, nb, 1, hkv, hd)
+    R.spoil(pool, tables, lens, hkv, hd)
+    q = randn_bf16(rng, (3 * tokens, group * hkv, hd))
+    want = np.zeros((3 * tokens, group * hkv, hd), bool)
+    for b, held in enumerate(lens):
+        for k in range(min(tokens, held)):  # token held - 1 - k
+            token, dim = held - 1 - k, (11 * k + 7 * b) % hd
+            R.put_code(pool, tables[b, token // 16], 0, k % 2, 1, token % 16, dim, hd, 0xff if k % 3 else 0x7f)
+            rows = b * tokens + np.arange(tokens - k - 1, tokens)
+            want[rows, k % 2 * group:(k % 2 + 1) * group, dim] = True
+    # a row sees `token` if it lies before its end; rows before the first token are zeros
+    for b, held in enumerate(lens):
+        for i in range(tokens):
+            if held - (tokens - 1 - i) <= 0:
+                want[b * tokens + i] = False
+    got = run_decode(q, pool, 0, tables, lens, hkv, hd, tokens)
+    assert np.array_equal(np.isnan(got), want)
+    clean = np.where(pool & 0x7f == 0x7f, 0, pool)
+    clean[..., 32 * hd:] = pool[..., 32 * hd:]
+    ref, bound = R.decode(R.bf16_f64(q), clean, 0, tables, lens, hkv, hd, tokens)
+    assert R.rounds_to(got, ref, bound)[~want].all()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("n,first,last", [(1, 0, 1), (33, 32, 33), (700, 96, 128), (700, 0, 256),
                                           (700, 0, 700), (6000, 0, 2000), (6000, 0, 6000)])
 def test_nan_keys_reach_every_row_that_sees_them(n, first, last, hd):

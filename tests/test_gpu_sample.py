@@ -168,6 +168,34 @@ def test_infinite_and_extreme_logits():
         assert got[0] == 77 and got[1] in (5, 900, 4000)
 
 
+@pytest.mark.parametrize("batch", [1, 30, 100])
+def test_extreme_logits_of_rows_over_several_ctas(batch):
+    """One token in each range beside the histogram's, in different slices of the row, and more
+    than one: the slow way, for the whole cluster."""
+    rng = np.random.default_rng(batch)
+    vocab = 70000 if batch < 100 else 40000
+    bits = randn_bf16(rng, (batch, vocab), scale=2.0)
+    for row in range(batch):
+        at = rng.integers(0, vocab, 40)
+        kind = row % 5 if batch > 1 else 0
+        if kind == 0:
+            bits[row, at[:4]] = (0x4500, 0x0123, 0x8123, 0xc500)  # one each
+        elif kind == 1:
+            bits[row, at[:2]] = (0x0123, 0x0124)
+        elif kind == 2:
+            bits[row, at[:4]] = (0x4500, 0x4501, 0x4500, 0x7f80)
+        elif kind == 3:
+            bits[row] = randn_bf16(rng, vocab, scale=1e-9)
+        else:
+            bits[row, at] = 0xc501
+    for seed in range(3):
+        rng = np.random.default_rng(seed)
+        par = params(rng, batch)
+        if seed == 0:
+            par = dict(temperature=np.full(batch, 300.0))  # the tails count
+        check(bits, rng.random(batch), **par)
+
+
 def test_ends_of_the_draw_and_odd_parameters():
     rng = np.random.default_rng(8)
     bits = randn_bf16(rng, (10, 400), scale=2.0)
