@@ -8,16 +8,16 @@
 //  * V: a lane holds hd/8 consecutive dims of 4 tokens and needs pairs of tokens per dim:
 //    two tokens' words are interleaved by bytes first, then converted.
 //
-// Bounds. 32 sequences of 8192 tokens, 28/4 heads of 128: 49.1 us for 269 MB, 84 % of a device
-// copy's rate, and 2 of 131072: 49.8 us. Between the first page (2.7 us after the start) and
+// Bounds. 32 sequences of 8192 tokens, 28/4 heads of 128: 48.1 to 49.1 us for 269 MB, 84 % of a
+// device copy's rate, and 2 of 131072: 49.9 us. Between the first page (2.7 us after the start) and
 // the last product (39 to 44 us, by SM) the pages come at the copy's rate, and the warps wait
 // for them: 268 instructions of a warp per page, 39 % of the issue slots, the tensor pipe 17 %.
 // What is left is the two ends: the chain length -> table -> page, SMs that share the same
 // bytes ending 4 us apart, the join of the last chunk and its pieces (2.5 us). With 24 columns
-// (3 drafted tokens, 8 sequences of 1024 .. 32000 tokens, 64/8 heads: 67 us of which 42 are
+// (3 drafted tokens, 8 sequences of 1024 .. 32000 tokens, 64/8 heads: 68 us of which 42 are
 // the copy's) two warps per scheduler have 405 instructions and 48 products per page: issue
 // 41 %, tensor pipe 39 %. Short contexts are bound by a CTA's chunks, 4 us each with the join
-// of eight columns (256 sequences of 100 .. 300 tokens, 28/4 heads of 128: 24.6 us).
+// of eight columns (256 sequences of 100 .. 300 tokens, 28/4 heads of 128: 24.4 us).
 #include "decode_stream.cuh"
 #include "kv8.cuh"
 
@@ -31,15 +31,16 @@ struct Kv8 {
     static constexpr int kPage = kv8_page_bytes(D);  // K and V of one kv head
     // Two pages at a time share their reads of q and overlap their products, where a stage of
     // two fits. (32 sequences of 8192 tokens, 14/2 heads of 64: 16.3 us, 19.0 us one at a time;
-    // 2 drafted tokens over 8 of 1024 .. 32000, 64/8 heads of 128: 56.8 us, 66.3 us.)
+    // 2 tokens each over 8 of 1024 .. 32000, 64/8 heads of 128: 57.1 us, 65.3 us.)
     template <int NT>
     static constexpr int kGroup = D == 64 || NT == 2 ? 2 : 1;
     static constexpr int kStages = 2;  // what fits beside a second CTA
-    // Pages per CTA at least. (One sequence of 203 tokens: 6.0 us, 6.6 us with 8 or 12; of 1024
-    // tokens, 14/2 heads of 64: 6.4 us, 8.0 us with 24.)
+    // Pages per CTA at least. (One sequence of 203 tokens: 5.6 us, 6.2 us with 8 or 12; of 1024
+    // tokens, 14/2 heads of 64: 6.4 us, 7.6 us with 24, which takes 10.3 us for one of 12345, 28/4
+    // heads of 128, where this takes 11.3 us.)
     static constexpr int kMinPages = 16;
-    // (64 sequences of 256 .. 4096 tokens, 14/2 heads of 64: 13.2 us, 14.6 us with 20, 13.8 with
-    // 60; 256 of 100 .. 300, 28/4 heads of 128: 28.0 us, 30.8 us with 8, 28.7 with 20.)
+    // (64 sequences of 256 .. 4096 tokens, 14/2 heads of 64: 13.2 us, 14.0 us with 20, 13.8 with
+    // 60; 256 of 100 .. 300, 28/4 heads of 128: 24.4 us, 26.7 us with 8, 24.8 with 20, 25.8 with 48.)
     static constexpr int kEdgeUnits = D == 64 ? 48 : 24;
     static constexpr bool kPageScales = true;
     static constexpr int kSteps = D / 16, kWords = D / 16;  // words per token and lane (K)

@@ -381,7 +381,8 @@ __device__ __forceinline__ void store_piece(const DecodeParams &p, int64_t place
 // lane works out one column's maximum, sum, the warps' factors and the place of its row, for
 // all columns at once; then they are joined one by one, the lanes over the dims. (By
 // join_states and write_row, column after column, it took 2 to 4 us, which short chunks
-// waited for: 256 sequences of 100 .. 300 tokens, 28/4 heads of 128, 8-bit pages, 27.9 us.)
+// waited for: 256 sequences of 100 .. 300 tokens, 28/4 heads of 128, 8-bit pages, 24.4 us
+// like this, 27.9 us.)
 template <class F, int NT>
 __device__ __forceinline__ void join_columns(const DecodeParams &p, const ChunkInfo &ch, bool whole,
                                              int64_t place, int edge, int lane,

@@ -22,10 +22,10 @@
 // turns up in one of 100 rows of 151936 normal ones); a row with more in one takes the slow
 // way, window by window of the values.
 //
-// Bounds. 256 rows of 151936 logits (78 MB, 12 us at a device copy's rate): 46.9 us. Counting
+// Bounds. 256 rows of 151936 logits (78 MB, 12 us at a device copy's rate): 47.5 us. Counting
 // takes 12 instructions for 32 tokens, and 3.75 cycles of shared memory, since 32 addresses out
 // of 8192 fall on 3.5 of a bank: about 5 tokens per cycle and SM, 16 us a row, and 256 rows are
-// two rows on most SMs. Then the questions, 5 to 8 us. One row is latency: 13.1 us, of them 2.3
+// two rows on most SMs. Then the questions, 5 to 8 us. One row is latency: 13.4 us, of them 2.3
 // the launch, 2.6 the reads and counts of its eight CTAs, 2.2 their addition, 1.9 the weights,
 // 0.7 each question, 1.5 the choice's way to the others and their look for the token. Rejected:
 // 17 bins of two binades per thread walked one by one (14.6 us), one warp that asks for all
@@ -257,7 +257,9 @@ __device__ __forceinline__ void remote_store(uint32_t at, int v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
 }
 
-// Running counts and weights of the threads' bins: (c, w) of thread t's, into upto_*.
+// Running counts and weights of the threads' bins: (c, w) of thread t's, into upto_*. The
+// warps' sums are added in their order, so that the weight does not fall from one warp's end
+// to the next one's; within a warp it may, by a rounding.
 __device__ __forceinline__ void running(int c, double w, Shared &s) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 #pragma unroll
@@ -268,20 +270,13 @@ __device__ __forceinline__ void running(int c, double w, Shared &s) {
     }
     if (lane == 31) s.warp_count[warp] = c, s.warp_weight[warp] = w;
     __syncthreads();
-    int cs = lane < kSampleWarps ? s.warp_count[lane] : 0;
-    double ws = lane < kSampleWarps ? s.warp_weight[lane] : 0.0;
+    int cs = 0;
+    double ws = 0.0;
 #pragma unroll
-    for (int d = 1; d < kSampleWarps; d <<= 1) {
-        const int uc = __shfl_up_sync(0xffffffffu, cs, d);
-        const double uw = __shfl_up_sync(0xffffffffu, ws, d);
-        if (lane >= d) cs += uc, ws += uw;
-    }
-    if (warp > 0) {
-        c += __shfl_sync(0xffffffffu, cs, warp - 1);
-        w += __shfl_sync(0xffffffffu, ws, warp - 1);
-    }
-    s.upto_count[tid] = c;
-    s.upto_weight[tid] = w;
+    for (int i = 0; i < kSampleWarps - 1; ++i)
+        if (i < warp) cs += s.warp_count[i], ws += s.warp_weight[i];
+    s.upto_count[tid] = cs + c;
+    s.upto_weight[tid] = ws + w;
     __syncthreads();
 }
 
@@ -387,7 +382,9 @@ __device__ __noinline__ void choose_slowly(const RowParams &r, const Row &row, S
         const double mine = from + (tid ? s.upto_weight[tid - 1] : 0.0);
         if (tid == 0) s.number = INT_MAX;
         __syncthreads();
-        if (!reached(mine) && reached(from + s.upto_weight[tid])) {
+        // the first of the threads that reach it: the running weight may fall by a rounding
+        const int count = s.upto_count[tid] - (tid ? s.upto_count[tid - 1] : 0);
+        if (count && reached(from + s.upto_weight[tid])) {
             int c = s.before[w].count + (tid ? s.upto_count[tid - 1] : 0), last = c;
             double sum = mine;
             for (int i = 0; i < kWindowOwn; ++i) {
@@ -403,12 +400,12 @@ __device__ __noinline__ void choose_slowly(const RowParams &r, const Row &row, S
                 c += h;
                 sum += h * each;
             }
-            s.number = last;
+            atomicMin(&s.number, last);
         }
         __syncthreads();
         const int n = s.number;
         __syncthreads();
-        return n;
+        return n == INT_MAX && reached(s.before[w + 1].weight) ? s.before[w + 1].count - 1 : n;
     };
     const int all = s.before[kWindows].count;
     int keep = all;
@@ -577,11 +574,14 @@ __device__ __forceinline__ void choose(const RowParams &r, Shared &s) {
         };
         // an answer stays while the next one is worked out, so one barrier is enough
         Shared::Answer &answer = s.answers[turn ^= 1];
-        const uint32_t here = __ballot_sync(
-            0xffffffffu, c > 0 && (from_c == 0 || !reached(from_c, from_w)) &&
-                             (reached(upto_c, upto_w) || upto_c == all));
-        if (here) {
-            const int from = __ffs(here) - 1;
+        // the warp at whose end it is reached and before which it was not: there is one
+        const uint32_t by_end =
+            __ballot_sync(0xffffffffu, upto_c == all || reached(upto_c, upto_w));
+        const uint32_t before = __ballot_sync(
+            0xffffffffu, from_c > 0 && (from_c == all || reached(from_c, from_w)));
+        if (by_end >> 31 && !(before & 1)) {
+            const uint32_t some = __ballot_sync(0xffffffffu, c > 0), first = some & by_end;
+            const int from = first ? __ffs(first) - 1 : 31 - __clz(some);
             const Seen seen = look(tid - lane + from);
             const int h = seen.h;
             int count = h;
@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleParams 
     if (tid < kRanges) s.in_range[tid] = kLastRank;
     if (tid == 0) s.best = INT_MAX, s.inv = 1.0 / (double)with.temperature;
     __syncthreads();
-    if (ctas > 1) cluster_arrive();
+    if (ctas > 1 && cta != 0) cluster_arrive();
     const uint32_t hist = smem_u32(s.hist), trash = (kBins + lane) * 4;
     // one word of a chunk: its largest logits go into `most`, its tokens into the histogram
     auto take = [&](const uint4 &u, uint32_t &most) {
@@ -709,7 +709,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleParams 
     }
     __syncthreads();
     if (ctas > 1) {
-        cluster_wait();  // the first CTA's histogram was zero before this
+        // The first CTA has counted before the others add to its bins two at a time: its own
+        // 32-bit atomics and these never meet. (One bin at a time, without this order: 64 rows
+        // of 151936 22.8 us, 21.9 like this; one row 13.2, 13.4.)
+        if (cta == 0) cluster_arrive();
+        cluster_wait();
         if (cta != 0) {
             const uint32_t to = in_cta(s.hist, 0);
             if (!greedy) {
