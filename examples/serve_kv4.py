@@ -102,8 +102,8 @@ class Engine:
                            k_scale=self.K_SCALE, v_scale=self.V_SCALE, workspace=self.ws,
                            dev_status=self.status)
 
-    def choose(self, out, logits):
-        """The next token of each row."""
+    def choose(self, out, logits, first=0):
+        """The next token of each row; row 0 is request `first`'s."""
         L.argmax(out, logits)
 
     def _append(self, qkv, positions, slot_map, layer):
@@ -180,12 +180,12 @@ class Engine:
         self.lens[which.long()] = 0
 
 
-def first_token(engine, hidden):
+def first_token(engine, hidden, request):
     s = engine.stack
     logits = torch.empty(1, s.embed.shape[0], dtype=torch.bfloat16, device="cuda")
     L.proj_gemm(logits, hidden[-1:].contiguous(), s.embed)
     out = torch.zeros(1, dtype=torch.int32, device="cuda")
-    engine.choose(out, logits)
+    engine.choose(out, logits, request)
     return out
 
 
@@ -195,7 +195,7 @@ def generate(engine, prompts, steps, chunk=256, graph=True):
     for slot, p in enumerate(prompts):
         for at in range(0, p.shape[0], chunk):
             hidden = engine.prompt(slot, p[at:at + chunk], at)
-        nxt.append(first_token(engine, hidden))
+        nxt.append(first_token(engine, hidden, slot))
     step = engine.start_decode(list(range(len(prompts))), torch.cat(nxt))
     got = [engine.token.clone()]
     if graph:

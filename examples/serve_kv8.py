@@ -16,12 +16,21 @@ import time
 import torch
 
 import serve_kv4 as base
-from serve_kv4 import PAGE, L, Stack, generate
+from serve_kv4 import PAGE, L, generate
+
+
+class Stack(base.Stack):
+    """With a small embedding, so that the tied head's logits leave a draw a choice."""
+
+    def __init__(self, *args, **kwargs):
+        super().__init__(*args, **kwargs)
+        self.embed *= 0.07
 
 
 class Engine(base.Engine):
-    """Up to `slots` sequences over one 8-bit pool; row i of a batch samples with entry i of
-    the parameters (None: temperature 1 and no filter)."""
+    """Up to `slots` sequences over one 8-bit pool; request i samples with entry i of the
+    parameters (None: temperature 1 and no filter). The random numbers begin anew after
+    max_steps choices."""
 
     def __init__(self, stack, slots=8, max_len=1024, num_blocks=256, temperature=None, top_k=None,
                  top_p=None, min_p=None, seed=0, max_steps=4096):
@@ -64,11 +73,12 @@ class Engine(base.Engine):
                            self.step_rows, self.batch_lens, max_context_len=self.width * PAGE,
                            workspace=self.ws, dev_status=self.status)
 
-    def choose(self, out, logits):
-        b = logits.shape[0]
-        rand = self.numbers.index_select(0, self.step_no)[0]
-        L.sample(out, logits, rand, **{k: None if v is None else v[:b] for k, v in self.params.items()})
-        self.step_no += 1
+    def choose(self, out, logits, first=0):
+        rows = slice(first, first + logits.shape[0])
+        rand = self.numbers.index_select(0, self.step_no)[0, rows]
+        L.sample(out, logits, rand,
+                 **{k: None if v is None else v[rows] for k, v in self.params.items()})
+        self.step_no.add_(1).remainder_(self.numbers.shape[0])
 
 
 def main():

@@ -53,27 +53,34 @@ def test_graph_steps_equal_eager_steps_and_pages_come_back():
     assert torch.equal(pools[0], pools[1])
 
 
-def test_the_chosen_tokens_are_the_formulas():
-    """Each step's tokens from that step's logits and numbers."""
+@pytest.mark.parametrize("max_steps", [4096, 5])
+def test_the_chosen_tokens_are_the_formulas(max_steps):
+    """Each step's tokens from that step's logits and numbers, a prompt's first token with its own
+    request's parameters; the numbers begin anew after the last."""
     import serve_kv8 as S
     stack = S.Stack(layers=1)
-    e = S.Engine(stack, slots=4, **PARAMS)
+    e = S.Engine(stack, slots=4, max_steps=max_steps, **PARAMS)
     seen = []
     chosen = e.choose
 
-    def record(out, logits):
+    def record(out, logits, first=0):
         n = int(e.step_no.item())
-        chosen(out, logits)
-        seen.append((n, from_device(logits), out.cpu().numpy().copy()))
+        chosen(out, logits, first)
+        seen.append((n, first, from_device(logits), out.cpu().numpy().copy()))
     e.choose = record
     S.generate(e, prompts_of(stack, (5, 33, 64, 200)), 12, graph=False)
     assert len(seen) == 4 + 11
+    assert [first for _, first, _, _ in seen] == [0, 1, 2, 3] + [0] * 11
+    assert [n for n, _, _, _ in seen] == [i % max_steps for i in range(15)]
     numbers = e.numbers.cpu().numpy()
-    for n, logits, out in seen:
-        for row, bits in enumerate(logits):
+    drawn = np.array([out - np.argmax(R.bf16_f64(logits), 1) for _, _, logits, out in seen[4:]])
+    # row 0 is greedy, and the others' draws are draws (one row may take its likeliest each time)
+    assert not drawn[:, 0].any() and drawn[:, 1:].any()
+    for n, first, logits, out in seen:
+        for row, bits in enumerate(logits, first):
             par = {k: v[row] if k == "top_k" else float(np.float32(v[row])) for k, v in PARAMS.items()}
             want, margin = choose(R.bf16_f64(bits), float(numbers[n, row]), **par)
-            assert out[row] == want or margin < 1e-12
+            assert out[row - first] == want or margin < 1e-12
 
 
 def test_prompt_chunks_and_decode_agree():
@@ -81,7 +88,7 @@ def test_prompt_chunks_and_decode_agree():
     tokens in the end), and its last token's attention over the 8-bit cache is the same through
     unpack + prefill and through decode."""
     import serve_kv8 as S
-    stack = S.Stack(layers=1)
+    stack = S.base.Stack(layers=1)
     tokens = prompts_of(stack, (150,))[0]
     whole, parts = S.Engine(stack), S.Engine(stack)
     a = whole.prompt(0, tokens)
