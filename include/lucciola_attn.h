@@ -79,8 +79,9 @@ const char *lc_version(void);
  *     then not write the context lengths/positions, the block tables, the
  *     biases, the RoPE tables, or this layer's cached K/V (a decode step's QKV
  *     projection or another layer's attention qualifies).
- * lc_paged_decode_kv4 follows the mode too; in mode 2 it reads nothing but the
- * context lengths before the wait.
+ * lc_paged_decode_kv4 and lc_paged_decode_kv8 follow the mode too; in mode 2 they read
+ * nothing but the context lengths before the wait. lc_qk_norm_rope_append_kv8 lets such a
+ * decode start early.
  * Returns the previous mode, or -1 for an invalid mode. */
 int lc_set_dependent_launch(int mode);
 

@@ -461,6 +461,9 @@ __global__ void __launch_bounds__(kNormRopeThreads, kNormRopeCtas)
     constexpr int kLanes = HD / 16, kHeads = 32 / kLanes, kHalf = HD / 2;
     constexpr int kWarps = kNormRopeThreads / 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // A decode launched to start early waits for the rows itself. (One sequence of 1024 tokens, 14/2
+    // heads of 64, append and decode in mode 2: 8.3 us, 9.3 us without; 9.4 us in mode 0.)
+    griddep_launch_dependents();
     if ((int)blockIdx.x < kv_blocks) {
         const int kinds = 2 * p.num_kv_heads;
         const uint32_t task = blockIdx.x * kWarps + warp;
