@@ -39,6 +39,7 @@ struct Kv4 {
     // 24, 18.3 with none; 256 of 100 .. 300: 15.2, 15.3, 19.5; 32 of 8192, 28/4 heads of 128:
     // 37.5, 37.4, 38.9, and 38.1 with 36.)
     static constexpr int kEdgeUnits = 32;
+    static constexpr int kAlonePages = 0;
     static constexpr bool kPageScales = false;
     static constexpr int kSteps = D / 16, kWords = D / 32;  // code words per token and lane (K)
 

@@ -36,12 +36,15 @@ struct Kv8 {
     static constexpr int kGroup = D == 64 || NT == 2 ? 2 : 1;
     static constexpr int kStages = 2;  // what fits beside a second CTA
     // Pages per CTA at least. (One sequence of 203 tokens: 5.6 us, 6.2 us with 8 or 12; of 1024
-    // tokens, 14/2 heads of 64: 6.4 us, 7.6 us with 24, which takes 10.3 us for one of 12345, 28/4
-    // heads of 128, where this takes 11.3 us.)
+    // tokens, 14/2 heads of 64: 6.4 us, 7.6 us with 24.)
     static constexpr int kMinPages = 16;
     // (64 sequences of 256 .. 4096 tokens, 14/2 heads of 64: 13.2 us, 14.0 us with 20, 13.8 with
     // 60; 256 of 100 .. 300, 28/4 heads of 128: 24.4 us, 26.7 us with 8, 24.8 with 20, 25.8 with 48.)
     static constexpr int kEdgeUnits = D == 64 ? 48 : 24;
+    // (One sequence of 8192 tokens, 64/8 heads of 128: 10.2 us in 128 CTAs of 32 pages, 11.6 us in
+    // 256 of 16; of 12345, 28/4 heads: 10.3 us in 132 of 24, 11.0 us in 196 of 16; of 16384, where
+    // 128 have 32 each, 11.2 us, 11.1 us in 256.)
+    static constexpr int kAlonePages = 32;
     static constexpr bool kPageScales = true;
     static constexpr int kSteps = D / 16, kWords = D / 16;  // words per token and lane (K)
 

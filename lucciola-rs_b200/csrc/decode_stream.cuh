@@ -78,6 +78,7 @@ struct DecodeParams {
     float v_scale;     // V's factor, or 1
     int pdl_mode;
     int seg_ctas;   // CTAs of the grid per segment, when there is one sequence
+    int seg_alone;  // as many as have an SM each, if an SM takes several
     int *ws_cnt;    // [CTAs][kCols] arrivals, at the CTA of a segment's first piece
     int *ws_group;  // [2][CTAs][kCols] arrivals of a group, at the CTA of its first piece
     float2 *ws_ml;  // [pieces][kCols] m, l
@@ -211,6 +212,13 @@ __device__ __forceinline__ int ctas_of(const DecodeParams &p, int total, int pag
     // round on a full grid does as well or better (100000 tokens, 64/8 heads: 32.4 us, 33.3
     // us in rounds).
     if (p.batch == 1 && p.seg_ctas > 0) {
+        // Before SMs get a second one, CTAs take up to F::kAlonePages.
+        if constexpr (F::kAlonePages > 0) {
+#pragma unroll
+            for (int n = F::kMinPages; n <= F::kAlonePages; n += 8)
+                if (pages <= n * p.seg_alone)
+                    return max(1, (int)((unsigned)(pages + n - 1) / (unsigned)n) * p.seg_per_seq);
+        }
         int each = p.seg_ctas;
         for (int r = 1; r <= 4; ++r) {
             if (pages > F::kMinPages * r * p.seg_ctas) continue;
@@ -1202,6 +1210,7 @@ int launch(DecodeParams p, int max_context_len, cudaStream_t stream) {
     }
     grid = std::max<int64_t>(grid, 1);
     p.seg_ctas = (int)(grid / p.seg_per_seq);
+    p.seg_alone = C::kCtasPerSm > 1 ? std::min(p.seg_ctas, sm_count() / p.seg_per_seq) : 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(C::kThreads);
