@@ -494,6 +494,16 @@ __device__ __forceinline__ bool last_piece(const DecodeParams &p, int c0, int pi
     return true;
 }
 
+// 16 bytes from L2, after the waits before it.
+__device__ __forceinline__ uint4 load_l2(const void *src) {
+    uint4 v;
+    asm volatile("ld.global.cg.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(src)
+                 : "memory");
+    return v;
+}
+
 __device__ __forceinline__ void cp_async16(void *dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src)
                  : "memory");
@@ -810,6 +820,9 @@ __global__ void __launch_bounds__(Cfg<F, NT>::kThreads, Cfg<F, NT>::kCtasPerSm)
         // q: column c of the slice is query token c / group, head c % group. Lane (g, t)
         // holds a quarter of column g's dims, as the products need them. A chunk's rows
         // are read while the chunk before it is prepared and the one before that joined.
+        // From L2 and not through the read-only path (__ldg): a launch that starts early is
+        // there while the append still writes these rows, and griddep_wait orders ordinary
+        // reads alone; L1 may hold neighbours of q from before that, where q lies over qkv.
         uint4 raw[HD / 32];
         auto read_q = [&]() {
             const int kvh = kv_head(p, cw.seg);
@@ -819,7 +832,7 @@ __global__ void __launch_bounds__(Cfg<F, NT>::kThreads, Cfg<F, NT>::kCtasPerSm)
                               (int64_t)(kvh * p.group + h) * HD + F::q_dim(t, 0);
 #pragma unroll
             for (int k = 0; k < HD / 32; ++k)
-                raw[k] = col < p.cols ? __ldg(reinterpret_cast<const uint4 *>(src + (F::q_dim(0, k) - F::q_dim(0, 0))))
+                raw[k] = col < p.cols ? load_l2(src + (F::q_dim(0, k) - F::q_dim(0, 0)))
                                       : make_uint4(0, 0, 0, 0);
         };
         read_q();
