@@ -639,7 +639,7 @@ int lc_sample(const void *logits, int64_t row_stride, int vocab, int batch,
 /* The same calls with their arguments in one block of num_words 8-byte words, in order:
  * integers sign-extended, pointers, floats as doubles. For bindings whose foreign calls cost
  * by the argument. Status of the call; LC_ERR_INVALID_ARGUMENT for another entry or number
- * of words. */
+ * of words, or an integer that its parameter cannot hold. */
 enum lc_packed_entry {
     LC_PACKED_QK_NORM_ROPE_APPEND_KV8 = 0,
     LC_PACKED_UNPACK_KV8 = 1,

@@ -4,6 +4,7 @@
 // launches are 5 to 10 us of GPU work each.
 #include <cstdint>
 #include <cstring>
+#include <tuple>
 #include <type_traits>
 #include <utility>
 
@@ -11,8 +12,9 @@
 
 namespace {
 
+// A word as the parameter's type; `fits` is cleared where an int cannot hold it.
 template <class T>
-T from_word(const unsigned char *w) {
+T from_word(const unsigned char *w, bool &fits) {
     if constexpr (std::is_floating_point_v<T>) {
         double d;
         std::memcpy(&d, w, 8);
@@ -20,14 +22,20 @@ T from_word(const unsigned char *w) {
     } else {
         uint64_t u;
         std::memcpy(&u, w, 8);
-        if constexpr (std::is_pointer_v<T>) return reinterpret_cast<T>((uintptr_t)u);
-        else return (T)u;
+        if constexpr (std::is_pointer_v<T>) {
+            return reinterpret_cast<T>((uintptr_t)u);
+        } else {
+            if (std::is_same_v<T, int> && (int64_t)u != (int)u) fits = false;
+            return (T)u;
+        }
     }
 }
 
 template <class... A, size_t... I>
 int call(int (*f)(A...), const unsigned char *words, std::index_sequence<I...>) {
-    return f(from_word<A>(words + 8 * I)...);
+    bool fits = true;
+    const std::tuple<A...> args{from_word<A>(words + 8 * I, fits)...};
+    return fits ? std::apply(f, args) : LC_ERR_INVALID_ARGUMENT;
 }
 
 template <class... A>
