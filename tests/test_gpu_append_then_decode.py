@@ -94,3 +94,45 @@ def test_q_over_the_qkv_rows(batch, rows, hq, hkv, hd, mode):
     """In place, with rows an odd number of 16 bytes apart: neighbouring heads, which different
     warps read and write, share 32-byte sectors."""
     Passes(batch, rows, hq, hkv, hd, seed=batch + rows, pad=8).check(mode, True)
+
+
+@pytest.mark.parametrize("mode", [1, 2])
+@pytest.mark.parametrize("batch,rows,hq,hkv,hd,tokens", [
+    (1, 1, 14, 2, 64, 1), (6, 1, 28, 4, 128, 1), (64, 1, 14, 2, 64, 1), (300, 1, 8, 8, 64, 1),
+    (3, 40, 12, 2, 128, 1), (96, 70, 28, 4, 128, 1),
+    (8, 3, 64, 8, 128, 3), (5, 2, 14, 2, 64, 2),  # drafted tokens
+])
+def test_new_rows_in_every_pass(batch, rows, hq, hkv, hd, tokens, mode):
+    Passes(batch, rows, hq, hkv, hd, seed=batch + rows + tokens, tokens=tokens).check(mode, False)
+
+
+@pytest.mark.parametrize("mode", [1, 2])
+def test_new_rows_in_every_pass_of_a_graph(mode):
+    """The same as one captured graph, replayed from the pool's first state."""
+    hq, hkv, hd, batch = 14, 2, 64, 7
+    p = Passes(batch, 1, hq, hkv, hd, seed=3)
+    want, want_pool = p.run(0, False)
+    pool = p.pool.clone()
+    q = [torch.zeros(batch, hq * hd, dtype=torch.bfloat16, device="cuda") for _ in p.qkv]
+    out = [torch.zeros_like(x) for x in q]
+    ws = L.alloc_decode_kv8_workspace(batch, hq, hkv, hd)
+    graph = torch.cuda.CUDAGraph()
+    old = L.set_dependent_launch(mode)
+    try:
+        with torch.cuda.graph(graph):
+            for i in range(PASSES):
+                L.qk_norm_rope_append_kv8(q[i], p.qkv[i], p.pos[i], p.slot[i], p.cos, p.sin, pool,
+                                          p.nb, 1, 0, hq, hkv, hd, q_norm=p.norm, k_norm=p.norm)
+                L.paged_decode_kv8(out[i], q[i], pool, p.nb, 1, 0, hq, hkv, hd, p.tables, p.lens[i],
+                                   p.longest, workspace=ws)
+    finally:
+        L.set_dependent_launch(old)
+    for _ in range(3):
+        pool.copy_(p.pool)
+        for x in q + out:
+            x.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(q + out, want):
+            assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+        assert torch.equal(pool, want_pool)
