@@ -629,8 +629,11 @@ int lc_sample_top_p(const void *logits, int64_t row_stride, int vocab, int batch
  * running weight exceeds rand_vals[b] (in [0, 1)) times their whole weight. A temperature
  * that is not positive takes the first token of the order. 0xffffffff where no logit
  * exceeds -1e30. Weights and sums are in 64 bits: the choice does not depend on the
- * batch, and equals the formula's but where rand times the weight lies within 1e-12 of a
- * border. bf16 rows, any stride and alignment. One launch, no workspace. */
+ * batch, and equals the formula's but where one of its three comparisons is within
+ * rounding: a running weight against top_p or rand times the weight (1e-12 of that weight),
+ * or a token's weight against min_p (1e-12 of it). A top_p or min_p on such a border may
+ * keep one value's tokens more or fewer, and the draw is then among those kept. bf16 rows,
+ * any stride and alignment. One launch, no workspace. */
 int lc_sample(const void *logits, int64_t row_stride, int vocab, int batch,
               const float *temperature, const int *top_k, const float *top_p,
               const float *min_p, const float *rand_vals, unsigned *out_idx,
