@@ -80,8 +80,8 @@ const char *lc_version(void);
  *     biases, the RoPE tables, or this layer's cached K/V (a decode step's QKV
  *     projection or another layer's attention qualifies).
  * lc_paged_decode_kv4 and lc_paged_decode_kv8 follow the mode too; in mode 2 they read
- * nothing but the context lengths before the wait. lc_qk_norm_rope_append_kv8 lets such a
- * decode start early.
+ * nothing but the context lengths before the wait. lc_qk_norm_rope_append_kv8 lets the
+ * launch behind it start early where that follows the mode.
  * Returns the previous mode, or -1 for an invalid mode. */
 int lc_set_dependent_launch(int mode);
 
@@ -633,7 +633,9 @@ int lc_sample_top_p(const void *logits, int64_t row_stride, int vocab, int batch
  * rounding: a running weight against top_p or rand times the weight (1e-12 of that weight),
  * or a token's weight against min_p (1e-12 of it). A top_p or min_p on such a border may
  * keep one value's tokens more or fewer, and the draw is then among those kept. bf16 rows,
- * any stride and alignment. One launch, no workspace. */
+ * any stride and alignment. One launch, no workspace. To bar tokens, -inf or the type's
+ * lowest value is quick; several finite logits of one sign beyond 2^10, or below 2^-22 in
+ * magnitude, are right but take a row ten times as long. */
 int lc_sample(const void *logits, int64_t row_stride, int vocab, int batch,
               const float *temperature, const int *top_k, const float *top_p,
               const float *min_p, const float *rand_vals, unsigned *out_idx,

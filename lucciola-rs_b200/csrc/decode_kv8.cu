@@ -39,11 +39,16 @@ struct Kv8 {
     // tokens, 14/2 heads of 64: 6.4 us, 7.6 us with 24.)
     static constexpr int kMinPages = 16;
     // (64 sequences of 256 .. 4096 tokens, 14/2 heads of 64: 13.2 us, 14.0 us with 20, 13.8 with
-    // 60; 256 of 100 .. 300, 28/4 heads of 128: 24.4 us, 26.7 us with 8, 24.8 with 20, 25.8 with 48.)
+    // 60; 256 of 100 .. 300, 28/4 heads of 128: 24.4 us, 26.7 us with 8, 24.8 with 20, 25.8 with 48.
+    // The other way round, 24 for 64 dims: 64 of 0 .. 4096 with their append 16.9 us, 16.0 so; 16 of 500 ..
+    // 16000, 14/2 heads, 14.3 and 13.7; but 64 of 256 .. 4096, 32/8 heads, 31.1 and 33.1. 48 for
+    // 128: 64 of 256 .. 4096, 28/4 heads, 31.4 us, 30.2 so; 16 of 500 .. 16000, 12/2 heads, 17.7 and 17.8.)
     static constexpr int kEdgeUnits = D == 64 ? 48 : 24;
     // (One sequence of 8192 tokens, 64/8 heads of 128: 10.2 us in 128 CTAs of 32 pages, 11.6 us in
     // 256 of 16; of 12345, 28/4 heads: 10.3 us in 132 of 24, 11.0 us in 196 of 16; of 16384, where
-    // 128 have 32 each, 11.2 us, 11.1 us in 256.)
+    // 128 have 32 each, 11.2 us, 11.1 us in 256. Heads of 64 gain where there are many: of 6917
+    // tokens, 32/8 heads, 9.1 us, 10.0 us without; of 5957, 12/12 heads, 9.1 and 9.8; of 33157, 14/2
+    // heads, 10.7 and 10.2; of 16581, 28/4 heads, 10.5 and 9.9.)
     static constexpr int kAlonePages = 32;
     static constexpr bool kPageScales = true;
     static constexpr int kSteps = D / 16, kWords = D / 16;  // words per token and lane (K)

@@ -26,8 +26,9 @@
 // with a warp per turn).
 //
 // Bounds. Those 16384 rows of 128-dim heads now take 27.9 us: 143 MB at 5.1 TB/s, 78 %
-// of a device copy's rate. What is missing are issue slots, the products and sums not
-// being contracted (counting rows and heads on without a division: 29.6 us before).
+// of a device copy's rate. What is missing are issue slots (counting rows and heads on
+// without a division: 29.6 us before); contracted products and sums would save 12
+// instructions of a turn, which has some hundreds.
 // Into the 4-bit pool (8192 rows of 28/4 heads, 33 us, 66 %) the quotients of K and V
 // come on top: 69 % of the issue slots, with the packed operations at half rate. 32
 // rows are launch and latency: 2.4 us.
@@ -277,16 +278,19 @@ int launch(const NormRopeParams &p, int head_dim, cudaStream_t stream) {
 // ---------------------------------------------------------------- 8-bit pool --
 // A page of a kv head has one scale for its 16 tokens, so the rows that a call adds to a
 // page are one piece of work: a run, adjacent rows of one page with rising offsets. The
-// warp that has the run takes K or V of one head: the rows' values stay in its registers,
-// their largest magnitude and the page's old scale give the new one, and where that grew
-// the page's other tokens are moved to it. Run starts are found from the slots: a warp
-// looks at `window` rows and works on the runs that start there.
+// warp that has the run takes K or V of one head: it goes through the rows once for their
+// largest magnitude, which with the page's old scale gives the new one, and once more for
+// their codes (append_run); where the scale grew the page's other tokens are moved to it.
+// Run starts are found from the slots: a warp looks at `window` rows and works on the runs
+// that start there.
 //
 // The first kv_blocks CTAs do so, the others the queries, as above.
 //
 // Bounds. 8192 rows of 28/4 heads of 128: 36 us for 147 MB, 62 % of a device copy's rate. 65 %
-// of the issue slots are taken, most of them by the queries' uncontracted products and sums, as
-// in the other pools' kernel. Rejected: cos, sin and the norm's weights kept for a row's
+// of the issue slots are taken: 23.05 M instructions, 313 for four heads of a row, which go to
+// unpacking rows and norm weights, to addresses, and to K's and V's second time (three of a
+// page's four chunks are loaded and unpacked twice, K's normed and rotated twice). Contracted
+// products and sums would save 12 of the 313. Rejected: cos, sin and the norm's weights kept for a row's
 // queries (48.0 us with the unpacking, 43.9 so: the registers spill), 5 or 6 CTAs per SM (47.6,
 // 45.9). 24 rows are launch and latency: slot -> scale beside the row, 5.7 us from a cold L2.
 constexpr int kMaxWindow = 8;  // a run's 16 rows from the last of 8 end within a warp's lanes

@@ -20,7 +20,10 @@
 // one for each of the four ranges beside them, 8197 in all: 33 KB of shared memory, where all
 // 65536 would fill more than an SM has. In such a range a row may have one token (a tiny logit
 // turns up in one of 100 rows of 151936 normal ones); a row with more in one takes the slow
-// way, window by window of the values.
+// way, window by window of the values, in one CTA. So does a row whose mask is finite and above
+// -1e30: with a sixteenth of 151936 tokens at -1e4, -65504 or -1e9 one row takes 213 us, 64
+// rows 315 to 319 and 256 rows 398, against 14.0, 23.4 and 48.4 us with -inf in their place
+// (the type's lowest value is as quick); with two tiny logits in every row 209, 304 to 309, 359.
 //
 // Bounds. 256 rows of 151936 logits (78 MB, 12 us at a device copy's rate): 47.5 us. Counting
 // takes 12 instructions for 32 tokens, and 3.75 cycles of shared memory, since 32 addresses out
