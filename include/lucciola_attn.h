@@ -634,8 +634,8 @@ int lc_sample_top_p(const void *logits, int64_t row_stride, int vocab, int batch
  * or a token's weight against min_p (1e-12 of it). A top_p or min_p on such a border may
  * keep one value's tokens more or fewer, and the draw is then among those kept. bf16 rows,
  * any stride and alignment. One launch, no workspace. To bar tokens, -inf or the type's
- * lowest value is quick; several finite logits of one sign beyond 2^10, or below 2^-22 in
- * magnitude, are right but take a row ten times as long. */
+ * lowest value is quick; several finite logits of one sign from 2^10 on, or below 2^-22 in
+ * magnitude but not zero, are right but take a row about ten times as long. */
 int lc_sample(const void *logits, int64_t row_stride, int vocab, int batch,
               const float *temperature, const int *top_k, const float *top_p,
               const float *min_p, const float *rand_vals, unsigned *out_idx,
